@@ -1,0 +1,463 @@
+"""The low-bit operators of the student's training and serving paths, measured against their plain forms.
+
+Operators: the AdamW step over many tensors (f32 states, or 8-bit block-scaled states with stochastic
+rounding), MXFP4 quantisation (and back) of rows, gathered rows or pair products, and the MXFP4 product
+y = act(Q(x) Q(W)^T + b).
+
+  AdamW     t = step + 1, g' = c g with c the clip coefficient of the tensor's group,
+            m' = b1 m + (1 - b1) g',  v' = b2 v + (1 - b2) g'^2,
+            p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps).
+  8 bits    per 32 consecutive elements of a tensor one power of two 2^k (byte k + 127): m as E4M3 codes
+            (largest 448), r = sqrt(v) as unsigned codes of 4 exponent and 4 mantissa bits, bias 7 (largest
+            496); k is the least that holds the block's largest value.  A value goes to the code below or
+            above it with the probability that keeps the mean of m, and of v = r^2, where it was: up where
+            u < (distance to the lower code) / (distance between the codes), u = (w + 1/2) / 65536.
+            w: 16 bits of Philox4x32-10, counter (element / 8, 65536 t + tensor), word (element mod 8) / 2,
+            half element mod 2; its bytes swapped for v.
+  MXFP4     per 32 consecutive values of a row one power of two 2^e, e = floor(log2 max|x|) - 2 (byte
+            e + 127), E2M1 codes of x / 2^e rounded to nearest, ties to even, saturated at 6.  Rows are
+            padded with zeros to a multiple of 128 values; the low half of a byte is the even element.
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+LR, BETA1, BETA2, EPS, DECAY, MAX_NORM = 0.005, 0.9, 0.999, 1e-8, 0.01, 1.0
+NODES, CHUNK = 235868, 1 << 18        # ogbl-collab's nodes; the edges that the scorer takes at a time
+
+
+# ---------------------------------------------------------------- cases
+def listed():
+    return [
+        # a Cora student's training step: 1433 keywords, two layers of 256, a two-layer predictor
+        {"name": "adamw32_cora", "op": "adamw", "bits": 32, "layers": 2, "inputs": 1433, "hidden": 256, "grad": "f32",
+         "copy": False, "step": 40},
+        # the widest student of the sweeps on the physics features, bf16 working copies beside the f32 weights
+        {"name": "adamw32_physics_2048", "op": "adamw", "bits": 32, "layers": 3, "inputs": 8415, "hidden": 2048,
+         "grad": "f32", "copy": True, "step": 1500},
+        # the Cora student with its moments in 8 bits
+        {"name": "adamw8_cora", "op": "adamw", "bits": 8, "layers": 2, "inputs": 1433, "hidden": 256, "grad": "f32",
+         "copy": False, "step": 40},
+        # the collab student (hidden 1024, three layers) with gradients that a bf16 backward leaves
+        {"name": "adamw8_collab_bf16", "op": "adamw", "bits": 8, "layers": 3, "inputs": 128, "hidden": 1024,
+         "grad": "bf16", "copy": True, "step": 7},
+        # the widest student again, in 8 bits
+        {"name": "adamw8_physics_2048", "op": "adamw", "bits": 8, "layers": 3, "inputs": 8415, "hidden": 2048,
+         "grad": "f32", "copy": True, "step": 1500},
+        # Cora's node features before the first layer, an odd width
+        {"name": "quantize_cora_f32", "op": "quantize", "rows": 2708, "cols": 1433, "type": "f32", "pairs": False},
+        # one scorer chunk's pair products h[e0] * h[e1] of collab embeddings
+        {"name": "quantize_pairs_bf16", "op": "quantize", "rows": CHUNK, "cols": 1024, "type": "bf16", "pairs": True},
+        # one link scored: a single row through a hidden layer
+        {"name": "product_one_link", "op": "product", "rows": 1, "cols": 1024, "outs": 1024, "type": "bf16",
+         "out": "bf16", "relu": True},
+        # a node's few dozen candidates, odd sizes, f32 throughout
+        {"name": "product_candidates_f32", "op": "product", "rows": 47, "cols": 1433, "outs": 257, "type": "f32",
+         "out": "f32", "relu": False},
+        # all collab nodes through the student's first layer
+        {"name": "product_collab_first", "op": "product", "rows": NODES, "cols": 128, "outs": 1024, "type": "bf16",
+         "out": "bf16", "relu": True},
+        # a hidden layer that hands MXFP4 rows to the next one
+        {"name": "product_chain_mx4", "op": "product", "rows": 20000, "cols": 1024, "outs": 1024, "type": "mx4",
+         "out": "mx4", "relu": True},
+        # a scorer chunk through a wide hidden layer, rows already in MXFP4
+        {"name": "product_chunk_2048", "op": "product", "rows": CHUNK, "cols": 2048, "outs": 2048, "type": "mx4",
+         "out": "bf16", "relu": True},
+    ]
+
+
+def _spread(rng, lo, hi):
+    return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    op = rng.choice(["adamw", "adamw", "quantize", "product", "product", "product"])
+    if op == "adamw":
+        while True:
+            c = {"op": op, "bits": rng.choice([32, 8]), "layers": rng.randint(1, 4), "inputs": _spread(rng, 16, 8500),
+                 "hidden": _spread(rng, 32, 2200), "grad": rng.choice(["f32", "bf16"]), "copy": rng.random() < 0.5,
+                 "step": _spread(rng, 1, 20000) - 1}
+            if sum(_numels(c)) <= sum(_numels(listed()[1])):
+                return c
+    if op == "quantize":
+        while True:
+            c = {"op": op, "rows": _spread(rng, 1, CHUNK), "cols": _spread(rng, 1, 8500),
+                 "type": rng.choice(["f32", "bf16"]), "pairs": rng.random() < 0.5}
+            if c["rows"] * c["cols"] <= CHUNK * 1024:
+                return c
+    while True:
+        c = {"op": op, "rows": _spread(rng, 1, CHUNK), "cols": _spread(rng, 16, 8500), "outs": _spread(rng, 8, 2200),
+             "type": rng.choice(["bf16", "f32", "mx4"]), "out": rng.choice(["bf16", "f32", "mx4"]),
+             "relu": rng.random() < 0.5}
+        if c["rows"] * max(c["cols"], c["outs"]) <= CHUNK * 1024:
+            return c
+
+
+def _numels(c):
+    """The tensors of a student of `layers` linear layers and its predictor, weights and biases."""
+    h, n = c["hidden"], []
+    for k in range(c["layers"]):
+        n += [(c["inputs"] if k == 0 else h) * h, h]
+    for k in range(max(1, c["layers"] - 1)):
+        n += [h * h, h]
+    return n + [h, 1]
+
+
+def _split(c):
+    """The number of tensors in the first clip group (the student's)."""
+    return 2 * c["layers"]
+
+
+def _padded(n):
+    return (n + 63) // 64 * 64
+
+
+def work(c):
+    if c["op"] == "adamw":
+        n, g = sum(_numels(c)), 4 if c["grad"] == "f32" else 2
+        state = 16 if c["bits"] == 32 else 2 + 2 / 32 + 4     # f32 read and written; codes read, values written
+        return {"bytes": n * (8 + g + state + (2 if c["copy"] else 0)), "flops": 14 * n}
+    kp = (c["cols"] + 127) // 128 * 128
+    size = {"f32": 4.0, "bf16": 2.0, "mx4": 17 / 32}
+    if c["op"] == "quantize":
+        n = c["rows"] * c["cols"]
+        # pairs: each embedding row that is used is read once, at least
+        read = n * size[c["type"]] if not c["pairs"] else min(2 * c["rows"], NODES) * c["cols"] * size[c["type"]] + 8 * c["rows"]
+        return {"bytes": read + 2 * n, "flops": 4 * n}
+    m, k, n = c["rows"], c["cols"], c["outs"]
+    out = 2.0 if c["out"] == "mx4" else size[c["out"]]
+    return {"bytes": m * (kp if c["type"] == "mx4" else k) * size[c["type"]] + n * kp * 17 / 32 + 4 * n + m * n * out,
+            "flops": 2.0 * m * n * k}
+
+
+# ---------------------------------------------------------------- inputs
+_TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "mx4": torch.bfloat16}
+
+
+def _llp(name):
+    at = os.path.join(os.getcwd(), "linkless-link-prediction_amd")
+    if at not in sys.path:
+        sys.path.insert(0, at)
+    return __import__(name)
+
+
+def prepare(c, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=g, device="cuda")
+
+    s = {"case": c}
+    if c["op"] == "adamw":
+        return _prepare_adamw(s, c, seed, normal)
+    if c["op"] == "quantize":
+        r, k, t = c["rows"], c["cols"], _TYPES[c["type"]]
+        if c["pairs"]:
+            nodes = min(NODES, 2 * r)
+            s["h"] = (normal(nodes, k) * 0.3).to(t)
+            s["e0"], s["e1"] = (torch.randint(0, nodes, (r,), generator=g, device="cuda", dtype=torch.int32) for _ in "ab")
+        else:
+            s["x"] = normal(r, k).mul_(0.5).to(t)
+        return s
+    m, k, n = c["rows"], c["cols"], c["outs"]
+    x = normal(m, k).relu_().mul_(0.4).to(_TYPES[c["type"]])      # a hidden layer's input: half zeros
+    s["x"] = _pack(*_mx4(x.float())) if c["type"] == "mx4" else x
+    s["w"] = _pack(*_mx4(normal(n, k) / math.sqrt(k)))
+    s["b"] = normal(n) * 0.1
+    if own:
+        mx = _llp("llp_mx")
+        s["w"] = mx.MX4(*s["w"], k)
+        s["x"] = mx.MX4(*s["x"], k) if c["type"] == "mx4" else s["x"]
+    return s
+
+
+def _prepare_adamw(s, c, seed, normal):
+    ns = _numels(c)
+    at = [0]
+    for n in ns:
+        at.append(at[-1] + _padded(n))
+    total, dev = at[-1], "cuda"
+    live = torch.zeros(total, device=dev)
+    s["tensor"] = torch.zeros(total // 8, dtype=torch.int64, device=dev)      # of each eight elements: the tensor,
+    s["eight"] = torch.zeros(total // 8, dtype=torch.int64, device=dev)       # and which eight of it
+    for i, (o, n) in enumerate(zip(at, ns)):
+        live[o:o + n] = 1
+        s["tensor"][o // 8:(o + _padded(n)) // 8] = i
+        s["eight"][o // 8:(o + _padded(n)) // 8] = torch.arange(_padded(n) // 8, device=dev)
+    p = normal(total) * 0.03 * live
+    size = torch.exp(normal(total)) * 1e-3 * live
+    grad = (normal(total) * size).to(_TYPES[c["grad"]])
+    m, r = normal(total) * size * 0.3, size * torch.exp(0.2 * normal(total))
+    s.update(p=p, grad=grad, split=at[_split(c)], seed=seed * 7919 + 13,
+             step=torch.full((1,), c["step"], dtype=torch.int64, device=dev),
+             sumsq=torch.tensor([0.4, 2.9], device=dev))
+    if c["bits"] == 32:
+        s.update(m=m, v=r * r)
+    else:
+        s["m"], s["ms"] = _nearest8(m, 3, 1.75)
+        s["v"], s["vs"] = _nearest8(r, 4, 1.9375)
+    out = {k: torch.zeros_like(s[k]) for k in ("p", "m", "v", "ms", "vs") if k in s}
+    if c["copy"]:
+        out["copy"] = torch.zeros(total, dtype=torch.bfloat16, device=dev)
+    if c["bits"] == 8:
+        out["m_value"] = torch.zeros(total, dtype=torch.bfloat16, device=dev)
+        out["v_value"] = torch.zeros(total, dtype=torch.bfloat16, device=dev)
+    s["out"] = out
+    if own:
+        def parts(flat, per=1):
+            return None if flat is None else [flat[o // per:o // per + -(-n // per)] for o, n in zip(at, ns)]
+
+        s["table"] = _llp("llp_optim").AdamWTable(
+            parts(p), parts(grad), parts(s["m"]), parts(s["v"]), exp_avg_scale=parts(s.get("ms"), 32),
+            exp_avg_sq_scale=parts(s.get("vs"), 32), groups=[int(i >= _split(c)) for i in range(len(ns))],
+            copies=parts(out.get("copy")),
+            out={"params": parts(out["p"]), "exp_avg": parts(out["m"]), "exp_avg_sq": parts(out["v"]),
+                 "exp_avg_scale": parts(out.get("ms"), 32), "exp_avg_sq_scale": parts(out.get("vs"), 32)},
+            values={"exp_avg": parts(out.get("m_value")), "exp_avg_sq": parts(out.get("v_value"))})
+    return s
+
+
+def _nearest8(x, bits, top):
+    """8-bit codes of each 32 values (E4M3 with a sign for bits = 3, unsigned with 4 mantissa bits for bits = 4), nearest."""
+    b = x.view(-1, 32)
+    f, e = torch.frexp(b.abs().amax(1))
+    k = torch.where(f * 2 <= top, e - 9, e - 8).clamp(-127, 127)
+    y = torch.ldexp(b.abs(), -k[:, None])
+    q = torch.ldexp(torch.ones_like(y), torch.frexp(y)[1].sub(1).clamp(min=-6) - bits)
+    code = _code8((y / q).round() * q, bits)
+    if bits == 3:
+        code = code + 128 * (b < 0)
+    return code.to(torch.uint8).view(-1), torch.where(f > 0, k + 127, torch.zeros_like(k)).to(torch.uint8)
+
+
+def _code8(y, bits):
+    """The code of a value y >= 0 that has one."""
+    e = torch.frexp(y)[1].sub(1).clamp(min=-6)
+    units = torch.ldexp(y, bits - e).to(torch.int32)
+    return (e + 6) * (1 << bits) + units
+
+
+# ---------------------------------------------------------------- the plain forms
+def run(s):
+    c = s["case"]
+    if c["op"] == "adamw":
+        return _own_adamw(s) if own else _plain_adamw(s)
+    if c["op"] == "quantize":
+        if own:
+            mx = _llp("llp_mx")
+            q = mx.quantize(s["h"], s["e0"], s["h"], s["e1"]) if c["pairs"] else mx.quantize(s["x"])
+            return mx.dequantize(q, torch.bfloat16)
+        x = s["h"][s["e0"].long()].float() * s["h"][s["e1"].long()].float() if c["pairs"] else s["x"].float()
+        return _unpack(*_pack(*_mx4(x)), c["cols"]).to(torch.bfloat16)
+    if own:
+        mx = _llp("llp_mx")
+        if c["out"] == "mx4":
+            return mx.dequantize(mx.linear(s["x"], s["w"], s["b"], relu=c["relu"], out_dtype="mx4"), torch.bfloat16)
+        return mx.linear(s["x"], s["w"], s["b"], relu=c["relu"], out_dtype=_TYPES[c["out"]])
+    k = c["cols"]
+    x = _unpack(*s["x"], k) if c["type"] == "mx4" else _unpack(*_pack(*_mx4(s["x"].float())), k)
+    y = x @ _unpack(*s["w"], k).t() + s["b"]
+    if c["relu"]:
+        y = y.clamp(min=0)
+    if c["out"] == "mx4":
+        return _unpack(*_pack(*_mx4(y)), c["outs"]).to(torch.bfloat16)
+    return y.to(_TYPES[c["out"]])
+
+
+def _own_adamw(s):
+    c, out = s["case"], s["out"]
+    s["table"].step(s["step"], lr=LR, betas=(BETA1, BETA2), eps=EPS, weight_decay=DECAY, sumsq=s["sumsq"],
+                    max_norm=MAX_NORM, seed=s["seed"])
+    if c["bits"] == 8:
+        s["table"].values()
+        r = [out["p"], out["m_value"], out["v_value"]]
+    else:
+        r = [out["p"], out["m"], out["v"]]
+    return r + ([out["copy"]] if c["copy"] else [])
+
+
+def _plain_adamw(s):
+    c, t = s["case"], s["case"]["step"] + 1
+    coef = (MAX_NORM / (s["sumsq"].sqrt() + 1e-6)).clamp(max=1.0)
+    g = s["grad"].float()
+    g = torch.cat([g[:s["split"]] * coef[0], g[s["split"]:] * coef[1]])
+    if c["bits"] == 32:
+        m, v = s["m"], s["v"]
+    else:
+        m, v = _values8(s["m"], s["ms"], 3), _values8(s["v"], s["vs"], 4).square()
+    m = BETA1 * m + (1 - BETA1) * g
+    v = BETA2 * v + (1 - BETA2) * g * g
+    step = m / (v.sqrt() / math.sqrt(1 - BETA2 ** t) + EPS)
+    p = s["p"] * (1 - LR * DECAY) - LR / (1 - BETA1 ** t) * step
+    if c["bits"] == 8:
+        w = _draws(s["eight"], s["tensor"], t, s["seed"])
+        m = _stochastic8(m, m.abs(), w, 3, 1.75).to(torch.bfloat16)
+        v = _stochastic8(v, v.sqrt(), (w >> 8) | ((w & 255) << 8), 4, 1.9375).to(torch.bfloat16)
+    return [p, m, v] + ([p.to(torch.bfloat16)] if c["copy"] else [])
+
+
+def _values8(codes, scales, bits):
+    """The values of 8-bit codes with a power of two for each 32."""
+    n = codes.to(torch.int32).view(-1, 32)
+    sign = 1 - 2 * (n >> 7) if bits == 3 else 1
+    n = n & 127 if bits == 3 else n
+    e, f = n >> bits, n & ((1 << bits) - 1)
+    y = torch.where(e > 0, f + (1 << bits), f).float() * sign
+    return torch.ldexp(y, e.clamp(min=1) - 7 - bits + scales.to(torch.int32)[:, None] - 127).view(-1)
+
+
+def _stochastic8(x, size, w, bits, top):
+    """x (m, or v with size = sqrt(v)) rounded to the values of 8-bit codes, up or down by the draws w."""
+    b = size.view(-1, 32)
+    f, e = torch.frexp(b.amax(1, keepdim=True))
+    k = torch.where(f * 2 <= top, e - 9, e - 8).clamp(-127, 127)
+    y = torch.ldexp(b, -k)
+    q = torch.ldexp(torch.ones_like(y), torch.frexp(y)[1].sub(1).clamp(min=-6) - bits)
+    low = (y / q).floor() * q
+    u = (w.view(-1, 32).float() + 0.5) / 65536
+    if bits == 3:
+        up = u < y / q - (y / q).floor()
+        return torch.ldexp(torch.where(up, low + q, low), k).view(-1) * torch.sign(x)
+    up = u < (torch.ldexp(x.view(-1, 32), -2 * k) - low * low) / (q * (2 * low + q))
+    return torch.ldexp(torch.where(up, low + q, low).square(), 2 * k).view(-1)
+
+
+def _draws(eight, tensor, t, seed):
+    """16 bits for each element: Philox4x32-10 of its eight, its tensor, the step and the seed."""
+    low = 0xFFFFFFFF
+    stream = tensor + 65536 * t
+    a, b, c, d = eight & low, eight >> 32, stream & low, stream >> 32
+    k0, k1 = seed & low, (seed >> 32) & low
+    for _ in range(10):
+        x, y = a * 0xD2511F53, c * 0xCD9E8D57
+        a, b, c, d = ((y >> 32) & low) ^ b ^ k0, y & low, ((x >> 32) & low) ^ d ^ k1, x & low
+        k0, k1 = (k0 + 0x9E3779B9) & low, (k1 + 0xBB67AE85) & low
+    words = torch.stack([a, b, c, d], 1)
+    return torch.stack([words & 65535, words >> 16], 2).view(-1)
+
+
+def _mx4(x):
+    """MXFP4 of the rows of x (f32): a code for each value and a scale byte for each 32, the row padded to 128s."""
+    r, k = x.shape
+    kp = (k + 127) // 128 * 128
+    b = torch.nn.functional.pad(x, (0, kp - k)).view(r, kp // 32, 32)
+    top = b.abs().amax(2)
+    e = (((top.view(torch.int32) >> 23) & 255) - 129).clamp(min=-127)
+    y = torch.ldexp(b.abs(), -e[..., None])
+    code = (y > 0.25).to(torch.uint8)
+    code += y >= 0.75
+    code += y > 1.25
+    code += y >= 1.75
+    code += y > 2.5
+    code += y >= 3.5
+    code += y > 5
+    code += 8 * (b < 0).to(torch.uint8)
+    return code.view(r, kp), torch.where(top > 0, e + 127, torch.zeros_like(e)).to(torch.uint8)
+
+
+def _pack(code, scale):
+    c = code.view(code.shape[0], -1, 2)
+    return c[..., 0] | (c[..., 1] << 4), scale
+
+
+def _unpack(packed, scale, k):
+    table = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6, -0.0, -0.5, -1, -1.5, -2, -3, -4, -6], device=packed.device)
+    y = table[torch.stack([packed & 15, packed >> 4], 2).to(torch.int32)].view(packed.shape[0], -1, 32)
+    return torch.ldexp(y, scale.to(torch.int32)[..., None] - 127).view(packed.shape[0], -1)[:, :k]
+
+
+# ---------------------------------------------------------------- the definition, in 64 bits
+def exact(c, seed):
+    global own
+    was, own = own, False
+    try:
+        s = prepare(c, seed)
+    finally:
+        own = was
+    if c["op"] == "adamw":
+        return _exact_adamw(s, c)
+    if c["op"] == "quantize":
+        x = s["h"].double()[s["e0"].long()] * s["h"].double()[s["e1"].long()] if c["pairs"] else s["x"].double()
+        return _rounded4(x.float().double())
+    x = _decoded4(*s["x"])[:, :c["cols"]] if c["type"] == "mx4" else _rounded4(s["x"].double())
+    y = torch.addmm(s["b"].double(), x, _decoded4(*s["w"])[:, :c["cols"]].t())
+    if c["relu"]:
+        y = torch.relu(y)
+    return _rounded4(y) if c["out"] == "mx4" else y
+
+
+def _floor_log2(y):
+    return torch.where(y > 0, torch.frexp(y)[1] - 1, torch.full_like(y, -10000).to(torch.int32))
+
+
+def _rounded4(x):
+    """x with every value replaced by the nearest that its block of 32 can hold."""
+    r, k = x.shape
+    b = torch.cat([x, x.new_zeros(r, -k % 32)], 1).view(r, -1, 32)
+    unit = torch.exp2((_floor_log2(b.abs().amax(2, keepdim=True)) - 2).clamp(min=-127).double())
+    y = b / unit
+    q = torch.exp2(_floor_log2(y.abs()).clamp(0, 2).double() - 1)
+    return ((y / q).round() * q).clamp(-6, 6).mul(unit).view(r, -1)[:, :k]
+
+
+def _decoded4(packed, scale):
+    n = torch.stack([packed & 15, packed >> 4], 2).view(packed.shape[0], -1).double()
+    sign, n = 1 - 2 * (n >= 8).double(), n.remainder(8)
+    size = torch.where(n < 2, n / 2, torch.exp2((n / 2).floor() - 1) * (1 + n.remainder(2) / 2))
+    return sign * size * torch.exp2(scale.double() - 127).repeat_interleave(32, 1)
+
+
+def _exact_adamw(s, c):
+    t = c["step"] + 1
+    norm = s["sumsq"].double().sqrt()
+    scale = torch.minimum(torch.ones_like(norm), MAX_NORM / (norm + 1e-6))
+    g = s["grad"].double()
+    g[:s["split"]] *= scale[0]
+    g[s["split"]:] *= scale[1]
+    if c["bits"] == 32:
+        m, v = s["m"].double(), s["v"].double()
+    else:
+        m, v = _decoded8(s["m"], s["ms"], True), _decoded8(s["v"], s["vs"], False) ** 2
+    m = torch.lerp(g, m, BETA1)
+    v = torch.lerp(g * g, v, BETA2)
+    p = s["p"].double() * (1 - LR * DECAY)
+    p -= LR * (m / (1 - BETA1 ** t)) / ((v / (1 - BETA2 ** t)).sqrt() + EPS)
+    if c["bits"] == 8:
+        w = _draws(s["eight"], s["tensor"], t, s["seed"])
+        m = _between8(m, w, True)
+        v = _between8(v, (w % 256) * 256 + w // 256, False)
+    return [p, m, v] + ([p] if c["copy"] else [])
+
+
+def _levels(signed):
+    """Every value that a code has, ascending from 0."""
+    f = 8 if signed else 16
+    n = torch.arange(127 if signed else 256, device="cuda").double()
+    e = (n / f).floor()
+    return torch.where(e > 0, (1 + n.remainder(f) / f) * torch.exp2(e - 7), n / f * 2.0 ** -6)
+
+
+def _decoded8(codes, scales, signed):
+    n = codes.long()
+    table = torch.cat([_levels(signed), torch.full((1,), math.nan, device="cuda").double()]) if signed else _levels(signed)
+    y = table[n % 128] * (1 - 2 * (n // 128)) if signed else table[n]
+    return y * torch.exp2(scales.double() - 127).repeat_interleave(32)
+
+
+def _between8(x, w, signed):
+    """x (v for signed = False, held by its root) sent to the code above or below it by the draws w."""
+    b = x.view(-1, 32).abs()
+    levels = _levels(signed) if signed else _levels(signed) ** 2
+    top = b.amax(1, keepdim=True)
+    k = torch.ceil(torch.log2(top.clamp(min=1e-300) / levels[-1]) / (1 if signed else 2)).clamp(-127, 127)
+    unit = torch.exp2(k if signed else 2 * k)
+    y = b / unit
+    i = (torch.searchsorted(levels, y, right=True) - 1).clamp(max=levels.numel() - 2)
+    low, high = levels[i], levels[i + 1]
+    up = (w.view(-1, 32).double() + 0.5) / 65536 < (y - low) / (high - low)
+    return (torch.where(up, high, low) * unit).view(-1) * torch.sign(x)
