@@ -210,7 +210,7 @@ def _prepare_adamw(s, c, seed, normal):
     s["out"] = out
     if own:
         def parts(flat, per=1):
-            return None if flat is None else [flat[o // per:o // per + -(-n // per)] for o, n in zip(at, ns)]
+            return None if flat is None else [flat[o // per:(o + _padded(n)) // per] for o, n in zip(at, ns)]
 
         s["table"] = _llp("llp_optim").AdamWTable(
             parts(p), parts(grad), parts(s["m"]), parts(s["v"]), exp_avg_scale=parts(s.get("ms"), 32),
