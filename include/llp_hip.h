@@ -620,6 +620,87 @@ int llp_adam_step_w(const llp_tensor_desc* descs, int n_tensors, int64_t max_num
 /* Refresh bf16 shadows from masters (after loading weights). */
 int llp_refresh_shadows(const llp_tensor_desc* descs, int n_tensors, int64_t max_numel, void* stream);
 
+/* ---------------------------------------------------------------- AdamW
+ * Decoupled weight decay (torch.optim.AdamW's step) over a table of tensors, moments in f32 or in
+ * 8 bits, one launch.  With g' = c g, c the clip coefficient of the tensor's group (as
+ * llp_adam_step; the gradient itself is not rewritten) and t = *step + 1:
+ *   m' = beta1 m + (1 - beta1) g',  v' = beta2 v + (1 - beta2) g'^2,
+ *   p' = p (1 - lr weight_decay) - lr / (1 - beta1^t) m' / (sqrt(v') / sqrt(1 - beta2^t) + eps).
+ * *step is read, not advanced (llp_step_end2 or llp_increment follows).  Every *_out may be its
+ * input (in place) or a buffer that overlaps no input: the state before the step then stays whole.
+ * state_bits 32: exp_avg / exp_avg_sq are f32[numel].
+ * state_bits 8: uint8[numel] codes and one scale byte s per 32 consecutive elements
+ *   (uint8[ceil(numel / 32)], the value 2^(s - 127); 255: the block holds a NaN): exp_avg as E4M3
+ *   codes, exp_avg_sq as codes of sqrt(v) with 4 exponent and 4 mantissa bits, bias 7, no sign (largest
+ *   496, 2^-10 apart below 2^-6).  Rounding is stochastic and keeps the means of m and v: one 16-bit
+ *   draw per element, half (e mod 2) of word (e mod 8) / 2 of the Philox block e / 8 in stream
+ *   65536 t + (the tensor's index in the table) with key `seed`; byte-swapped for exp_avg_sq.
+ *   The same seed, step and inputs give the same bits.
+ * work: n_work (tensor, item) int32 pairs, each tensor's items 0 .. llp_adamw_work_items(numel) - 1.
+ * llp_adamw_values: 8-bit moments (of the *_out buffers) as the values m and v they stand for, f32 or
+ *   bf16 (dtype), to exp_avg_value / exp_avg_sq_value (either may be NULL).
+ * llp_adamw_copy_t: copy_t[c, r] = param_out[r, c] for n_work (tensor, tile) pairs, each tensor's
+ *   tiles 0 .. llp_adamw_copy_t_items(rows, cols) - 1: the transposed working copies, after a step. */
+typedef struct llp_adamw_desc {
+  const void* param;               /* param_dtype [numel]                                      */
+  const void* grad;                /* grad_dtype [numel]                                       */
+  const void* exp_avg;
+  const void* exp_avg_sq;
+  const uint8_t* exp_avg_scale;    /* state_bits 8 only                                        */
+  const uint8_t* exp_avg_sq_scale;
+  void* param_out;
+  void* exp_avg_out;
+  void* exp_avg_sq_out;
+  uint8_t* exp_avg_scale_out;
+  uint8_t* exp_avg_sq_scale_out;
+  void* copy;                      /* working copy of the new parameter (copy_dtype), or NULL  */
+  void* copy_t;                    /* transposed working copy [cols][rows], or NULL            */
+  void* exp_avg_value;             /* llp_adamw_values' outputs, or NULL                       */
+  void* exp_avg_sq_value;
+  int64_t numel;
+  int64_t rows;                    /* of the copies                                            */
+  int64_t cols;
+  int64_t copy_ld;                 /* row stride of copy (0 = cols)                            */
+  int64_t copy_t_ld;               /* row stride of copy_t (0 = rows)                          */
+  int32_t group;                   /* clip group id                                            */
+  int32_t copy_dtype;              /* LLP_F32 or LLP_BF16                                      */
+} llp_adamw_desc;
+int64_t llp_adamw_work_items(int64_t numel);
+int llp_adamw_step(const llp_adamw_desc* descs, int n_tensors, const int32_t* work, int64_t n_work, int state_bits,
+                   int param_dtype, int grad_dtype, const float* sumsq, double max_norm, double lr, double beta1,
+                   double beta2, double eps, double weight_decay, const int64_t* step, uint64_t seed, void* stream);
+int llp_adamw_values(const llp_adamw_desc* descs, const int32_t* work, int64_t n_work, int dtype, void* stream);
+int64_t llp_adamw_copy_t_items(int64_t rows, int64_t cols);
+int llp_adamw_copy_t(const llp_adamw_desc* descs, const int32_t* work, int64_t n_work, int param_dtype, void* stream);
+
+/* ---------------------------------------------------------------- MXFP4
+ * A matrix in microscaled 4-bit floating point (OCP MX): each 32 consecutive values of a row share a
+ * power of two 2^(s - 127) (byte s; 255: the block holds a NaN or infinity and reads as NaN), each value
+ * is an E2M1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign).  Rows are padded with zero codes to Kp = K
+ * rounded up to 128: codes uint8 [rows][Kp / 2], the even element in the low half of a byte, row stride
+ * ld_codes (bytes, a multiple of 16, 16-B aligned); scales uint8 [rows][Kp / 32], row stride ld_scales
+ * (a multiple of 4, 4-B aligned).
+ * llp_mx4_quantize: rows of X (f32 or bf16; plain, gathered, or the pair product of two gathered rows,
+ *   formed in f32 and not rounded before): s - 127 = floor(log2 max|x|) - 2, not under -127, codes to nearest,
+ *   ties to even, saturated at 6.  X->rows_dev must be NULL.
+ * llp_mx4_dequantize: the values, as f32 or bf16 (exact in both), [M, K] with row stride ldy.
+ * llp_gemm_nt_mx4: C[m, n] = act(sum_k A[m, k] W[n, k] + bias[n]) with W in MXFP4 and A in MXFP4 (A4) or
+ *   f32 / bf16 rows (A, plain; quantised on the way as llp_mx4_quantize does: for few rows).  Exactly one
+ *   of A and A4.  Products exact, f32 sums.  act NONE or RELU; bias f32[N] or NULL.  Out: C (f32 or bf16)
+ *   or C4 (MXFP4 with K := N, the values quantised from f32; padding written), exactly one of them.
+ *   Inference only: there is no gradient through it. */
+typedef struct llp_mx4 {
+  void* codes;
+  void* scales;
+  int64_t ld_codes;
+  int64_t ld_scales;
+} llp_mx4;
+int llp_mx4_quantize(int dtype, int64_t M, int64_t K, const llp_operand* X, const llp_mx4* out, void* stream);
+int llp_mx4_dequantize(int64_t M, int64_t K, const llp_mx4* X, int dtype, void* Y, int64_t ldy, void* stream);
+int llp_gemm_nt_mx4(int64_t M, int64_t N, int64_t K, int a_dtype, const llp_operand* A, const llp_mx4* A4,
+                    const llp_mx4* W, void* C, int64_t ldc, int c_dtype, const llp_mx4* C4, const float* bias, int act,
+                    void* stream);
+
 /* ---------------------------------------------------------------- small utilities */
 int llp_convert(int src_dtype, int dst_dtype, int64_t n, const void* src, void* dst, void* stream);
 /* Sum loss terms into a running total (device), so an epoch needs one host sync. */

@@ -1,0 +1,371 @@
+// MXFP4: quantisation, its inverse, and the product C = act(A W^T + bias) on the scaled matrix
+// instruction (v_mfma_scale_f32_32x32x64_f8f6f4, both operands E2M1 with a power of two per 32 values).
+// Format and rounding: include/llp_hip.h.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "llp_common.h"
+
+namespace {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+
+template <typename T>
+__device__ __forceinline__ float as_f32(T x);
+template <>
+__device__ __forceinline__ float as_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float as_f32<bf16_t>(bf16_t x) { return bf2f(x); }
+
+typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u4_any2 __attribute__((ext_vector_type(4), aligned(2)));
+
+// 8 values at any element offset (gfx950's global loads need no alignment), zeros past n
+__device__ __forceinline__ void load8(const float* p, int n, float (&x)[8]) {
+  if (n >= 8) {
+    const f4_any a = *reinterpret_cast<const f4_any*>(p), b = *reinterpret_cast<const f4_any*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < n ? p[i] : 0.f;
+  }
+}
+__device__ __forceinline__ void load8(const bf16_t* p, int n, float (&x)[8]) {
+  if (n >= 8) {
+    const u4_any2 a = *reinterpret_cast<const u4_any2*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(a[i] << 16);
+      x[2 * i + 1] = __uint_as_float(a[i] & 0xFFFF0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < n ? bf2f(p[i]) : 0.f;
+  }
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+// the scale byte of a block whose largest value has the bits `top`: floor(log2) - 2, at least 2^-127
+__device__ __forceinline__ uint32_t mx4_scale(uint32_t top) {
+  const uint32_t e = top >> 23;
+  return e == 255u ? 255u : e < 2u ? 0u : e - 2u;
+}
+// the scale as the f32 that the conversion divides by
+__device__ __forceinline__ float mx4_scale_f32(uint32_t s) {
+  return __uint_as_float(s ? s << 23 : 0x00400000u);
+}
+// 8 values to codes: the conversion rounds to nearest even and saturates at 6
+__device__ __forceinline__ uint32_t mx4_codes(const float* x, float scale) {
+  uint32_t c = 0;
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[0], x[1], scale, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2], x[3], scale, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[4], x[5], scale, 2);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], scale, 3);
+  return c;
+}
+
+__device__ __forceinline__ uint32_t quad_umax(uint32_t x) {
+  x = umax(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 0xF, 0xF, true));   // lane ^ 1
+  return umax(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 0xF, 0xF, true));   // lane ^ 2
+}
+
+// ---------------------------------------------------------------- quantise
+// 8 values per lane, a block of 32 per quad: the block's largest by two quad exchanges, 4 bytes of
+// codes per lane, one scale byte per quad.  Bound by memory: 4 or 2 B read, 17/32 B written per value.
+template <typename T, bool PAIRS>
+__global__ __launch_bounds__(256) void mx4_quantize_kernel(int64_t M, int64_t K, int64_t per_row, llp_operand X,
+                                                           llp_mx4 out) {
+  const int64_t units = M * per_row;
+  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < units; u += (int64_t)gridDim.x * 256) {
+    const int64_t r = u / per_row, c = (u - r * per_row) * 8;
+    const int n = (int)(K - c < 8 ? (K - c < 0 ? 0 : K - c) : 8);
+    float x[8];
+    load8((const T*)X.ptr + (X.idx ? (int64_t)X.idx[r] : r) * X.ld + c, n, x);
+    if constexpr (PAIRS) {
+      float y[8];
+      load8((const T*)X.ptr2 + (X.idx2 ? (int64_t)X.idx2[r] : r) * X.ld2 + c, n, y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= y[i];
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = umax(top, abs_bits(x[i]));
+    const uint32_t s = mx4_scale(quad_umax(top));
+    const uint32_t codes = s == 255u ? 0u : mx4_codes(x, mx4_scale_f32(s));
+    *(uint32_t*)((uint8_t*)out.codes + r * out.ld_codes + (c >> 1)) = codes;
+    if ((threadIdx.x & 3) == 0) ((uint8_t*)out.scales)[r * out.ld_scales + (c >> 5)] = (uint8_t)s;
+  }
+}
+
+// the value of code c (E2M1 has f32's fields but for the bias: 2 exponent bits, 1 mantissa bit)
+__device__ __forceinline__ float mx4_value(uint32_t c, float scale) {
+  const float m = __uint_as_float((c & 7u) << 22) * 0x1p126f;
+  return __uint_as_float(__float_as_uint(m) | ((c & 8u) << 28)) * scale;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void mx4_dequantize_kernel(int64_t M, int64_t K, int64_t per_row, llp_mx4 X,
+                                                             T* __restrict__ Y, int64_t ldy) {
+  const int64_t units = M * per_row;
+  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < units; u += (int64_t)gridDim.x * 256) {
+    const int64_t r = u / per_row, c = (u - r * per_row) * 8;
+    const int64_t n = K - c;
+    const uint32_t codes = *(const uint32_t*)((const uint8_t*)X.codes + r * X.ld_codes + (c >> 1));
+    const uint32_t s = ((const uint8_t*)X.scales)[r * X.ld_scales + (c >> 5)];
+    const float f = s == 255u ? __uint_as_float(0x7FC00000u) : mx4_scale_f32(s);
+    T* y = Y + r * ldy + c;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = mx4_value(codes >> (4 * i), f);
+    if (n >= 8) {
+      if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<f4_any*>(y) = f4_any{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f4_any*>(y + 4) = f4_any{v[4], v[5], v[6], v[7]};
+      } else {
+        u4_any2 o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = (uint32_t)f2bf(v[2 * i]) | ((uint32_t)f2bf(v[2 * i + 1]) << 16);
+        *reinterpret_cast<u4_any2*>(y) = o;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) {
+          if constexpr (sizeof(T) == 4) y[i] = v[i];
+          else y[i] = f2bf(v[i]);
+        }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- product
+// The matrix instruction's first operand is W and its second A, so that its 32 x 32 result holds, in
+// lane l, row m = l % 32 of C at the 16 columns 8 (i / 4) + 4 (l / 32) + i % 4: runs of 4 along the row.
+// Operand lane l: row l % 32, the 32 values of block l / 32 of the 64 that one instruction takes, in
+// 4 registers (16 consecutive bytes of codes), and that block's scale byte: a lane's own.
+struct Mx4Args {
+  int64_t M, N, K, Kp;
+  const void* A;         // f32 / bf16 rows
+  int64_t lda;
+  llp_mx4 A4, W, C4;
+  void* C;
+  int64_t ldc;
+  const float* bias;
+  int relu;
+};
+
+__device__ __forceinline__ void load_block(const llp_mx4& x, int64_t row, int64_t kb, bool ok, v8i& v, int& s) {
+  u4v c = {0, 0, 0, 0};
+  s = 0;
+  if (ok) {
+    c = *(const u4v*)((const uint8_t*)x.codes + row * x.ld_codes + kb * 16);
+    s = ((const uint8_t*)x.scales)[row * x.ld_scales + kb];
+  }
+  v = v8i{(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
+}
+
+// a block of 32 values of an f32 / bf16 row, quantised in the lane that feeds it to the instruction
+template <typename T>
+__device__ __forceinline__ void quantize_block(const T* row, int64_t k, int64_t K, bool ok, v8i& v, int& s) {
+  float x[32];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float y[8];
+    const int64_t left = ok ? K - k - 8 * j : 0;
+    load8(row + k + 8 * j, (int)(left < 0 ? 0 : left > 8 ? 8 : left), y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[8 * j + i] = y[i];
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) top = umax(top, abs_bits(x[i]));
+  const uint32_t b = mx4_scale(top);
+  const float f = mx4_scale_f32(b);
+  s = (int)b;
+  v = v8i{0, 0, 0, 0, 0, 0, 0, 0};
+  if (b != 255u) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = (int)mx4_codes(x + 8 * j, f);
+  }
+}
+
+// One workgroup per 32 x 32 tile of C, its K split over 4 waves and joined through LDS in wave order.
+// SRC 0: A in MXFP4, 1: f32, 2: bf16.  OUT 0: f32, 1: bf16, 2: MXFP4.
+template <int SRC, int OUT>
+__global__ __launch_bounds__(256) void gemm_mx4_tile_kernel(Mx4Args g) {
+  __shared__ float part[3][64][17];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t n0 = (int64_t)blockIdx.x * 32, m0 = (int64_t)blockIdx.y * 32;
+  const int64_t wr = n0 + (lane & 31), ar = m0 + (lane & 31);
+  float16_t acc = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+  for (int64_t kb = 2 * wave + (lane >> 5); kb < g.Kp / 32; kb += 8) {
+    v8i w, a;
+    int sw, sa;
+    load_block(g.W, wr, kb, wr < g.N, w, sw);
+    if constexpr (SRC == 0) load_block(g.A4, ar, kb, ar < g.M, a, sa);
+    else if constexpr (SRC == 1) quantize_block((const float*)g.A + ar * g.lda, kb * 32, g.K, ar < g.M, a, sa);
+    else quantize_block((const bf16_t*)g.A + ar * g.lda, kb * 32, g.K, ar < g.M, a, sa);
+    acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, a, acc, 4, 4, 0, sw, 0, sa);
+  }
+  if (wave > 0)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) part[wave - 1][lane][i] = acc[i];
+  __syncthreads();
+  if (wave > 0) return;
+  const int h = lane >> 5;
+  float y[16];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int64_t n = n0 + 8 * (i >> 2) + 4 * h + (i & 3);
+    float v = ((acc[i] + part[0][lane][i]) + part[1][lane][i]) + part[2][lane][i];
+    if (g.bias) v += n < g.N ? g.bias[n] : 0.f;
+    if (g.relu) v = v < 0.f ? 0.f : v;   // a NaN stays
+    y[i] = n < g.N ? v : 0.f;
+    top = umax(top, abs_bits(y[i]));
+  }
+  if constexpr (OUT == 2) {
+    top = umax(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+    const uint32_t s = mx4_scale(top);
+    const float f = mx4_scale_f32(s);
+    if (ar < g.M) {
+      uint8_t* c = (uint8_t*)g.C4.codes + ar * g.C4.ld_codes + n0 / 2 + 2 * h;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t q = 0;
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[4 * j], y[4 * j + 1], f, 0);
+        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[4 * j + 2], y[4 * j + 3], f, 1);
+        *(uint16_t*)(c + 4 * j) = s == 255u ? 0 : (uint16_t)q;
+      }
+      if (h == 0) ((uint8_t*)g.C4.scales)[ar * g.C4.ld_scales + n0 / 32] = (uint8_t)s;
+    }
+  } else {
+    if (ar < g.M)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int64_t n = n0 + 8 * (i >> 2) + 4 * h + (i & 3);
+        if (n < g.N) {
+          if constexpr (OUT == 0) ((float*)g.C)[ar * g.ldc + n] = y[i];
+          else ((bf16_t*)g.C)[ar * g.ldc + n] = f2bf(y[i]);
+        }
+      }
+  }
+}
+
+int64_t pad128(int64_t k) { return (k + 127) / 128 * 128; }
+
+const char* bad_mx4(const llp_mx4* x, int64_t rows, int64_t K) {
+  if (!x) return "null";
+  if (rows > 0 && (!x->codes || !x->scales)) return "null buffer";
+  if (x->ld_codes < pad128(K) / 2 || x->ld_codes % 16 || ((uintptr_t)x->codes & 15)) return "codes need rows of Kp / 2 bytes, 16-B aligned";
+  if (x->ld_scales < pad128(K) / 32 || x->ld_scales % 4 || ((uintptr_t)x->scales & 3)) return "scales need rows of Kp / 32 bytes, 4-B aligned";
+  return nullptr;
+}
+
+}  // namespace
+
+extern "C" int llp_mx4_quantize(int dtype, int64_t M, int64_t K, const llp_operand* X, const llp_mx4* out, void* stream) {
+  LLP_CHECK_ARG(dtype == LLP_F32 || dtype == LLP_BF16, "llp_mx4_quantize: rows in f32 or bf16");
+  LLP_CHECK_ARG(M >= 0 && K >= 1 && K < (1ll << 31), "llp_mx4_quantize: M >= 0, 1 <= K < 2^31");
+  if (M == 0) return LLP_OK;
+  LLP_CHECK_ARG(X && X->ptr, "llp_mx4_quantize: null pointer");
+  LLP_CHECK_ARG(!X->rows_dev, "llp_mx4_quantize: no device row count");
+  LLP_CHECK_ARG(!X->idx2 || X->ptr2, "llp_mx4_quantize: idx2 without ptr2");
+  const char* why = bad_mx4(out, M, K);
+  LLP_CHECK_ARG(!why, "llp_mx4_quantize: out: %s", why);
+  const int64_t per_row = pad128(K) / 8;
+  const unsigned nb = (unsigned)std::min<int64_t>((M * per_row + 255) / 256, 1 << 20);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(nb), dim3(256), 0, (hipStream_t)stream, M, K, per_row, *X, *out);
+  };
+  if (dtype == LLP_F32) X->ptr2 ? go(mx4_quantize_kernel<float, true>) : go(mx4_quantize_kernel<float, false>);
+  else X->ptr2 ? go(mx4_quantize_kernel<bf16_t, true>) : go(mx4_quantize_kernel<bf16_t, false>);
+  LLP_LAUNCH_CHECK();
+  return LLP_OK;
+}
+
+extern "C" int llp_mx4_dequantize(int64_t M, int64_t K, const llp_mx4* X, int dtype, void* Y, int64_t ldy, void* stream) {
+  LLP_CHECK_ARG(dtype == LLP_F32 || dtype == LLP_BF16, "llp_mx4_dequantize: values in f32 or bf16");
+  LLP_CHECK_ARG(M >= 0 && K >= 1 && K < (1ll << 31) && ldy >= K, "llp_mx4_dequantize: M >= 0, 1 <= K < 2^31, ldy >= K");
+  if (M == 0) return LLP_OK;
+  LLP_CHECK_ARG(Y, "llp_mx4_dequantize: null pointer");
+  const char* why = bad_mx4(X, M, K);
+  LLP_CHECK_ARG(!why, "llp_mx4_dequantize: X: %s", why);
+  const int64_t per_row = (K + 7) / 8;
+  const unsigned nb = (unsigned)std::min<int64_t>((M * per_row + 255) / 256, 1 << 20);
+  if (dtype == LLP_F32)
+    hipLaunchKernelGGL(mx4_dequantize_kernel<float>, dim3(nb), dim3(256), 0, (hipStream_t)stream, M, K, per_row, *X, (float*)Y, ldy);
+  else
+    hipLaunchKernelGGL(mx4_dequantize_kernel<bf16_t>, dim3(nb), dim3(256), 0, (hipStream_t)stream, M, K, per_row, *X, (bf16_t*)Y, ldy);
+  LLP_LAUNCH_CHECK();
+  return LLP_OK;
+}
+
+extern "C" int llp_gemm_nt_mx4(int64_t M, int64_t N, int64_t K, int a_dtype, const llp_operand* A, const llp_mx4* A4,
+                               const llp_mx4* W, void* C, int64_t ldc, int c_dtype, const llp_mx4* C4,
+                               const float* bias, int act, void* stream) {
+  LLP_CHECK_ARG(M >= 0 && N >= 0 && K >= 1 && M < (1ll << 31) && N < (1ll << 31) && K < (1ll << 31),
+                "llp_gemm_nt_mx4: M, N >= 0, K >= 1, each < 2^31");
+  LLP_CHECK_ARG(act == LLP_ACT_NONE || act == LLP_ACT_RELU, "llp_gemm_nt_mx4: act must be NONE or RELU");
+  LLP_CHECK_ARG((A != nullptr) != (A4 != nullptr), "llp_gemm_nt_mx4: exactly one of A and A4");
+  if (M == 0 || N == 0) return LLP_OK;
+  LLP_CHECK_ARG((C != nullptr) != (C4 != nullptr), "llp_gemm_nt_mx4: exactly one of C and C4");
+  const char* why = bad_mx4(W, N, K);
+  LLP_CHECK_ARG(!why, "llp_gemm_nt_mx4: W: %s", why);
+  Mx4Args g{};
+  g.M = M, g.N = N, g.K = K, g.Kp = pad128(K), g.W = *W, g.bias = bias, g.relu = act == LLP_ACT_RELU;
+  int src = 0, out = 2;
+  if (A4) {
+    why = bad_mx4(A4, M, K);
+    LLP_CHECK_ARG(!why, "llp_gemm_nt_mx4: A4: %s", why);
+    g.A4 = *A4;
+  } else {
+    LLP_CHECK_ARG(a_dtype == LLP_F32 || a_dtype == LLP_BF16, "llp_gemm_nt_mx4: A in f32 or bf16");
+    LLP_CHECK_ARG(A->ptr && !A->idx && !A->ptr2 && !A->idx2 && !A->rows_dev, "llp_gemm_nt_mx4: A must be plain rows");
+    LLP_CHECK_ARG(M == 1 || A->ld >= K, "llp_gemm_nt_mx4: A's rows overlap");
+    g.A = A->ptr, g.lda = A->ld;
+    src = a_dtype == LLP_F32 ? 1 : 2;
+  }
+  if (C4) {
+    why = bad_mx4(C4, M, N);
+    LLP_CHECK_ARG(!why, "llp_gemm_nt_mx4: C4: %s", why);
+    g.C4 = *C4;
+  } else {
+    LLP_CHECK_ARG(c_dtype == LLP_F32 || c_dtype == LLP_BF16, "llp_gemm_nt_mx4: C in f32 or bf16");
+    LLP_CHECK_ARG(M == 1 || ldc >= N, "llp_gemm_nt_mx4: C's rows overlap");
+    g.C = C, g.ldc = ldc;
+    out = c_dtype == LLP_F32 ? 0 : 1;
+  }
+  const int64_t nt = (C4 ? pad128(N) : N + 31) / 32, mt = (M + 31) / 32;
+  auto go = [&](auto kernel) -> int {
+    // the grid's second dimension ends at 65,535: longer M in slices
+    for (int64_t b = 0; b < mt; b += 65535) {
+      Mx4Args h = g;
+      const int64_t r = b * 32;
+      h.M = std::min<int64_t>(M - r, 65535 * 32);
+      if (h.A) h.A = (const char*)h.A + r * h.lda * (src == 1 ? 4 : 2);
+      if (A4) h.A4.codes = (char*)h.A4.codes + r * h.A4.ld_codes, h.A4.scales = (char*)h.A4.scales + r * h.A4.ld_scales;
+      if (h.C) h.C = (char*)h.C + r * h.ldc * (out == 0 ? 4 : 2);
+      if (C4) h.C4.codes = (char*)h.C4.codes + r * h.C4.ld_codes, h.C4.scales = (char*)h.C4.scales + r * h.C4.ld_scales;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)nt, (unsigned)std::min<int64_t>(mt - b, 65535)), dim3(256), 0,
+                         (hipStream_t)stream, h);
+      LLP_LAUNCH_CHECK();
+    }
+    return LLP_OK;
+  };
+  switch (src * 3 + out) {
+    case 0: return go(gemm_mx4_tile_kernel<0, 0>);
+    case 1: return go(gemm_mx4_tile_kernel<0, 1>);
+    case 2: return go(gemm_mx4_tile_kernel<0, 2>);
+    case 3: return go(gemm_mx4_tile_kernel<1, 0>);
+    case 4: return go(gemm_mx4_tile_kernel<1, 1>);
+    case 5: return go(gemm_mx4_tile_kernel<1, 2>);
+    case 6: return go(gemm_mx4_tile_kernel<2, 0>);
+    case 7: return go(gemm_mx4_tile_kernel<2, 1>);
+    default: return go(gemm_mx4_tile_kernel<2, 2>);
+  }
+}

@@ -46,8 +46,32 @@ class TensorDesc(C.Structure):
                 ("shadow_dtype", C.c_int32), ("shadow_ld", c_i64), ("shadow_t_ld", c_i64)]
 
 
+class AdamWDesc(C.Structure):
+    """llp_adamw_desc: one tensor of an AdamW table."""
+    _fields_ = [("param", c_vp), ("grad", c_vp), ("exp_avg", c_vp), ("exp_avg_sq", c_vp), ("exp_avg_scale", c_vp),
+                ("exp_avg_sq_scale", c_vp), ("param_out", c_vp), ("exp_avg_out", c_vp), ("exp_avg_sq_out", c_vp),
+                ("exp_avg_scale_out", c_vp), ("exp_avg_sq_scale_out", c_vp), ("copy", c_vp), ("copy_t", c_vp),
+                ("exp_avg_value", c_vp), ("exp_avg_sq_value", c_vp), ("numel", c_i64), ("rows", c_i64), ("cols", c_i64),
+                ("copy_ld", c_i64), ("copy_t_ld", c_i64), ("group", C.c_int32), ("copy_dtype", C.c_int32)]
+
+
+class Mx4(C.Structure):
+    """llp_mx4: a matrix in MXFP4 (llp_mx.MX4 holds the tensors)."""
+    _fields_ = [("codes", c_vp), ("scales", c_vp), ("ld_codes", c_i64), ("ld_scales", c_i64)]
+
+
 _SIGS = {
     "llp_version": (c_int, []),
+    "llp_adamw_work_items": (c_i64, [c_i64]),
+    "llp_adamw_step": (c_int, [c_vp, c_int, c_vp, c_i64, c_int, c_int, c_int, c_vp, c_f64, c_f64, c_f64, c_f64, c_f64,
+                               c_f64, c_vp, c_u64, c_vp]),
+    "llp_adamw_values": (c_int, [c_vp, c_vp, c_i64, c_int, c_vp]),
+    "llp_adamw_copy_t_items": (c_i64, [c_i64, c_i64]),
+    "llp_adamw_copy_t": (c_int, [c_vp, c_vp, c_i64, c_int, c_vp]),
+    "llp_mx4_quantize": (c_int, [c_int, c_i64, c_i64, C.POINTER(Operand), C.POINTER(Mx4), c_vp]),
+    "llp_mx4_dequantize": (c_int, [c_i64, c_i64, C.POINTER(Mx4), c_int, c_vp, c_i64, c_vp]),
+    "llp_gemm_nt_mx4": (c_int, [c_i64, c_i64, c_i64, c_int, C.POINTER(Operand), C.POINTER(Mx4), C.POINTER(Mx4), c_vp,
+                                c_i64, c_int, C.POINTER(Mx4), c_vp, c_int, c_vp]),
     "llp_last_error": (C.c_char_p, []),
     "llp_last_gemm_kernel": (C.c_char_p, []),
     "llp_device_count": (c_int, []),
@@ -896,11 +920,30 @@ def increment(ctr):
 
 
 def descs_to_device(descs, device):
-    """Pack a list of TensorDesc into a device byte tensor."""
-    arr = (TensorDesc * len(descs))(*descs)
+    """Pack a list of TensorDesc (or AdamWDesc) into a device byte tensor."""
+    arr = (type(descs[0]) * len(descs))(*descs)
     raw = bytes(C.string_at(C.addressof(arr), C.sizeof(arr)))
     host = torch.frombuffer(bytearray(raw), dtype=torch.uint8)
     return host.to(device)
+
+
+class on_device:
+    """The launch context of ``dev``: its current stream's handle, with ``dev`` the current device
+    (a kernel launches on the current device; a tensor may live on another)."""
+    __slots__ = ("dev", "prev")
+
+    def __init__(self, dev):
+        self.dev = dev.index
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.dev:
+            torch.cuda.set_device(self.dev)
+        return torch.cuda.current_stream(self.dev).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.prev != self.dev:
+            torch.cuda.set_device(self.prev)
 
 
 def relu_bwd(gy, y, alpha, out):

@@ -1,0 +1,178 @@
+"""MXFP4 (microscaled 4-bit floating point) matrices for serving the student: quantisation, its
+inverse and the product, on the hand-written kernels of csrc/mx4.hip.
+
+  q = quantize(x)                        rows of x (f32 / bf16) in 4.25 bits a value
+  q = quantize(h, e0, h, e1)             the predictor's input h[e0] * h[e1] (src/models.py:140)
+  y = linear(x, w, bias, relu=True)      relu(Q(x) w^T + bias), w = quantize(weight), laid out once;
+                                         x in f32 / bf16, or already in MXFP4; y in f32 / bf16 / MXFP4
+  x = dequantize(q)                      the values
+
+Each 32 consecutive values of a row share a power of two; a value is a 4-bit code (0, 0.5, 1, 1.5, 2, 3,
+4, 6 and a sign) to nearest, ties to even, saturated at 6.  A block with a NaN or an infinity reads as
+NaN.  Products are exact and summed in f32.  There is no gradient: under autograd, with an input that
+requires one, the calls raise.  Replaces nn.Linear + ReLU of MLP / LinkPredictor in evaluation
+(src/models.py:45-54,139-150); used by llp_eval with dtype "mxfp4".
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+import llp_hip as K
+
+# f32 / bf16 inputs of up to this many rows are quantised inside the product (one launch); more rows
+# are quantised first, once, instead of once for each 32 columns of the result.
+DIRECT_ROWS = 64
+
+
+def _pad(k):
+    return -(-k // 128) * 128
+
+
+class MX4:
+    """A [rows, cols] matrix in MXFP4: ``codes`` uint8 [rows, pad / 2] (even element in the low half) and
+    ``scales`` uint8 [rows, pad / 32] with pad = cols rounded up to 128 (zero codes behind cols)."""
+    __slots__ = ("codes", "scales", "cols", "c")
+
+    def __init__(self, codes, scales, cols):
+        for name, t, per in (("codes", codes, 2), ("scales", scales, 32)):
+            if t.dtype != torch.uint8 or t.dim() != 2:
+                raise TypeError(f"MX4 {name}: a 2-D uint8 tensor")
+            if t.shape[1] * per != _pad(cols) or (t.shape[1] > 1 and t.stride(1) != 1):
+                raise ValueError(f"MX4 {name}: rows of {_pad(cols) // per} contiguous bytes for {cols} columns")
+        if cols < 1 or codes.shape[0] != scales.shape[0] or codes.device != scales.device:
+            raise ValueError("MX4: codes and scales of the same rows, on the same device")
+        self.codes, self.scales, self.cols = codes, scales, int(cols)
+        self.c = K.Mx4(codes.data_ptr(), scales.data_ptr(), codes.stride(0), scales.stride(0))
+
+    @staticmethod
+    def empty(rows, cols, device):
+        p = _pad(cols)
+        return MX4(torch.empty(rows, p // 2, dtype=torch.uint8, device=device),
+                   torch.empty(rows, p // 32, dtype=torch.uint8, device=device), cols)
+
+    @property
+    def rows(self):
+        return self.codes.shape[0]
+
+    @property
+    def shape(self):
+        return (self.codes.shape[0], self.cols)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def _rows2d(x, what):
+    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise ValueError(f"{what}: a 2-D tensor with contiguous rows")
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"{what}: f32 or bf16, not {x.dtype}")
+    if not x.is_cuda:
+        raise RuntimeError("LLP ops run only on the MI355X HIP device (got a CPU tensor; no CPU fallback)")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise RuntimeError(f"{what}: MXFP4 has no gradient; call it under torch.no_grad()")
+
+
+def _index(i, x, what):
+    if i is None:
+        return
+    if i.dtype != torch.int32 or i.dim() != 1 or not i.is_contiguous():
+        raise TypeError(f"{what}: a contiguous 1-D int32 tensor")
+    if i.device != x.device:
+        raise ValueError(f"{what}: on {i.device}, the rows on {x.device}")
+
+
+def quantize(x, idx=None, x2=None, idx2=None, out=None):
+    """MXFP4 of x[idx] (of x2[idx2] * x[idx], formed in f32, with x2); idx None: all rows.  The indices
+    must lie within the rows (they are read on the device and not checked)."""
+    _rows2d(x, "quantize")
+    _index(idx, x, "quantize idx")
+    rows = x.shape[0] if idx is None else idx.shape[0]
+    if x2 is None:
+        if idx2 is not None:
+            raise ValueError("quantize: idx2 without x2")
+        op = K.Operand(x.data_ptr(), K.ptr(idx), None, None, x.stride(0), 0, None)
+    else:
+        _rows2d(x2, "quantize x2")
+        _index(idx2, x, "quantize idx2")
+        if x2.dtype != x.dtype or x2.device != x.device or x2.shape[1] != x.shape[1]:
+            raise ValueError("quantize: x and x2 of one dtype, device and width")
+        if (x2.shape[0] if idx2 is None else idx2.shape[0]) != rows:
+            raise ValueError("quantize: x[idx] and x2[idx2] differ in rows")
+        op = K.Operand(x.data_ptr(), K.ptr(idx), x2.data_ptr(), K.ptr(idx2), x.stride(0), x2.stride(0), None)
+    if rows and min(x.shape[0], rows if x2 is None else x2.shape[0]) == 0:
+        raise ValueError("quantize: indices into no rows")
+    if x.shape[1] < 1:
+        raise ValueError("quantize: no columns")
+    if out is None:
+        out = MX4.empty(rows, x.shape[1], x.device)
+    elif out.shape != (rows, x.shape[1]) or out.device != x.device:
+        raise ValueError(f"quantize: out is {out.shape} on {out.device}, the rows are {(rows, x.shape[1])} on {x.device}")
+    L = K.lib()
+    with K.on_device(x.device) as stream:
+        K.check(L.llp_mx4_quantize(K.dtype_code(x.dtype), rows, x.shape[1], C.byref(op), C.byref(out.c), stream),
+                "llp_mx4_quantize")
+    return out
+
+
+def dequantize(q, dtype=torch.float32, out=None):
+    """The values of q (exact in f32; in bf16 too, down to 2^-133)."""
+    if out is None:
+        out = torch.empty(q.rows, q.cols, dtype=dtype, device=q.device)
+    elif tuple(out.shape) != q.shape or out.device != q.device or (q.cols > 1 and out.stride(1) != 1):
+        raise ValueError("dequantize: out needs q's shape, on its device, with contiguous rows")
+    L = K.lib()
+    with K.on_device(q.device) as stream:
+        K.check(L.llp_mx4_dequantize(q.rows, q.cols, C.byref(q.c), K.dtype_code(out.dtype), out.data_ptr(),
+                                     max(out.stride(0), q.cols), stream), "llp_mx4_dequantize")
+    return out
+
+
+def linear(x, w, bias=None, relu=False, out_dtype=None, out=None):
+    """act(Q(x) w^T + bias): x [..., cols] in f32 / bf16 or an MX4, w an MX4 [N, cols], bias [N].
+    out_dtype torch.float32 / torch.bfloat16 / "mx4" (default x's dtype; bf16 for an MX4 x); ``out``: a
+    2-D tensor with contiguous rows, or an MX4, written in place of a new one."""
+    lead = None
+    if isinstance(x, MX4):
+        rows, dt = x.rows, torch.bfloat16
+        width, dev = x.cols, x.device
+    else:
+        if x.dim() != 2:
+            lead = x.shape[:-1]
+            x = x.reshape(-1, x.shape[-1])
+        _rows2d(x, "linear")
+        rows, dt = x.shape[0], x.dtype
+        width, dev = x.shape[1], x.device
+    if width != w.cols or dev != w.device:
+        raise ValueError(f"linear: x has {width} columns on {dev}, w has {w.cols} on {w.device}")
+    N = w.rows
+    if bias is not None:
+        if torch.is_grad_enabled() and bias.requires_grad:
+            raise RuntimeError("linear: MXFP4 has no gradient; call it under torch.no_grad()")
+        if bias.shape != (N,) or bias.device != dev:
+            raise ValueError(f"linear: bias of {N} values on {dev}")
+        bias = bias.detach().float().contiguous()
+    if out is None:
+        out_dtype = dt if out_dtype is None else out_dtype
+        out = MX4.empty(rows, N, dev) if out_dtype == "mx4" else torch.empty(rows, N, dtype=out_dtype, device=dev)
+    elif tuple(out.shape) != (rows, N) or out.device != dev or lead is not None:
+        raise ValueError(f"linear: out is {tuple(out.shape)} on {out.device}, the result is {(rows, N)} on {dev}")
+    four = isinstance(out, MX4)
+    if not four and (out.dtype not in (torch.float32, torch.bfloat16) or (N > 1 and out.stride(1) != 1)):
+        raise TypeError("linear: out in f32 or bf16 with contiguous rows")
+    if not isinstance(x, MX4) and rows > DIRECT_ROWS:
+        x = quantize(x)
+    L = K.lib()
+    op, code = None, 0
+    if not isinstance(x, MX4):
+        op = C.byref(K.Operand(x.data_ptr(), None, None, None, x.stride(0), 0, None))
+        code = K.dtype_code(x.dtype)
+    with K.on_device(dev) as stream:
+        K.check(L.llp_gemm_nt_mx4(rows, N, width, code, op, None if op else C.byref(x.c), C.byref(w.c),
+                                  None if four else out.data_ptr(), 0 if four else max(out.stride(0), N),
+                                  0 if four else K.dtype_code(out.dtype), C.byref(out.c) if four else None,
+                                  K.ptr(bias), K.ACT_RELU if relu else K.ACT_NONE, stream), "llp_gemm_nt_mx4")
+    return out if lead is None or four else out.reshape(*lead, N)

@@ -1,0 +1,312 @@
+"""AdamW over many tensors, its moments in f32 or in 8 bits (csrc/adamw.hip).
+
+``AdamW`` is a torch.optim.Optimizer: torch.optim.AdamW's update (decoupled weight decay) in one launch
+for each parameter group, ``state_bits=8`` with block-scaled moments of 8.25 bits a value, rounded
+stochastically so that their means are kept.  The training engines take it in place of
+torch.optim.Adam (src/main.py:400-402).  ``AdamWTable`` is the step itself over lists of tensors, in
+place or into other buffers.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+import llp_hip as K
+
+
+def _check(name, ts, ref, dtypes, dev):
+    if len(ts) != len(ref):
+        raise ValueError(f"AdamWTable: {len(ref)} params, {len(ts)} {name}")
+    for t in ts:
+        if t.device != dev:
+            raise ValueError(f"AdamWTable: {name} on {t.device}, params on {dev}")
+        if not t.is_contiguous():
+            raise ValueError(f"AdamWTable: {name} must be contiguous")
+        if t.dtype != ts[0].dtype or t.dtype not in dtypes:
+            raise TypeError(f"AdamWTable: {name} must share one dtype of {[str(d) for d in dtypes]}")
+
+
+_FLOATS = (torch.float32, torch.bfloat16)
+
+
+class AdamWTable:
+    """The tensors of an AdamW step: ``params`` and ``grads`` (lists, f32 or bf16) and the moments
+    ``exp_avg`` / ``exp_avg_sq``: f32 lists, or uint8 codes with ``exp_avg_scale`` /
+    ``exp_avg_sq_scale`` (uint8, one per 32 elements of a tensor; ``AdamWTable.state8`` makes zero ones).
+
+    groups     clip group (0..7) of each tensor, an index into the step's ``sumsq``
+    copies     working copies of the new params (f32 or bf16; None entries: none): a tensor of the
+               param's shape, or (tensor, row stride) for rows inside a wider operand
+    copies_t   transposed working copies, likewise
+    out        {"params", "exp_avg", "exp_avg_sq"[, "exp_avg_scale", "exp_avg_sq_scale"]}: lists to
+               write instead of the inputs (default: in place); the state before the step then stays
+    values     {"exp_avg", "exp_avg_sq"}: lists that ``values()`` fills with the 8-bit moments' values
+
+    The table holds the addresses; it stays valid while the tensors keep their storage, and the
+    launches of ``step`` can be captured into a graph."""
+
+    def __init__(self, params, grads, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_sq_scale=None, groups=None,
+                 copies=None, copies_t=None, out=None, values=None):
+        if not params:
+            raise ValueError("AdamWTable: no params")
+        if len(params) > 65536:
+            raise ValueError("AdamWTable: at most 65,536 params")
+        dev = params[0].device
+        _check("params", params, params, _FLOATS, dev)
+        _check("grads", grads, params, _FLOATS, dev)
+        self.bits = 8 if exp_avg_scale is not None else 32
+        if (exp_avg_scale is None) != (exp_avg_sq_scale is None):
+            raise ValueError("AdamWTable: exp_avg_scale and exp_avg_sq_scale go together")
+        kinds = (torch.uint8,) if self.bits == 8 else (torch.float32,)
+        ins = {"params": params, "exp_avg": exp_avg, "exp_avg_sq": exp_avg_sq}
+        if self.bits == 8:
+            ins.update(exp_avg_scale=exp_avg_scale, exp_avg_sq_scale=exp_avg_sq_scale)
+        outs = dict(ins)
+        for k, v in (out or {}).items():
+            if v is not None:
+                if k not in ins:
+                    raise ValueError(f"AdamWTable: out has no {k!r} here")
+                outs[k] = v
+        values = {k: v for k, v in (values or {}).items() if v is not None}
+        if values and self.bits != 8:
+            raise ValueError("AdamWTable: f32 moments are their values")
+        for d in (ins, outs):
+            for k, ts in d.items():
+                _check(k, ts, params, (params[0].dtype,) if k == "params" else kinds, dev)
+        self.values_dtype = None
+        for k, ts in values.items():
+            if k not in ("exp_avg", "exp_avg_sq"):
+                raise ValueError(f"AdamWTable: values has no {k!r}")
+            _check(f"values[{k!r}]", ts, params, _FLOATS, dev)
+            if self.values_dtype not in (None, ts[0].dtype):
+                raise TypeError("AdamWTable: values in one dtype")
+            self.values_dtype = ts[0].dtype
+        for i, p in enumerate(params):
+            n, blocks = p.numel(), -(-p.numel() // 32)
+            for d in (ins, outs, {"grads": grads}, values):
+                for k, ts in d.items():
+                    want = blocks if k.endswith("scale") else n
+                    if ts[i].numel() != want:
+                        raise ValueError(f"AdamWTable: {k}[{i}] has {ts[i].numel()} elements, {want} are needed")
+        groups = [0] * len(params) if groups is None else [int(g) for g in groups]
+        if len(groups) != len(params) or any(not 0 <= g < 8 for g in groups):
+            raise ValueError("AdamWTable: a clip group in 0..7 for each param")
+        self.n_groups = max(groups) + 1
+        copies, copies_t = self._copies(copies, params, dev), self._copies(copies_t, params, dev)
+        if not params[0].is_cuda:
+            raise RuntimeError("AdamWTable runs only on the MI355X HIP device (got CPU tensors; no CPU fallback)")
+        self._apart(ins, outs, grads, copies, copies_t, values)
+        L = K.load()
+        descs, work, work_t = [], [], []
+
+        def at(ts, i):
+            return None if ts is None else ts[i].data_ptr()
+
+        for i, p in enumerate(params):
+            rows, cols = (p.shape[0], p.shape[1]) if p.dim() == 2 else (1, p.numel())
+            c, ct = copies[i], copies_t[i]
+            kinds = {t.dtype for t, _ in (c, ct) if t is not None}
+            if len(kinds) > 1:
+                raise TypeError("AdamWTable: a param's copies in one dtype")
+            descs.append(K.AdamWDesc(
+                p.data_ptr(), grads[i].data_ptr(), exp_avg[i].data_ptr(), exp_avg_sq[i].data_ptr(),
+                at(ins.get("exp_avg_scale"), i), at(ins.get("exp_avg_sq_scale"), i), outs["params"][i].data_ptr(),
+                outs["exp_avg"][i].data_ptr(), outs["exp_avg_sq"][i].data_ptr(), at(outs.get("exp_avg_scale"), i),
+                at(outs.get("exp_avg_sq_scale"), i), K.ptr(c[0]), K.ptr(ct[0]),
+                at(values.get("exp_avg"), i), at(values.get("exp_avg_sq"), i), p.numel(), rows, cols,
+                c[1], ct[1], groups[i], K.dtype_code(kinds.pop()) if kinds else K.LLP_F32))
+            items = L.llp_adamw_work_items(p.numel())
+            work.append(torch.stack([torch.full((items,), i, dtype=torch.int32), torch.arange(items, dtype=torch.int32)], 1))
+            if ct[0] is not None:
+                tiles = L.llp_adamw_copy_t_items(rows, cols)
+                work_t.append(torch.stack([torch.full((tiles,), i, dtype=torch.int32),
+                                           torch.arange(tiles, dtype=torch.int32)], 1))
+        self.device = dev
+        self.n = len(params)
+        self.param_code, self.grad_code = K.dtype_code(params[0].dtype), K.dtype_code(grads[0].dtype)
+        self._descs = K.descs_to_device(descs, dev)
+        self._work = torch.cat(work).to(dev)
+        self._work_t = torch.cat(work_t).to(dev) if work_t else None
+        self._keep = (ins, outs, grads, copies, copies_t, values)
+
+    @staticmethod
+    def state8(numel, device):
+        """Zero 8-bit moments of ``numel`` elements: (codes, scales)."""
+        return (torch.zeros(numel, dtype=torch.uint8, device=device),
+                torch.zeros(-(-numel // 32), dtype=torch.uint8, device=device))
+
+    @staticmethod
+    def _copies(ts, params, dev):
+        if ts is None:
+            return [(None, 0)] * len(params)
+        if len(ts) != len(params):
+            raise ValueError("AdamWTable: an entry (or None) of copies for each param")
+        got = []
+        for t in ts:
+            t, ld = t if isinstance(t, tuple) else (t, 0)
+            if t is not None:
+                if t.device != dev or t.dtype not in _FLOATS:
+                    raise TypeError(f"AdamWTable: copies in f32 or bf16 on {dev}")
+                if not ld and not t.is_contiguous():
+                    raise ValueError("AdamWTable: copies contiguous, or given with their row stride")
+            got.append((t, int(ld)))
+        return got
+
+    @staticmethod
+    def _apart(ins, outs, grads, copies, copies_t, values):
+        """What a step writes overlaps nothing else that it reads or writes but its own input in place."""
+        spans = []
+
+        def add(t, write, own):
+            if t is not None and t.numel():
+                lo = t.data_ptr()
+                spans.append((lo, lo + t.numel() * t.element_size(), write, own))
+
+        for k in ins:
+            for i, (a, b) in enumerate(zip(ins[k], outs[k])):
+                if a.data_ptr() == b.data_ptr():
+                    add(a, True, None)
+                else:
+                    add(a, False, None)
+                    add(b, True, None)
+        for t in grads:
+            add(t, False, None)
+        for t, ld in copies + copies_t:
+            if not ld:
+                add(t, True, None)
+        for ts in (values or {}).values():
+            for t in ts:
+                add(t, True, None)
+        spans.sort()
+        end, wrote = 0, 0       # the furthest ends of what was seen, read or written
+        for lo, hi, write, _ in spans:
+            if lo < wrote or (write and lo < end):
+                raise ValueError("AdamWTable: a buffer that the step writes overlaps another one")
+            end = max(end, hi)
+            wrote = max(wrote, hi) if write else wrote
+
+    def step(self, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, sumsq=None, max_norm=1.0, seed=0):
+        """One update, number *step + 1 (``step``: int64 device scalar, read and not advanced).  sumsq (f32,
+        one per clip group; llp_grad_sumsq): gradients are taken times min(1, max_norm / (norm + 1e-6)) of
+        their group.  ``seed`` keys the stochastic rounding of 8-bit moments."""
+        if step.dtype != torch.int64 or step.device != self.device:
+            raise TypeError(f"AdamWTable.step: step as an int64 tensor on {self.device}")
+        if sumsq is not None and (sumsq.dtype != torch.float32 or sumsq.device != self.device
+                                  or sumsq.numel() < self.n_groups or not sumsq.is_contiguous()):
+            raise TypeError(f"AdamWTable.step: sumsq as f32[{self.n_groups}] on {self.device}")
+        L = K.lib()
+        with K.on_device(self.device) as stream:
+            K.check(L.llp_adamw_step(self._descs.data_ptr(), self.n, self._work.data_ptr(), self._work.shape[0],
+                                     self.bits, self.param_code, self.grad_code, K.ptr(sumsq), max_norm, lr, betas[0],
+                                     betas[1], eps, weight_decay, step.data_ptr(), int(seed) & 0xFFFFFFFFFFFFFFFF,
+                                     stream), "llp_adamw_step")
+            if self._work_t is not None:
+                K.check(L.llp_adamw_copy_t(self._descs.data_ptr(), self._work_t.data_ptr(), self._work_t.shape[0],
+                                           self.param_code, stream), "llp_adamw_copy_t")
+
+    def values(self):
+        """Fill the ``values`` lists with the values of the 8-bit moments that the last step wrote."""
+        if self.values_dtype is None:
+            raise RuntimeError("AdamWTable: built without values")
+        L = K.lib()
+        with K.on_device(self.device) as stream:
+            K.check(L.llp_adamw_values(self._descs.data_ptr(), self._work.data_ptr(), self._work.shape[0],
+                                       K.dtype_code(self.values_dtype), stream), "llp_adamw_values")
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW on the HIP step: ``lr``, ``betas``, ``eps``, ``weight_decay`` as there (no amsgrad,
+    no maximize); ``state_bits`` 32 or 8; ``seed`` of the 8-bit moments' rounding.
+
+    Params in f32 or bf16 on the GPU, dense gradients of one dtype in a group.  ``state[p]`` holds
+    ``step`` and exp_avg / exp_avg_sq (f32, or uint8 codes with exp_avg_scale / exp_avg_sq_scale).  A
+    param without a gradient is left as it is; the update number is the group's, as long as its
+    params always step together.  After a first eager step on the same gradients' storage ``step()`` can
+    be captured into a graph (``zero_grad(set_to_none=False)``)."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
+        if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and 0 <= betas[0] < 1 and 0 <= betas[1] < 1):
+            raise ValueError("AdamW: lr, eps, weight_decay >= 0 and betas in [0, 1)")
+        if state_bits not in (32, 8):
+            raise ValueError("AdamW: state_bits 32 or 8")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        self.state_bits, self.seed = int(state_bits), int(seed)
+        self._tables = {}      # per group: (addresses, table, device step counter)
+
+    def init_state(self, p):
+        """state[p], made on first use."""
+        st = self.state[p]
+        if "exp_avg" not in st:
+            st["step"] = torch.tensor(0.0)
+            if self.state_bits == 8:
+                st["exp_avg"], st["exp_avg_scale"] = AdamWTable.state8(p.numel(), p.device)
+                st["exp_avg_sq"], st["exp_avg_sq_scale"] = AdamWTable.state8(p.numel(), p.device)
+            else:
+                st["exp_avg"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                st["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+        return st
+
+    def table(self, params, grads, **more):
+        """The AdamWTable of these params with this optimizer's state."""
+        sts = [self.init_state(p) for p in params]
+        if self.state_bits == 8:
+            more.update(exp_avg_scale=[s["exp_avg_scale"] for s in sts],
+                        exp_avg_sq_scale=[s["exp_avg_sq_scale"] for s in sts])
+        return AdamWTable([p.detach() for p in params], [g.detach() for g in grads], [s["exp_avg"] for s in sts],
+                          [s["exp_avg_sq"] for s in sts], **more)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for i, group in enumerate(self.param_groups):
+            params = [p for p in group["params"] if p.grad is not None]
+            if not params:
+                continue
+            grads = [p.grad for p in params]
+            if any(g.is_sparse for g in grads):
+                raise RuntimeError("AdamW: dense gradients only")
+            where = tuple((p.data_ptr(), g.data_ptr(), p.numel(), p.dtype, g.dtype,
+                           self.init_state(p)["exp_avg"].data_ptr()) for p, g in zip(params, grads))
+            at = self._tables.get(i)
+            if at is None or at[0] != where:
+                if params[0].is_cuda and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("AdamW: run one eager step on these gradients before a capture")
+                steps = {float(self.state[p]["step"]) for p in params} if at is None else {float(at[2].item())}
+                if len(steps) != 1:
+                    raise RuntimeError("AdamW: a group's params must have taken the same number of steps")
+                ctr = torch.full((1,), int(steps.pop()), dtype=torch.int64, device=params[0].device)
+                at = self._tables[i] = (where, self.table(params, grads), ctr)
+            _, table, ctr = at
+            table.step(ctr, lr=float(group["lr"]), betas=group["betas"], eps=float(group["eps"]),
+                       weight_decay=float(group["weight_decay"]), seed=self.seed + (i << 48))
+            with K.on_device(ctr.device):
+                K.increment(ctr)
+        return loss
+
+    def _sync_steps(self):
+        for i, (_, _, ctr) in self._tables.items():
+            n = float(ctr.item())
+            for p in self.param_groups[i]["params"]:
+                if "step" in self.state[p]:
+                    self.state[p]["step"] = torch.tensor(n)
+
+    def state_dict(self):
+        self._sync_steps()
+        return super().state_dict()
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        self._tables = {}
+        # the base class casts state to the param's dtype: the moments are taken over as they are
+        order = [p for g in self.param_groups for p in g["params"]]
+        ids = [k for g in state_dict["param_groups"] for k in g["params"]]
+        for k, p in zip(ids, order):
+            if k in state_dict["state"]:
+                for name, v in state_dict["state"][k].items():
+                    self.state[p][name] = v.detach().clone() if name == "step" else v.detach().clone().to(p.device)
+                if ("exp_avg_scale" in self.state[p]) != (self.state_bits == 8):
+                    raise ValueError(f"AdamW: the loaded moments are not in {self.state_bits} bits")

@@ -1,0 +1,181 @@
+"""Refusals and host-side checks of the low-bit operators (llp_mx, llp_optim and their C entries), on the CPU."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import llp_hip as K
+import llp_mx
+import llp_optim
+from oracle import lowbit_oracle as Q
+
+
+def _u8(*s):
+    return torch.zeros(*s, dtype=torch.uint8)
+
+
+def test_mx4_object_checks():
+    llp_mx.MX4(_u8(3, 64), _u8(3, 4), 100)
+    with pytest.raises(TypeError):
+        llp_mx.MX4(torch.zeros(3, 64), _u8(3, 4), 100)
+    with pytest.raises(ValueError):
+        llp_mx.MX4(_u8(3, 64), _u8(3, 4), 129)
+    with pytest.raises(ValueError):
+        llp_mx.MX4(_u8(3, 64), _u8(2, 4), 100)
+    with pytest.raises(ValueError):
+        llp_mx.MX4(_u8(64, 3).t(), _u8(3, 4), 100)
+    with pytest.raises(ValueError):
+        llp_mx.MX4(_u8(3, 0), _u8(3, 0), 0)
+
+
+def test_mx4_cpu_tensors_and_types_are_refused():
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        llp_mx.quantize(torch.zeros(2, 4))
+    with pytest.raises(TypeError):
+        llp_mx.quantize(torch.zeros(2, 4, dtype=torch.float64))
+    with pytest.raises(ValueError):
+        llp_mx.quantize(torch.zeros(4))
+    with pytest.raises(ValueError):
+        llp_mx.quantize(torch.zeros(4, 2).t())
+    w = llp_mx.MX4(_u8(3, 64), _u8(3, 4), 100)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        llp_mx.linear(torch.zeros(2, 100), w)
+
+
+def _entry(name, *args):
+    rc = getattr(K.load(), name)(*args)
+    return rc, K.load().llp_last_error().decode()
+
+
+def test_mx4_c_entries_refuse():
+    op = K.Operand(4096, None, None, None, 128, 0, None)
+    ok = K.Mx4(4096, 4096, 64, 4)
+    for bad, why in ((K.Mx4(4097, 4096, 64, 4), "16-B"), (K.Mx4(4096, 4096, 48, 4), "rows"), (K.Mx4(4096, 4096, 64, 2), "rows"),
+                     (K.Mx4(None, 4096, 64, 4), "null"), (K.Mx4(4096, 4098, 64, 4), "4-B"), (K.Mx4(4096, 4096, 72, 4), "16-B")):
+        rc, msg = _entry("llp_mx4_quantize", 0, 2, 128, C.byref(op), C.byref(bad), None)
+        assert rc == 10001 and why in msg, msg
+        rc, msg = _entry("llp_mx4_dequantize", 2, 128, C.byref(bad), 0, 4096, 128, None)
+        assert rc == 10001 and why in msg, msg
+        rc, msg = _entry("llp_gemm_nt_mx4", 2, 2, 128, 0, None, C.byref(bad), C.byref(ok), 4096, 2, 0, None, None, 0, None)
+        assert rc == 10001 and why in msg, msg
+    for args, why in (
+            ((2, 2, 128, 0, None, None, C.byref(ok), 4096, 2, 0, None, None, 0, None), "one of A"),
+            ((2, 2, 128, 0, C.byref(op), C.byref(ok), C.byref(ok), 4096, 2, 0, None, None, 0, None), "one of A"),
+            ((2, 2, 128, 0, None, C.byref(ok), C.byref(ok), None, 2, 0, None, None, 0, None), "one of C"),
+            ((2, 2, 128, 0, None, C.byref(ok), C.byref(ok), 4096, 2, 0, C.byref(ok), None, 0, None), "one of C"),
+            ((2, 2, 128, 0, None, C.byref(ok), C.byref(ok), 4096, 2, 0, None, None, 2, None), "act"),
+            ((2, 2, 128, 0, None, C.byref(ok), C.byref(ok), 4096, 1, 0, None, None, 0, None), "overlap"),
+            ((2, 2, 128, 2, C.byref(op), None, C.byref(ok), 4096, 2, 0, None, None, 0, None), "f32 or bf16"),
+            ((2, 2, 128, 0, None, C.byref(ok), C.byref(ok), 4096, 2, 2, None, None, 0, None), "f32 or bf16"),
+            ((2, 2, 0, 0, None, C.byref(ok), C.byref(ok), 4096, 2, 0, None, None, 0, None), "K >= 1"),
+            ((-1, 2, 8, 0, None, C.byref(ok), C.byref(ok), 4096, 2, 0, None, None, 0, None), "M, N >= 0")):
+        rc, msg = _entry("llp_gemm_nt_mx4", *args)
+        assert rc == 10001 and why in msg, (why, msg)
+    assert _entry("llp_gemm_nt_mx4", 0, 2, 128, 0, None, C.byref(ok), C.byref(ok), None, 0, 0, None, None, 0, None)[0] == 0
+    rows = K.Operand(4096, None, None, None, 128, 0, 4096)
+    assert "device row count" in _entry("llp_mx4_quantize", 0, 2, 128, C.byref(rows), C.byref(ok), None)[1]
+
+
+def test_adamw_c_entries_refuse():
+    good = dict(descs=4096, n=1, work=4096, n_work=1, bits=32, pt=0, gt=0, sumsq=None, mn=1.0, lr=0.1, b1=0.9, b2=0.99,
+                eps=1e-8, wd=0.0, step=4096, seed=0, stream=None)
+    for change, why in (({"bits": 16}, "state_bits"), ({"pt": 2}, "f32 or bf16"), ({"gt": -1}, "f32 or bf16"),
+                        ({"lr": -1.0}, "lr"), ({"b1": 1.0}, "betas"), ({"b2": -0.1}, "betas"), ({"wd": -1.0}, "weight_decay"),
+                        ({"eps": float("nan")}, "eps"), ({"descs": None}, "null"), ({"work": None}, "null"),
+                        ({"step": None}, "null"), ({"n": 70000}, "n_tensors"), ({"n_work": -1}, "n_work")):
+        rc, msg = _entry("llp_adamw_step", *{**good, **change}.values())
+        assert rc == 10001 and why in msg, (change, msg)
+    assert _entry("llp_adamw_step", *{**good, "n_work": 0}.values())[0] == 0
+    assert _entry("llp_adamw_values", 4096, 4096, 1, 2, None)[0] == 10001
+    assert _entry("llp_adamw_copy_t", None, 4096, 1, 0, None)[0] == 10001
+    L = K.load()
+    assert [L.llp_adamw_work_items(n) for n in (0, 1, 2048, 2049)] == [0, 1, 1, 2]
+    assert L.llp_adamw_copy_t_items(65, 64) == 2
+
+
+def _lists(n=40):
+    f = [torch.zeros(n)]
+    return f, [torch.zeros(n)], [torch.zeros(n)], [torch.zeros(n)]
+
+
+def test_adamw_table_refuses():
+    p, g, m, v = _lists()
+    T = llp_optim.AdamWTable
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        T(p, g, m, v)
+    with pytest.raises(ValueError, match="no params"):
+        T([], [], [], [])
+    with pytest.raises(ValueError):
+        T(p, g + g, m, v)
+    with pytest.raises(TypeError):
+        T(p, [torch.zeros(40, dtype=torch.float64)], m, v)
+    with pytest.raises(TypeError):
+        T(p, g, [torch.zeros(40, dtype=torch.bfloat16)], v)
+    with pytest.raises(ValueError):
+        T(p, [torch.zeros(39)], m, v)
+    with pytest.raises(ValueError):
+        T([torch.zeros(8, 10)[:, ::2]], g, m, v)
+    with pytest.raises(ValueError, match="together"):
+        T(p, g, [_u8(40)], [_u8(40)], exp_avg_scale=[_u8(2)])
+    with pytest.raises(ValueError, match="exp_avg_scale"):
+        T(p, g, [_u8(40)], [_u8(40)], exp_avg_scale=[_u8(1)], exp_avg_sq_scale=[_u8(2)])
+    with pytest.raises(ValueError, match="group"):
+        T(p, g, m, v, groups=[8])
+    with pytest.raises(ValueError, match="out has no"):
+        T(p, g, m, v, out={"exp_avg_scale": [_u8(2)]})
+    with pytest.raises(ValueError, match="values"):
+        T(p, g, m, v, values={"exp_avg": m})
+
+
+def test_adamw_table_refuses_overlaps():
+    flat = torch.zeros(400)
+    a, b, c, d = flat[:40], flat[100:140], flat[200:240], flat[300:340]
+    apart = llp_optim.AdamWTable._apart
+    none = [(None, 0)]
+
+    def ins(p=a, m=c, v=d):
+        return {"params": [p], "exp_avg": [m], "exp_avg_sq": [v]}
+
+    apart(ins(), ins(), [b], none, none, None)                                     # in place
+    apart(ins(), ins(p=flat[40:80]), [b], none, none, None)                        # beside
+    for bad in (ins(p=flat[20:60]), ins(p=b), ins(m=flat[210:250]), ins(v=c)):
+        with pytest.raises(ValueError, match="overlaps"):
+            apart(ins(), bad, [b], none, none, None)
+    with pytest.raises(ValueError, match="overlaps"):                              # the same param twice
+        apart({"params": [a, a], "exp_avg": [c, flat[250:290]], "exp_avg_sq": [d, flat[350:390]]},
+              {"params": [a, a], "exp_avg": [c, flat[250:290]], "exp_avg_sq": [d, flat[350:390]]}, [b, b], none * 2, none * 2, None)
+    with pytest.raises(ValueError, match="overlaps"):                              # a gradient that is the param
+        apart(ins(), ins(), [a], none, none, None)
+    apart(ins(), ins(), [b], [(flat[140:180], 0)], none, None)
+    with pytest.raises(ValueError, match="overlaps"):
+        apart(ins(), ins(), [b], [(flat[120:160], 0)], none, None)
+
+
+def test_adamw_optimizer_refuses():
+    p = torch.nn.Parameter(torch.zeros(4))
+    for kw in (dict(lr=-1), dict(betas=(1.0, 0.9)), dict(eps=-1), dict(weight_decay=-1), dict(state_bits=16)):
+        with pytest.raises(ValueError):
+            llp_optim.AdamW([p], **kw)
+    p.grad = torch.ones(4)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        llp_optim.AdamW([p]).step()
+
+
+def test_oracle_round_trips():
+    """The 64-bit restatement: every code is its own nearest, draws keep the mean, scales hold the block."""
+    for signed in (True, False):
+        lv = Q.levels8(signed)
+        assert (np.diff(lv) > 0).all() and lv[-1] == (448 if signed else 496)
+        # over all 65,536 draws the mean is the value, to one draw's share of the codes' distance (1/8)
+        for x in np.linspace(1, 1.0625, 9):
+            x = np.full(65536, x)
+            s = Q.scales8(x, signed)
+            c, _ = Q.round8(x if signed else x * x, np.arange(65536), s, signed)
+            q = Q.values8(c, s, signed)
+            assert abs((q if signed else q * q).mean() - (x[0] if signed else x[0] ** 2)) <= 0.125 / 65536 + 1e-12
+    v = np.concatenate([-Q.E2M1[::-1], Q.E2M1])[None, :]
+    assert np.array_equal(Q.mx4_round(v), v)
+    d = Q.draws16(20, 3, 5, 99)
+    from oracle import llp_oracle as O
+    assert d[9] == (int(O.philox_u32(99, 65536 * 5 + 3, np.array([4]))[0]) >> 16) & 0xFFFF
