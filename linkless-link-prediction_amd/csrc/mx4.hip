@@ -148,7 +148,7 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(int64_t M, int64_t 
 // Operand lane l: row l % 32, the 32 values of block l / 32 of the 64 that one instruction takes, in
 // 4 registers (16 consecutive bytes of codes), and that block's scale byte: a lane's own.
 struct Mx4Args {
-  int64_t M, N, K, Kp;
+  int64_t M, N, K, Kp, Np;   // Kp, Np: K and N up to 128
   const void* A;         // f32 / bf16 rows
   int64_t lda;
   llp_mx4 A4, W, C4;
@@ -256,6 +256,226 @@ __global__ __launch_bounds__(256) void gemm_mx4_tile_kernel(Mx4Args g) {
   }
 }
 
+// ---------------------------------------------------------------- the tiled product
+// A workgroup of 4 waves (2 x 2) computes 64 MI rows x 64 NI columns of C, a wave 32 MI x 32 NI.  128 of K
+// at a time go through LDS: 64 bytes of codes and 4 scale bytes per row of W and A, by LDS-DMA
+// (global_load_lds) into one of three stages, two of them in flight while one is read, so one barrier
+// a stage.  Chunk c (16 bytes) of row r lies at place c ^ (r / 2 % 4) of its row: the 8 lanes that read
+// LDS together then touch 32 different banks.
+template <int MI, int NI>
+struct Mx4Stage {
+  static constexpr int TM = 64 * MI, TN = 64 * NI, ROWS = TM + TN;
+  static constexpr int BYTES = ROWS * 68;
+  static constexpr int DATA = ROWS / 64;                        // 16-byte DMA instructions per wave
+  static constexpr int SCALE_ROWS = ROWS / 4;                   // scale words per wave
+  static constexpr int SCALE = (SCALE_ROWS + 63) / 64;          // 4-byte DMA instructions per wave
+};
+
+// LDS-DMA from inline asm: the kernel counts its own outstanding loads (vmcnt)
+__device__ __forceinline__ void dma16(uint32_t voff, const void* base, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void dma4(const void* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// the 16 values of one 32 x 32 tile: bias, ReLU, zero past N; returns the largest |value|'s bits
+__device__ __forceinline__ uint32_t tile_values(const float16_t& acc, const Mx4Args& g, int64_t n0, int h, float (&y)[16]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t n = n0 + 8 * j + 4 * h;
+    float b[4] = {0.f, 0.f, 0.f, 0.f};
+    if (g.bias) {
+      if (n + 4 <= g.N) {
+        const f4_any v = *reinterpret_cast<const f4_any*>(g.bias + n);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = v[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = n + i < g.N ? g.bias[n + i] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float v = acc[4 * j + i] + b[i];
+      if (g.relu) v = v < 0.f ? 0.f : v;   // a NaN stays
+      y[4 * j + i] = n + i < g.N ? v : 0.f;
+      top = umax(top, abs_bits(y[4 * j + i]));
+    }
+  }
+  return top;
+}
+
+template <int MI, int NI, int OUT>
+__global__ __launch_bounds__(256, 2) void gemm_mx4_kernel(Mx4Args g, int64_t tiles_n, int64_t tiles) {
+  using S = Mx4Stage<MI, NI>;
+  __shared__ __align__(16) uint8_t smem[3 * S::BYTES];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t tile = llp_xcd_block(blockIdx.x, tiles);
+  const int64_t n0 = tile % tiles_n * S::TN, m0 = tile / tiles_n * S::TM;
+
+  // this wave's DMA sources: 16 rows per data instruction (all of W's or all of A's), clamped to the last
+  // valid row (what lies past it is not stored)
+  uint32_t voff[S::DATA];
+  const uint8_t* base[S::DATA];
+#pragma unroll
+  for (int i = 0; i < S::DATA; ++i) {
+    const int r0 = (wave * S::DATA + i) * 16, r = r0 + (lane >> 2);
+    const bool isw = r0 < S::TN;
+    const int64_t last = isw ? g.N - 1 - n0 : g.M - 1 - m0;
+    int64_t row = isw ? r : r - S::TN;
+    row = row < last ? row : last;
+    voff[i] = (uint32_t)(row * (isw ? g.W.ld_codes : g.A4.ld_codes)) + (((lane & 3) ^ ((r >> 1) & 3)) << 4);
+    base[i] = isw ? (const uint8_t*)g.W.codes + n0 * g.W.ld_codes : (const uint8_t*)g.A4.codes + m0 * g.A4.ld_codes;
+  }
+  const uint8_t* sp[S::SCALE];
+#pragma unroll
+  for (int i = 0; i < S::SCALE; ++i) {
+    const int r = wave * S::SCALE_ROWS + i * 64 + lane;
+    const bool isw = r < S::TN;
+    const int64_t last = isw ? g.N - 1 : g.M - 1;
+    int64_t row = isw ? n0 + r : m0 + r - S::TN;
+    row = row < last ? row : last;
+    sp[i] = isw ? (const uint8_t*)g.W.scales + row * g.W.ld_scales : (const uint8_t*)g.A4.scales + row * g.A4.ld_scales;
+  }
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+  auto issue = [&](int64_t k, int buf) {
+    const uint32_t at = lds0 + buf * S::BYTES;
+#pragma unroll
+    for (int i = 0; i < S::DATA; ++i) dma16(voff[i], base[i] + k * 64, at + (wave * S::DATA + i) * 1024);
+#pragma unroll
+    for (int i = 0; i < S::SCALE; ++i)
+      if (S::SCALE_ROWS % 64 == 0 || i * 64 + lane < S::SCALE_ROWS)
+        dma4(sp[i] + k * 4, at + S::ROWS * 64 + (wave * S::SCALE_ROWS + i * 64) * 4);
+  };
+
+  const int wn = wave & 1, wm = wave >> 1, h = lane >> 5, li = lane & 31;
+  float16_t acc[NI][MI];
+#pragma unroll
+  for (int f = 0; f < NI; ++f)
+#pragma unroll
+    for (int e = 0; e < MI; ++e)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[f][e][i] = 0.f;
+  const int wrow = wn * 32 * NI + li, arow = S::TN + wm * 32 * MI + li, sw = (li >> 1) & 3;
+
+  const int64_t nk = g.Kp / 128;
+  issue(0, 0);
+  if (nk > 1) issue(1, 1);
+  int buf = 0;
+  for (int64_t k = 0; k < nk; ++k) {
+    if (k + 1 < nk) wait_vm<S::DATA + S::SCALE>();
+    else wait_vm<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (k + 2 < nk) issue(k + 2, buf == 0 ? 2 : buf - 1);
+    const uint8_t* st = smem + buf * S::BYTES;
+    int ws[NI], as[MI];
+#pragma unroll
+    for (int f = 0; f < NI; ++f) ws[f] = (int)(*(const uint32_t*)(st + S::ROWS * 64 + (wrow + 32 * f) * 4) >> (8 * h));
+#pragma unroll
+    for (int e = 0; e < MI; ++e) as[e] = (int)(*(const uint32_t*)(st + S::ROWS * 64 + (arow + 32 * e) * 4) >> (8 * h));
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      v8i w[NI], a[MI];
+#pragma unroll
+      for (int f = 0; f < NI; ++f) {
+        const u4v c = *(const u4v*)(st + (wrow + 32 * f) * 64 + (((2 * s + h) ^ sw) << 4));
+        w[f] = v8i{(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int e = 0; e < MI; ++e) {
+        const u4v c = *(const u4v*)(st + (arow + 32 * e) * 64 + (((2 * s + h) ^ sw) << 4));
+        a[e] = v8i{(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int f = 0; f < NI; ++f)
+#pragma unroll
+        for (int e = 0; e < MI; ++e)
+          acc[f][e] = s == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[f], a[e], acc[f][e], 4, 4, 0, ws[f], 0, as[e])
+                             : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[f], a[e], acc[f][e], 4, 4, 2, ws[f], 2, as[e]);
+    }
+    buf = buf == 2 ? 0 : buf + 1;
+  }
+
+#pragma unroll
+  for (int e = 0; e < MI; ++e) {
+    const int64_t m = m0 + (wm * MI + e) * 32 + li;
+    const bool live = m < g.M;
+#pragma unroll
+    for (int f = 0; f < NI; ++f) {
+      const int64_t nb = n0 + (wn * NI + f) * 32;
+      float y[16];
+      uint32_t top = tile_values(acc[f][e], g, nb, h, y);
+      if constexpr (OUT == 2) {
+        top = umax(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+        const uint32_t sc = mx4_scale(top);
+        const float q = mx4_scale_f32(sc);
+        uint32_t c[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) c[j] = sc == 255u ? 0u : mx4_codes(y + 8 * j, q);
+        // lane l holds the halves 4 h .. 4 h + 3 of each run of 8 columns: after the exchange lane l < 32 holds
+        // columns 0 .. 15 of its row, lane l + 32 columns 16 .. 31
+        const auto x = __builtin_amdgcn_permlane32_swap(c[0], c[1], false, false);
+        if (live && nb < g.Np) {
+          uint32_t* o = (uint32_t*)((uint8_t*)g.C4.codes + m * g.C4.ld_codes + nb / 2 + 8 * h);
+          o[0] = (x[0] & 0xFFFFu) | (x[1] << 16);
+          o[1] = (x[0] >> 16) | (x[1] & 0xFFFF0000u);
+          if (h == 0) ((uint8_t*)g.C4.scales)[m * g.C4.ld_scales + nb / 32] = (uint8_t)sc;
+        }
+      } else if constexpr (OUT == 1) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {   // 16 columns: 8 of them in each half of the wave after the exchange
+          uint32_t p[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[i] = (uint32_t)f2bf(y[8 * j + 2 * i]) | ((uint32_t)f2bf(y[8 * j + 2 * i + 1]) << 16);
+          const auto x0 = __builtin_amdgcn_permlane32_swap(p[0], p[2], false, false);
+          const auto x1 = __builtin_amdgcn_permlane32_swap(p[1], p[3], false, false);
+          const int64_t n = nb + 16 * j + 8 * h;
+          bf16_t* o = (bf16_t*)g.C + m * g.ldc + n;
+          const uint32_t d[4] = {x0[0], x1[0], x0[1], x1[1]};
+          if (live && n + 8 <= g.N) {
+            *reinterpret_cast<u4_any2*>(o) = u4_any2{d[0], d[1], d[2], d[3]};
+          } else if (live) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (n + i < g.N) o[i] = (bf16_t)(d[i >> 1] >> (16 * (i & 1)));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int64_t n = nb + 8 * j + 4 * h;
+          float* o = (float*)g.C + m * g.ldc + n;
+          if (live && n + 4 <= g.N) {
+            *reinterpret_cast<f4_any*>(o) = f4_any{y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]};
+          } else if (live) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (n + i < g.N) o[i] = y[4 * j + i];
+          }
+        }
+      }
+    }
+  }
+}
+
+template <int MI, int NI>
+int launch_tiled(const Mx4Args& g, int out, int64_t n_out, hipStream_t s) {
+  using S = Mx4Stage<MI, NI>;
+  const int64_t tn = (n_out + S::TN - 1) / S::TN, tiles = tn * ((g.M + S::TM - 1) / S::TM);
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(256), 0, s, g, tn, tiles); };
+  if (out == 0) go(gemm_mx4_kernel<MI, NI, 0>);
+  else if (out == 1) go(gemm_mx4_kernel<MI, NI, 1>);
+  else go(gemm_mx4_kernel<MI, NI, 2>);
+  LLP_LAUNCH_CHECK();
+  return LLP_OK;
+}
+
 int64_t pad128(int64_t k) { return (k + 127) / 128 * 128; }
 
 const char* bad_mx4(const llp_mx4* x, int64_t rows, int64_t K) {
@@ -317,7 +537,7 @@ extern "C" int llp_gemm_nt_mx4(int64_t M, int64_t N, int64_t K, int a_dtype, con
   const char* why = bad_mx4(W, N, K);
   LLP_CHECK_ARG(!why, "llp_gemm_nt_mx4: W: %s", why);
   Mx4Args g{};
-  g.M = M, g.N = N, g.K = K, g.Kp = pad128(K), g.W = *W, g.bias = bias, g.relu = act == LLP_ACT_RELU;
+  g.M = M, g.N = N, g.K = K, g.Kp = pad128(K), g.Np = pad128(N), g.W = *W, g.bias = bias, g.relu = act == LLP_ACT_RELU;
   int src = 0, out = 2;
   if (A4) {
     why = bad_mx4(A4, M, K);
@@ -341,6 +561,9 @@ extern "C" int llp_gemm_nt_mx4(int64_t M, int64_t N, int64_t K, int a_dtype, con
     out = c_dtype == LLP_F32 ? 0 : 1;
   }
   const int64_t nt = (C4 ? pad128(N) : N + 31) / 32, mt = (M + 31) / 32;
+  // (32-bit row offsets within a tile)
+  const bool near = W->ld_codes < (1 << 23) && (!A4 || A4->ld_codes < (1 << 23));
+  if (A4 && near && nt * mt >= 1024) return launch_tiled<2, 4>(g, out, C4 ? pad128(N) : N, (hipStream_t)stream);
   auto go = [&](auto kernel) -> int {
     // the grid's second dimension ends at 65,535: longer M in slices
     for (int64_t b = 0; b < mt; b += 65535) {
