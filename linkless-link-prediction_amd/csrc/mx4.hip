@@ -258,17 +258,22 @@ __global__ __launch_bounds__(256) void gemm_mx4_tile_kernel(Mx4Args g) {
 
 // ---------------------------------------------------------------- the tiled product
 // A workgroup of 4 waves (2 x 2) computes 64 MI rows x 64 NI columns of C, a wave 32 MI x 32 NI.  128 of K
-// at a time go through LDS: 64 bytes of codes and 4 scale bytes per row of W and A, by LDS-DMA
-// (global_load_lds) into one of three stages, two of them in flight while one is read, so one barrier
-// a stage.  Chunk c (16 bytes) of row r lies at place c ^ (r / 2 % 4) of its row: the 8 lanes that read
-// LDS together then touch 32 different banks.
+// at a time (a step) go through LDS: 64 bytes of codes per row of W and A, by LDS-DMA (global_load_lds)
+// into one of three stages, two of them in flight while one is read, so one barrier a step.  Chunk c (16
+// bytes) of row r lies at place c ^ place(r) of its row, so that the 8 (16) lanes that read LDS
+// together, 8 (16) neighbouring rows at one c, touch 32 (64) different banks.  The scale bytes of 4 steps (16 per row) come at once: 4 of them a step
+// would touch as many cache lines as the codes do.  They are read into registers at the first of
+// the 4 steps, and the next 16 follow into the same LDS once every wave has read.  SHORT: K of at most
+// 3 steps, whose rows hold fewer than 16 scale bytes: 4 bytes at a time, all before the first step.
+__device__ __forceinline__ int place(int r) { return ((r >> 2) & 1) | ((((r >> 1) ^ (r >> 3)) & 1) << 1); }
 template <int MI, int NI>
 struct Mx4Stage {
   static constexpr int TM = 64 * MI, TN = 64 * NI, ROWS = TM + TN;
-  static constexpr int BYTES = ROWS * 68;
-  static constexpr int DATA = ROWS / 64;                        // 16-byte DMA instructions per wave
-  static constexpr int SCALE_ROWS = ROWS / 4;                   // scale words per wave
-  static constexpr int SCALE = (SCALE_ROWS + 63) / 64;          // 4-byte DMA instructions per wave
+  static constexpr int BYTES = ROWS * 64;
+  static constexpr int DATA = ROWS / 64;                        // 16-byte DMA instructions per wave and step
+  static constexpr int SCALE_ROWS = ROWS / 4;                   // rows whose scales a wave fetches
+  static constexpr int SCALE = (SCALE_ROWS + 63) / 64;          // DMA instructions for them
+  static constexpr int LDS = 3 * BYTES + ROWS * 16 + 16;        // (a read of 16 bytes may begin 12 late)
 };
 
 // LDS-DMA from inline asm: the kernel counts its own outstanding loads (vmcnt)
@@ -278,43 +283,123 @@ __device__ __forceinline__ void dma16(uint32_t voff, const void* base, uint32_t 
 __device__ __forceinline__ void dma4(const void* p, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds) : "memory");
 }
+__device__ __forceinline__ void dma16p(const void* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory");
+}
 template <int N>
 __device__ __forceinline__ void wait_vm() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// the 16 values of one 32 x 32 tile: bias, ReLU, zero past N; returns the largest |value|'s bits
-__device__ __forceinline__ uint32_t tile_values(const float16_t& acc, const Mx4Args& g, int64_t n0, int h, float (&y)[16]) {
-  uint32_t top = 0;
+// bias of a lane's 16 columns n0 + 8 j + 4 h + i (zero past N)
+__device__ __forceinline__ void tile_bias(const Mx4Args& g, int64_t n0, int h, bool full, float (&b)[16]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int64_t n = n0 + 8 * j + 4 * h;
-    float b[4] = {0.f, 0.f, 0.f, 0.f};
+    f4_any v = {0.f, 0.f, 0.f, 0.f};
     if (g.bias) {
-      if (n + 4 <= g.N) {
-        const f4_any v = *reinterpret_cast<const f4_any*>(g.bias + n);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) b[i] = v[i];
+      if (full || n + 4 <= g.N) {
+        v = *reinterpret_cast<const f4_any*>(g.bias + n);
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) b[i] = n + i < g.N ? g.bias[n + i] : 0.f;
+        for (int i = 0; i < 4; ++i) v[i] = n + i < g.N ? g.bias[n + i] : 0.f;
       }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float v = acc[4 * j + i] + b[i];
-      if (g.relu) v = v < 0.f ? 0.f : v;   // a NaN stays
-      y[4 * j + i] = n + i < g.N ? v : 0.f;
-      top = umax(top, abs_bits(y[4 * j + i]));
-    }
+    for (int i = 0; i < 4; ++i) b[4 * j + i] = v[i];
   }
-  return top;
 }
 
-template <int MI, int NI, int OUT>
+// bias and ReLU (a NaN stays: IEEE maximum, not the maxNum of fmaxf)
+__device__ __forceinline__ float relu_or(float x, float floor) { return __builtin_elementwise_maximum(x, floor); }
+__device__ __forceinline__ void tile_act(const float16_t& acc, const float (&b)[16], int relu, float (&y)[16]) {
+  const float floor = relu ? 0.f : -__builtin_inff();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) y[i] = relu_or(acc[i] + b[i], floor);
+}
+
+// the larger of a lane's value and that of lane ^ 32
+__device__ __forceinline__ uint32_t halves_max(uint32_t x) {
+  const auto p = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return umax(p[0], p[1]);
+}
+
+// MXFP4 of the 32 columns of a tile's row (16 in lane l, 16 in lane l ^ 32): the scale byte, and in c the
+// codes of columns 0 .. 15 in lanes below 32, of 16 .. 31 above
+__device__ __forceinline__ void tile_codes(const float (&y)[16], int h, uint32_t (&c)[2], uint32_t& sc) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) top = umax(top, abs_bits(y[i]));
+  sc = mx4_scale(halves_max(top));
+  const float q = mx4_scale_f32(sc);
+  uint32_t d[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) d[j] = sc == 255u ? 0u : mx4_codes(y + 8 * j, q);
+  // d holds the halves 4 h .. 4 h + 3 of each run of 8 columns
+  const auto x = __builtin_amdgcn_permlane32_swap(d[0], d[1], false, false);
+  c[0] = (x[0] & 0xFFFFu) | (x[1] << 16);
+  c[1] = (x[0] >> 16) | (x[1] & 0xFFFF0000u);
+}
+
+// One 32 x 32 tile of a wave's result stored: bias, ReLU, the output's type.  FULL: the whole tile lies
+// within M and N.
+template <int OUT, bool FULL>
+__device__ __forceinline__ void store_tile(const Mx4Args& g, const float16_t& acc, const float (&b)[16], int64_t m,
+                                           int64_t nb, int h) {
+  const bool live = FULL || m < g.M;
+  float y[16];
+  tile_act(acc, b, g.relu, y);
+  if constexpr (OUT == 2) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (!FULL && nb + 8 * (i >> 2) + 4 * h + (i & 3) >= g.N) y[i] = 0.f;
+    uint32_t c[2], sc;
+    tile_codes(y, h, c, sc);
+    if (live && (FULL || nb < g.Np)) {
+      uint32_t* o = (uint32_t*)((uint8_t*)g.C4.codes + m * g.C4.ld_codes + nb / 2 + 8 * h);
+      o[0] = c[0];
+      o[1] = c[1];
+      if (h == 0) ((uint8_t*)g.C4.scales)[m * g.C4.ld_scales + nb / 32] = (uint8_t)sc;
+    }
+  } else if constexpr (OUT == 1) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {   // 16 columns: 8 of them in each half of the wave after the exchange
+      uint32_t p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = (uint32_t)f2bf(y[8 * j + 2 * i]) | ((uint32_t)f2bf(y[8 * j + 2 * i + 1]) << 16);
+      const auto x0 = __builtin_amdgcn_permlane32_swap(p[0], p[2], false, false);
+      const auto x1 = __builtin_amdgcn_permlane32_swap(p[1], p[3], false, false);
+      const int64_t n = nb + 16 * j + 8 * h;
+      bf16_t* o = (bf16_t*)g.C + m * g.ldc + n;
+      const uint32_t d[4] = {x0[0], x1[0], x0[1], x1[1]};
+      if (FULL || (live && n + 8 <= g.N)) {
+        *reinterpret_cast<u4_any2*>(o) = u4_any2{d[0], d[1], d[2], d[3]};
+      } else if (live) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (n + i < g.N) o[i] = (bf16_t)(d[i >> 1] >> (16 * (i & 1)));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t n = nb + 8 * j + 4 * h;
+      float* o = (float*)g.C + m * g.ldc + n;
+      if (FULL || (live && n + 4 <= g.N)) {
+        *reinterpret_cast<f4_any*>(o) = f4_any{y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]};
+      } else if (live) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n + i < g.N) o[i] = y[4 * j + i];
+      }
+    }
+  }
+}
+
+template <int MI, int NI, int OUT, bool SHORT>
 __global__ __launch_bounds__(256, 2) void gemm_mx4_kernel(Mx4Args g, int64_t tiles_n, int64_t tiles) {
   using S = Mx4Stage<MI, NI>;
-  __shared__ __align__(16) uint8_t smem[3 * S::BYTES];
+  __shared__ __align__(16) uint8_t smem[S::LDS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t tile = llp_xcd_block(blockIdx.x, tiles);
   const int64_t n0 = tile % tiles_n * S::TN, m0 = tile / tiles_n * S::TM;
@@ -330,7 +415,7 @@ __global__ __launch_bounds__(256, 2) void gemm_mx4_kernel(Mx4Args g, int64_t til
     const int64_t last = isw ? g.N - 1 - n0 : g.M - 1 - m0;
     int64_t row = isw ? r : r - S::TN;
     row = row < last ? row : last;
-    voff[i] = (uint32_t)(row * (isw ? g.W.ld_codes : g.A4.ld_codes)) + (((lane & 3) ^ ((r >> 1) & 3)) << 4);
+    voff[i] = (uint32_t)(row * (isw ? g.W.ld_codes : g.A4.ld_codes)) + (((lane & 3) ^ place(r)) << 4);
     base[i] = isw ? (const uint8_t*)g.W.codes + n0 * g.W.ld_codes : (const uint8_t*)g.A4.codes + m0 * g.A4.ld_codes;
   }
   const uint8_t* sp[S::SCALE];
@@ -344,14 +429,28 @@ __global__ __launch_bounds__(256, 2) void gemm_mx4_kernel(Mx4Args g, int64_t til
     sp[i] = isw ? (const uint8_t*)g.W.scales + row * g.W.ld_scales : (const uint8_t*)g.A4.scales + row * g.A4.ld_scales;
   }
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
-  auto issue = [&](int64_t k, int buf) {
+  const int nk = (int)(g.Kp / 128);
+  constexpr int SC = 3 * S::BYTES;   // the scales' place
+  auto issue = [&](int k, int buf) {
     const uint32_t at = lds0 + buf * S::BYTES;
 #pragma unroll
-    for (int i = 0; i < S::DATA; ++i) dma16(voff[i], base[i] + k * 64, at + (wave * S::DATA + i) * 1024);
+    for (int i = 0; i < S::DATA; ++i) dma16(voff[i], base[i] + (int64_t)k * 64, at + (wave * S::DATA + i) * 1024);
+  };
+  // scale bytes of steps 4 c .. 4 c + 3; the last 16 of the row where fewer are left
+  auto issue_scales = [&](int c) {
+    if constexpr (SHORT) {
+      for (int k = 0; k < nk; ++k)
 #pragma unroll
-    for (int i = 0; i < S::SCALE; ++i)
-      if (S::SCALE_ROWS % 64 == 0 || i * 64 + lane < S::SCALE_ROWS)
-        dma4(sp[i] + k * 4, at + S::ROWS * 64 + (wave * S::SCALE_ROWS + i * 64) * 4);
+        for (int i = 0; i < S::SCALE; ++i)
+          if (S::SCALE_ROWS % 64 == 0 || i * 64 + lane < S::SCALE_ROWS)
+            dma4(sp[i] + 4 * k, lds0 + SC + k * S::ROWS * 4 + (wave * S::SCALE_ROWS + i * 64) * 4);
+    } else {
+      const int at = 16 * c < 4 * nk - 16 ? 16 * c : 4 * nk - 16;
+#pragma unroll
+      for (int i = 0; i < S::SCALE; ++i)
+        if (S::SCALE_ROWS % 64 == 0 || i * 64 + lane < S::SCALE_ROWS)
+          dma16p(sp[i] + at, lds0 + SC + (wave * S::SCALE_ROWS + i * 64) * 16);
+    }
   };
 
   const int wn = wave & 1, wm = wave >> 1, h = lane >> 5, li = lane & 31;
@@ -362,104 +461,132 @@ __global__ __launch_bounds__(256, 2) void gemm_mx4_kernel(Mx4Args g, int64_t til
     for (int e = 0; e < MI; ++e)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[f][e][i] = 0.f;
-  const int wrow = wn * 32 * NI + li, arow = S::TN + wm * 32 * MI + li, sw = (li >> 1) & 3;
+  const int wrow = wn * 32 * NI + li, arow = S::TN + wm * 32 * MI + li, sw = place(li);
 
-  const int64_t nk = g.Kp / 128;
+  // a wave's scale words of 4 steps; byte 2 s + h of a word belongs to the lane: shifted to bytes 0 and 2
+  uint32_t ws[NI][4], as[MI][4];
+  auto read_scales = [&](int c) {
+    const int late = SHORT ? 0 : (16 * c < 4 * nk - 16 ? 0 : 16 * c - (4 * nk - 16));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (SHORT && j == 3) break;
+      const uint8_t* at = smem + SC + (SHORT ? j * S::ROWS * 4 : 4 * j + late);
+      constexpr int P = SHORT ? 4 : 16;
+#pragma unroll
+      for (int f = 0; f < NI; ++f) ws[f][j] = *(const uint32_t*)(at + (wrow + 32 * f) * P) >> (8 * h);
+#pragma unroll
+      for (int e = 0; e < MI; ++e) as[e][j] = *(const uint32_t*)(at + (arow + 32 * e) * P) >> (8 * h);
+    }
+  };
+  issue_scales(0);
   issue(0, 0);
   if (nk > 1) issue(1, 1);
   int buf = 0;
-  for (int64_t k = 0; k < nk; ++k) {
-    if (k + 1 < nk) wait_vm<S::DATA + S::SCALE>();
-    else wait_vm<0>();
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (k + 2 < nk) issue(k + 2, buf == 0 ? 2 : buf - 1);
-    const uint8_t* st = smem + buf * S::BYTES;
-    int ws[NI], as[MI];
+  for (int c = 0; 4 * c < nk; ++c) {
 #pragma unroll
-    for (int f = 0; f < NI; ++f) ws[f] = (int)(*(const uint32_t*)(st + S::ROWS * 64 + (wrow + 32 * f) * 4) >> (8 * h));
+    for (int j = 0; j < 4; ++j) {
+      const int k = 4 * c + j;
+      if (k < nk) {
+        // what was issued in the last step may stay in flight: one stage, after step 1 the scales too
+        if (k + 1 == nk) wait_vm<0>();
+        else if (!SHORT && j == 2 && 4 * c + 4 < nk) wait_vm<S::DATA + S::SCALE>();
+        else wait_vm<S::DATA>();
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (!SHORT && j == 1 && 4 * c + 4 < nk) issue_scales(c + 1);
+        if (k + 2 < nk) issue(k + 2, buf == 0 ? 2 : buf - 1);
+        if (j == 0) read_scales(c);
+        const uint8_t* st = smem + buf * S::BYTES;
 #pragma unroll
-    for (int e = 0; e < MI; ++e) as[e] = (int)(*(const uint32_t*)(st + S::ROWS * 64 + (arow + 32 * e) * 4) >> (8 * h));
+        for (int s = 0; s < 2; ++s) {
+          v8i w[NI], a[MI];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      v8i w[NI], a[MI];
+          for (int f = 0; f < NI; ++f) {
+            const u4v q = *(const u4v*)(st + (wrow + 32 * f) * 64 + (((2 * s + h) ^ sw) << 4));
+            w[f] = v8i{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0};
+          }
 #pragma unroll
-      for (int f = 0; f < NI; ++f) {
-        const u4v c = *(const u4v*)(st + (wrow + 32 * f) * 64 + (((2 * s + h) ^ sw) << 4));
-        w[f] = v8i{(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
+          for (int e = 0; e < MI; ++e) {
+            const u4v q = *(const u4v*)(st + (arow + 32 * e) * 64 + (((2 * s + h) ^ sw) << 4));
+            a[e] = v8i{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0};
+          }
+#pragma unroll
+          for (int f = 0; f < NI; ++f)
+#pragma unroll
+            for (int e = 0; e < MI; ++e)
+              acc[f][e] = s == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[f], a[e], acc[f][e], 4, 4, 0, (int)ws[f][j], 0, (int)as[e][j])
+                                 : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[f], a[e], acc[f][e], 4, 4, 2, (int)ws[f][j], 2, (int)as[e][j]);
+        }
+        buf = buf == 2 ? 0 : buf + 1;
       }
-#pragma unroll
-      for (int e = 0; e < MI; ++e) {
-        const u4v c = *(const u4v*)(st + (arow + 32 * e) * 64 + (((2 * s + h) ^ sw) << 4));
-        a[e] = v8i{(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
-      }
-#pragma unroll
-      for (int f = 0; f < NI; ++f)
-#pragma unroll
-        for (int e = 0; e < MI; ++e)
-          acc[f][e] = s == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[f], a[e], acc[f][e], 4, 4, 0, ws[f], 0, as[e])
-                             : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[f], a[e], acc[f][e], 4, 4, 2, ws[f], 2, as[e]);
     }
-    buf = buf == 2 ? 0 : buf + 1;
   }
 
+  const bool full = m0 + S::TM <= g.M && n0 + S::TN <= g.N;
+  if constexpr (OUT != 0) {
+    // Through LDS, so that a store covers whole lines of the output's rows (the registers hold runs of 8 bytes,
+    // or 2 of codes, in 32 rows).  A wave writes and reads its own part.
+    if (full) {
+      constexpr int BYTES = OUT == 1 ? 64 * NI : 16 * NI, ROW = BYTES + 16;   // 4 banks on from row to row
+      constexpr int PART = 32 * MI * (ROW + (OUT == 2 ? NI : 0));
+      static_assert(4 * PART <= S::LDS, "C tile in LDS");
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the last stage was read by all
+      uint8_t* part = smem + wave * PART;
 #pragma unroll
-  for (int e = 0; e < MI; ++e) {
-    const int64_t m = m0 + (wm * MI + e) * 32 + li;
-    const bool live = m < g.M;
+      for (int f = 0; f < NI; ++f) {
+        const int64_t nb = n0 + (wn * NI + f) * 32;
+        float b[16];
+        tile_bias(g, nb, h, true, b);
 #pragma unroll
-    for (int f = 0; f < NI; ++f) {
-      const int64_t nb = n0 + (wn * NI + f) * 32;
-      float y[16];
-      uint32_t top = tile_values(acc[f][e], g, nb, h, y);
-      if constexpr (OUT == 2) {
-        top = umax(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-        const uint32_t sc = mx4_scale(top);
-        const float q = mx4_scale_f32(sc);
-        uint32_t c[2];
+        for (int e = 0; e < MI; ++e) {
+          float y[16];
+          tile_act(acc[f][e], b, g.relu, y);
+          uint8_t* at = part + (32 * e + li) * ROW;
+          if constexpr (OUT == 1) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) c[j] = sc == 255u ? 0u : mx4_codes(y + 8 * j, q);
-        // lane l holds the halves 4 h .. 4 h + 3 of each run of 8 columns: after the exchange lane l < 32 holds
-        // columns 0 .. 15 of its row, lane l + 32 columns 16 .. 31
-        const auto x = __builtin_amdgcn_permlane32_swap(c[0], c[1], false, false);
-        if (live && nb < g.Np) {
-          uint32_t* o = (uint32_t*)((uint8_t*)g.C4.codes + m * g.C4.ld_codes + nb / 2 + 8 * h);
-          o[0] = (x[0] & 0xFFFFu) | (x[1] << 16);
-          o[1] = (x[0] >> 16) | (x[1] & 0xFFFF0000u);
-          if (h == 0) ((uint8_t*)g.C4.scales)[m * g.C4.ld_scales + nb / 32] = (uint8_t)sc;
-        }
-      } else if constexpr (OUT == 1) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {   // 16 columns: 8 of them in each half of the wave after the exchange
-          uint32_t p[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) p[i] = (uint32_t)f2bf(y[8 * j + 2 * i]) | ((uint32_t)f2bf(y[8 * j + 2 * i + 1]) << 16);
-          const auto x0 = __builtin_amdgcn_permlane32_swap(p[0], p[2], false, false);
-          const auto x1 = __builtin_amdgcn_permlane32_swap(p[1], p[3], false, false);
-          const int64_t n = nb + 16 * j + 8 * h;
-          bf16_t* o = (bf16_t*)g.C + m * g.ldc + n;
-          const uint32_t d[4] = {x0[0], x1[0], x0[1], x1[1]};
-          if (live && n + 8 <= g.N) {
-            *reinterpret_cast<u4_any2*>(o) = u4_any2{d[0], d[1], d[2], d[3]};
-          } else if (live) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (n + i < g.N) o[i] = (bf16_t)(d[i >> 1] >> (16 * (i & 1)));
-          }
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int64_t n = nb + 8 * j + 4 * h;
-          float* o = (float*)g.C + m * g.ldc + n;
-          if (live && n + 4 <= g.N) {
-            *reinterpret_cast<f4_any*>(o) = f4_any{y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]};
-          } else if (live) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (n + i < g.N) o[i] = y[4 * j + i];
+            for (int j = 0; j < 4; ++j) {
+              uint2 p;
+              p.x = (uint32_t)f2bf(y[4 * j]) | ((uint32_t)f2bf(y[4 * j + 1]) << 16);
+              p.y = (uint32_t)f2bf(y[4 * j + 2]) | ((uint32_t)f2bf(y[4 * j + 3]) << 16);
+              *reinterpret_cast<uint2*>(at + 64 * f + 16 * j + 8 * h) = p;
+            }
+          } else {
+            uint32_t c[2], sc;
+            tile_codes(y, h, c, sc);
+            *reinterpret_cast<uint2*>(at + 16 * f + 8 * h) = make_uint2(c[0], c[1]);
+            if (h == 0) part[32 * MI * ROW + (32 * e + li) * NI + f] = (uint8_t)sc;
           }
         }
       }
+      constexpr int LANES = BYTES / 16;       // lanes to a row
+#pragma unroll
+      for (int i = 0; i < 32 * MI * LANES / 64; ++i) {
+        const int r = i * (64 / LANES) + lane / LANES, q = lane % LANES;
+        const u4v v = *reinterpret_cast<const u4v*>(part + r * ROW + 16 * q);
+        const int64_t m = m0 + wm * 32 * MI + r;
+        if constexpr (OUT == 1)
+          *reinterpret_cast<u4_any2*>((bf16_t*)g.C + m * g.ldc + n0 + wn * 32 * NI + 8 * q) = u4_any2{v[0], v[1], v[2], v[3]};
+        else
+          *reinterpret_cast<u4v*>((uint8_t*)g.C4.codes + m * g.C4.ld_codes + (n0 + wn * 32 * NI) / 2 + 16 * q) = v;
+      }
+      if constexpr (OUT == 2) {
+        static_assert(NI == 4, "a row's scales as one word");
+        for (int r = lane; r < 32 * MI; r += 64)
+          *(uint32_t*)((uint8_t*)g.C4.scales + (m0 + wm * 32 * MI + r) * g.C4.ld_scales + n0 / 32 + wn * NI) =
+              *(const uint32_t*)(part + 32 * MI * ROW + r * NI);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int f = 0; f < NI; ++f) {
+    const int64_t nb = n0 + (wn * NI + f) * 32;
+    float b[16];
+    tile_bias(g, nb, h, full, b);
+#pragma unroll
+    for (int e = 0; e < MI; ++e) {
+      const int64_t m = m0 + (wm * MI + e) * 32 + li;
+      if (full) store_tile<OUT, true>(g, acc[f][e], b, m, nb, h);
+      else store_tile<OUT, false>(g, acc[f][e], b, m, nb, h);
     }
   }
 }
@@ -469,9 +596,8 @@ int launch_tiled(const Mx4Args& g, int out, int64_t n_out, hipStream_t s) {
   using S = Mx4Stage<MI, NI>;
   const int64_t tn = (n_out + S::TN - 1) / S::TN, tiles = tn * ((g.M + S::TM - 1) / S::TM);
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(256), 0, s, g, tn, tiles); };
-  if (out == 0) go(gemm_mx4_kernel<MI, NI, 0>);
-  else if (out == 1) go(gemm_mx4_kernel<MI, NI, 1>);
-  else go(gemm_mx4_kernel<MI, NI, 2>);
+  if (g.Kp <= 384) out == 0 ? go(gemm_mx4_kernel<MI, NI, 0, true>) : out == 1 ? go(gemm_mx4_kernel<MI, NI, 1, true>) : go(gemm_mx4_kernel<MI, NI, 2, true>);
+  else out == 0 ? go(gemm_mx4_kernel<MI, NI, 0, false>) : out == 1 ? go(gemm_mx4_kernel<MI, NI, 1, false>) : go(gemm_mx4_kernel<MI, NI, 2, false>);
   LLP_LAUNCH_CHECK();
   return LLP_OK;
 }

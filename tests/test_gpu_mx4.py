@@ -230,6 +230,15 @@ def test_linear_nan_stays_in_its_row():
         y = m.linear(x[rows], w, relu=True)
         bad = torch.isnan(y)
         assert bad[3].all() and not torch.cat([bad[:3], bad[4:]]).any()
+    big, wide = torch.randn(9000, 256, device=DEV), m.quantize(torch.randn(320, 256, device=DEV))
+    for i in (0, 130, 8999):
+        big[i, 200] = float("inf")
+    want = torch.zeros(9000, dtype=torch.bool, device=DEV)
+    want[[0, 130, 8999]] = True
+    for od in (torch.float32, torch.bfloat16, "mx4"):
+        y = m.linear(big, wide, torch.ones(320, device=DEV), relu=True, out_dtype=od)
+        bad = torch.isnan(m.dequantize(y) if od == "mx4" else y)
+        assert torch.equal(bad.all(1), want) and torch.equal(bad.any(1), want)
     q = m.dequantize(m.linear(x, w, out_dtype="mx4"))
     assert torch.isnan(q[3]).all() and torch.isfinite(torch.cat([q[:3], q[4:]])).all()
 
