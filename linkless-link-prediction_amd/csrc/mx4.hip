@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <stdlib.h>
 
 #include "llp_common.h"
 
@@ -21,6 +22,7 @@ __device__ __forceinline__ float as_f32<bf16_t>(bf16_t x) { return bf2f(x); }
 
 typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u4_any2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u4_any4 __attribute__((ext_vector_type(4), aligned(4)));
 
 // 8 values at any element offset (gfx950's global loads need no alignment), zeros past n
 __device__ __forceinline__ void load8(const float* p, int n, float (&x)[8]) {
@@ -260,8 +262,8 @@ __global__ __launch_bounds__(256) void gemm_mx4_tile_kernel(Mx4Args g) {
 // A workgroup of 4 waves (2 x 2) computes 64 MI rows x 64 NI columns of C, a wave 32 MI x 32 NI.  128 of K
 // at a time (a step) go through LDS: 64 bytes of codes per row of W and A, by LDS-DMA (global_load_lds)
 // into one of three stages, two of them in flight while one is read, so one barrier a step.  Chunk c (16
-// bytes) of row r lies at place c ^ place(r) of its row, so that the 8 (16) lanes that read LDS
-// together, 8 (16) neighbouring rows at one c, touch 32 (64) different banks.  The scale bytes of 4 steps (16 per row) come at once: 4 of them a step
+// bytes) of row r lies at place c ^ place(r) of its row, so that the 16 lanes that read LDS together
+// (neighbouring rows at one c) touch all 64 banks.  The scale bytes of 4 steps (16 per row) come at once: 4 of them a step
 // would touch as many cache lines as the codes do.  They are read into registers at the first of
 // the 4 steps, and the next 16 follow into the same LDS once every wave has read.  SHORT: K of at most
 // 3 steps, whose rows hold fewer than 16 scale bytes: 4 bytes at a time, all before the first step.
@@ -602,6 +604,194 @@ int launch_tiled(const Mx4Args& g, int out, int64_t n_out, hipStream_t s) {
   return LLP_OK;
 }
 
+// ---------------------------------------------------------------- the wide product
+// What bounds the tiled kernel on long K is the number of its requests to L2: 64 bytes each, 480 a step for
+// 128 x 256 columns (126 M for 65536 x 8192 x 2048, 78 % of what the L2 channels take in its time, the matrix
+// units at 42 %).  Here a step is 256 of K, so that a row's codes are a whole line of 128 bytes, and a tile 256 x 256,
+// a third of the requests.  One workgroup of 8 waves (2 x 4: 128 rows x 64 columns each) per CU takes tile after
+// tile; the steps of all its tiles are one sequence, the codes of the next step (the next tile's first) arriving in one
+// half of LDS while the other is read.  Row r's chunk c lies at place c ^ place8(r) of its 128 bytes.  K a
+// multiple of 256, at least 512.
+struct Mx4Wide {
+  static constexpr int T = 256, STAGE = 2 * T * 128, SC = 2 * STAGE, OUTB = SC + 2 * T * 16, LDS = OUTB + 8 * 2560;
+};
+static_assert(Mx4Wide::LDS <= 163840, "LDS of a CU");
+__device__ __forceinline__ int place8(int r) { return (r >> 1) & 7; }
+
+template <int OUT>
+__global__ __launch_bounds__(512, 2) void gemm_mx4_wide_kernel(Mx4Args g, int64_t tiles_n, int64_t tiles) {
+  using S = Mx4Wide;
+  __shared__ __align__(16) uint8_t smem[S::LDS];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = lane >> 5, li = lane & 31;
+  const int ns = (int)(g.Kp / 256), row_scales = (int)(g.Kp / 32);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+  // tiles are dealt in turns of gridDim.x; within a turn each XCD has a contiguous range of them
+  auto tile_of = [&](int64_t turn) { return turn * gridDim.x + llp_xcd_block(blockIdx.x, gridDim.x); };
+
+  // DMA sources of the tile that is being fetched: waves 0 .. 3 W's rows, 4 .. 7 A's, 64 each, 8 rows of 128 bytes an
+  // instruction; rows past the last valid one repeat it
+  const bool isw = wave < 4;
+  const uint8_t* const codes = (const uint8_t*)(isw ? g.W.codes : g.A4.codes);
+  const uint8_t* const scales = (const uint8_t*)(isw ? g.W.scales : g.A4.scales);
+  const int64_t ldc = isw ? g.W.ld_codes : g.A4.ld_codes, lds = isw ? g.W.ld_scales : g.A4.ld_scales;
+  const uint32_t ld32 = (uint32_t)ldc;
+  const int r8 = (wave & 3) * 64 + (lane >> 3);
+  const uint32_t chunk = ((lane & 7) ^ (r8 >> 1 & 3)) << 4;      // (bit 3 of the row: per instruction below)
+  int last = 0;
+  const uint8_t *base = nullptr, *sp = nullptr;
+  auto aim = [&](int64_t tile) {
+    const int64_t r0 = isw ? tile % tiles_n * S::T : tile / tiles_n * S::T, left = (isw ? g.N : g.M) - 1 - r0;
+    last = __builtin_amdgcn_readfirstlane((int)(left < S::T ? left : S::T));
+    const int r = (wave & 3) * 64 + lane;
+    base = codes + r0 * ldc;
+    sp = scales + (r0 + (r < last ? r : last)) * lds;
+  };
+  auto issue = [&](int k, int buf) {
+    const uint32_t at = lds0 + buf * S::STAGE + wave * 8192;
+    const uint64_t from = (uint64_t)(base + (int64_t)k * 128);
+    const uint64_t s = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(from >> 32)) << 32) |
+                       (uint32_t)__builtin_amdgcn_readfirstlane((int)from);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = r8 + 8 * i;
+      dma16((uint32_t)(r < last ? r : last) * ld32 + (chunk ^ ((i & 1) << 6)), (const void*)s, at + i * 1024);
+    }
+  };
+  auto scale_at = [&](int k) { return 8 * k < row_scales - 16 ? 8 * k : row_scales - 16; };   // bytes of steps k, k + 1
+  auto issue_scales = [&](int k) { dma16p(sp + scale_at(k), lds0 + S::SC + wave * 1024); };
+
+  const int wn = wave & 3, wm = wave >> 2;
+  const int wrow = wn * 64 + li, arow = S::T + wm * 128 + li, sw = place8(li);
+  uint8_t* const out = smem + S::OUTB + wave * 2560;
+  int64_t turn = 0, tile = tile_of(0);
+  if (tile >= tiles) return;
+  aim(tile);
+  issue_scales(0);
+  issue(0, 0);
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  int buf = 0;
+  for (; tile < tiles;) {
+    const int64_t next = tile_of(++turn);
+    float16_t acc[2][4];
+#pragma unroll
+    for (int f = 0; f < 2; ++f)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[f][e][i] = 0.f;
+    uint32_t ws[2][4], as[4][4];
+    for (int k2 = 0; k2 < ns; k2 += 2) {
+#pragma unroll
+      for (int odd = 0; odd < 2; ++odd) {
+        const int k = k2 + odd;
+        if (odd && k == ns) break;
+        if (!odd) {
+          const int late = 8 * k - scale_at(k);   // 8 where the row's last 16 bytes begin a step early
+          auto words = [&](int row, uint32_t (&to)[4]) {
+            const uint8_t* at = smem + S::SC + row * 16;
+            u4v v = *(const u4v*)at;
+            v[0] = late ? v[2] : v[0];
+            v[1] = late ? v[3] : v[1];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to[j] = v[j] >> (8 * h);
+          };
+#pragma unroll
+          for (int f = 0; f < 2; ++f) words(wrow + 32 * f, ws[f]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) words(arow + 32 * e, as[e]);
+        }
+        if (k + 1 < ns) {
+          if (odd) issue_scales(k + 1);
+          issue(k + 1, buf ^ 1);
+        } else if (next < tiles) {
+          if (!odd) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // all have read these scales
+          aim(next);
+          issue_scales(0);
+          issue(0, buf ^ 1);
+        }
+        const uint8_t* st = smem + buf * S::STAGE;
+        u4v w[2], a[4];
+#pragma unroll
+        for (int f = 0; f < 2; ++f) w[f] = *(const u4v*)(st + (wrow + 32 * f) * 128 + ((h ^ sw) << 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = *(const u4v*)(st + (arow + 32 * e) * 128 + ((h ^ sw) << 4));
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const int p = 2 * odd + (s >> 1);
+          u4v wnext[2];
+          const int at = (((2 * (s + 1) + h) ^ sw) & 7) << 4;
+          if (s < 3)
+#pragma unroll
+            for (int f = 0; f < 2; ++f) wnext[f] = *(const u4v*)(st + (wrow + 32 * f) * 128 + at);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const v8i av = v8i{(int)a[e][0], (int)a[e][1], (int)a[e][2], (int)a[e][3], 0, 0, 0, 0};
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+              const v8i wv = v8i{(int)w[f][0], (int)w[f][1], (int)w[f][2], (int)w[f][3], 0, 0, 0, 0};
+              acc[f][e] = (s & 1) == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv, av, acc[f][e], 4, 4, 0, (int)ws[f][p], 0, (int)as[e][p])
+                                       : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv, av, acc[f][e], 4, 4, 2, (int)ws[f][p], 2, (int)as[e][p]);
+            }
+            if (s < 3) a[e] = *(const u4v*)(st + (arow + 32 * e) * 128 + at);   // the next step's, in the same registers
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          if (s < 3)
+#pragma unroll
+            for (int f = 0; f < 2; ++f) w[f] = wnext[f];
+        }
+        buf ^= 1;
+        // the next step's codes have arrived and every wave is done with this step's.  After the tile's last step this
+        // comes before its stores, so that they drain under the next tile's first step.
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      }
+    }
+
+    const int64_t n0 = tile % tiles_n * S::T + wn * 64, m0 = tile / tiles_n * S::T + wm * 128;
+    const bool full = m0 + 128 <= g.M && n0 + 64 <= g.N;
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      const int64_t nb = n0 + 32 * f;
+      float b[16];
+      tile_bias(g, nb, h, full, b);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t m = m0 + 32 * e + li;
+        __builtin_amdgcn_sched_barrier(0);
+        if (OUT != 1 || !full) {
+          if (full) store_tile<OUT, true>(g, acc[f][e], b, m, nb, h);
+          else store_tile<OUT, false>(g, acc[f][e], b, m, nb, h);
+          continue;
+        }
+        float y[16];
+        tile_act(acc[f][e], b, g.relu, y);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint2 q;
+          q.x = (uint32_t)f2bf(y[4 * j]) | ((uint32_t)f2bf(y[4 * j + 1]) << 16);
+          q.y = (uint32_t)f2bf(y[4 * j + 2]) | ((uint32_t)f2bf(y[4 * j + 3]) << 16);
+          *reinterpret_cast<uint2*>(out + li * 80 + 16 * j + 8 * h) = q;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = 16 * i + (lane >> 2), q = lane & 3;
+          const u4v v = *reinterpret_cast<const u4v*>(out + r * 80 + 16 * q);
+          *reinterpret_cast<u4_any2*>((bf16_t*)g.C + (m0 + 32 * e + r) * g.ldc + nb + 8 * q) = u4_any2{v[0], v[1], v[2], v[3]};
+        }
+      }
+    }
+    tile = next;
+  }
+}
+
+int launch_wide(const Mx4Args& g, int out, int64_t n_out, hipStream_t s) {
+  const int64_t tn = (n_out + 255) / 256, tiles = tn * ((g.M + 255) / 256);
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>(tiles, 256)), dim3(512), 0, s, g, tn, tiles); };
+  out == 0 ? go(gemm_mx4_wide_kernel<0>) : out == 1 ? go(gemm_mx4_wide_kernel<1>) : go(gemm_mx4_wide_kernel<2>);
+  LLP_LAUNCH_CHECK();
+  return LLP_OK;
+}
+
 int64_t pad128(int64_t k) { return (k + 127) / 128 * 128; }
 
 const char* bad_mx4(const llp_mx4* x, int64_t rows, int64_t K) {
@@ -651,6 +841,7 @@ extern "C" int llp_mx4_dequantize(int64_t M, int64_t K, const llp_mx4* X, int dt
   return LLP_OK;
 }
 
+int64_t g_resident_rows = getenv("RR") ? atoll(getenv("RR")) : 8192;
 extern "C" int llp_gemm_nt_mx4(int64_t M, int64_t N, int64_t K, int a_dtype, const llp_operand* A, const llp_mx4* A4,
                                const llp_mx4* W, void* C, int64_t ldc, int c_dtype, const llp_mx4* C4,
                                const float* bias, int act, void* stream) {
@@ -689,6 +880,7 @@ extern "C" int llp_gemm_nt_mx4(int64_t M, int64_t N, int64_t K, int a_dtype, con
   const int64_t nt = (C4 ? pad128(N) : N + 31) / 32, mt = (M + 31) / 32;
   // (32-bit row offsets within a tile)
   const bool near = W->ld_codes < (1 << 23) && (!A4 || A4->ld_codes < (1 << 23));
+  if (A4 && near && M >= g_resident_rows && g.Kp >= 512 && g.Kp % 256 == 0) return launch_wide(g, out, C4 ? g.Np : N, (hipStream_t)stream);
   if (A4 && near && nt * mt >= 1024) return launch_tiled<2, 4>(g, out, C4 ? pad128(N) : N, (hipStream_t)stream);
   auto go = [&](auto kernel) -> int {
     // the grid's second dimension ends at 65,535: longer M in slices
