@@ -608,12 +608,12 @@ int launch_tiled(const Mx4Args& g, int out, int64_t n_out, hipStream_t s) {
 // What bounds the tiled kernel on long K is the number of its requests to L2: 64 bytes each, 480 a step for
 // 128 x 256 columns (126 M for 65536 x 8192 x 2048, 78 % of what the L2 channels take in its time, the matrix
 // units at 42 %).  Here a step is 256 of K, so that a row's codes are a whole line of 128 bytes, and a tile 256 x 256,
-// a third of the requests.  One workgroup of 8 waves (2 x 4: 128 rows x 64 columns each) per CU takes tile after
+// a third of the requests.  One workgroup of 8 waves (4 x 2: 64 rows x 128 columns each) per CU takes tile after
 // tile; the steps of all its tiles are one sequence, the codes of the next step (the next tile's first) arriving in one
 // half of LDS while the other is read.  Row r's chunk c lies at place c ^ place8(r) of its 128 bytes.  K a
 // multiple of 256, at least 512.
 struct Mx4Wide {
-  static constexpr int T = 256, STAGE = 2 * T * 128, SC = 2 * STAGE, OUTB = SC + 2 * T * 16, LDS = OUTB + 8 * 2560;
+  static constexpr int T = 256, STAGE = 2 * T * 128, SC = 2 * STAGE, BIAS = SC + 2 * T * 16, LDS = BIAS + 2 * 4 * T;
 };
 static_assert(Mx4Wide::LDS <= 163840, "LDS of a CU");
 __device__ __forceinline__ int place8(int r) { return (r >> 1) & 7; }
@@ -640,12 +640,18 @@ __global__ __launch_bounds__(512, 2) void gemm_mx4_wide_kernel(Mx4Args g, int64_
   const uint32_t chunk = ((lane & 7) ^ (r8 >> 1 & 3)) << 4;      // (bit 3 of the row: per instruction below)
   int last = 0;
   const uint8_t *base = nullptr, *sp = nullptr;
+  const float* bp = nullptr;
   auto aim = [&](int64_t tile) {
     const int64_t r0 = isw ? tile % tiles_n * S::T : tile / tiles_n * S::T, left = (isw ? g.N : g.M) - 1 - r0;
     last = __builtin_amdgcn_readfirstlane((int)(left < S::T ? left : S::T));
     const int r = (wave & 3) * 64 + lane;
     base = codes + r0 * ldc;
     sp = scales + (r0 + (r < last ? r : last)) * lds;
+    bp = isw && g.bias ? g.bias + r0 + (r < last ? r : last) : nullptr;
+  };
+  // the tile's 256 bias values, in one of two places in turn
+  auto issue_bias = [&](int64_t of) {
+    if (isw && g.bias) dma4(bp, lds0 + S::BIAS + (int)(of & 1) * 4 * S::T + wave * 256);
   };
   auto issue = [&](int k, int buf) {
     const uint32_t at = lds0 + buf * S::STAGE + wave * 8192;
@@ -661,26 +667,27 @@ __global__ __launch_bounds__(512, 2) void gemm_mx4_wide_kernel(Mx4Args g, int64_
   auto scale_at = [&](int k) { return 8 * k < row_scales - 16 ? 8 * k : row_scales - 16; };   // bytes of steps k, k + 1
   auto issue_scales = [&](int k) { dma16p(sp + scale_at(k), lds0 + S::SC + wave * 1024); };
 
-  const int wn = wave & 3, wm = wave >> 2;
-  const int wrow = wn * 64 + li, arow = S::T + wm * 128 + li, sw = place8(li);
-  uint8_t* const out = smem + S::OUTB + wave * 2560;
+  const int wn = wave & 1, wm = wave >> 1;
+  const int wrow = wn * 128 + li, arow = S::T + wm * 64 + li, sw = place8(li);
   int64_t turn = 0, tile = tile_of(0);
   if (tile >= tiles) return;
+  if (!g.bias) *(float*)(smem + S::BIAS + 4 * threadIdx.x) = 0.f;
   aim(tile);
   issue_scales(0);
+  issue_bias(0);
   issue(0, 0);
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   int buf = 0;
   for (; tile < tiles;) {
     const int64_t next = tile_of(++turn);
-    float16_t acc[2][4];
+    float16_t acc[4][2];
 #pragma unroll
-    for (int f = 0; f < 2; ++f)
+    for (int f = 0; f < 4; ++f)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[f][e][i] = 0.f;
-    uint32_t ws[2][4], as[4][4];
+    uint32_t ws[4][4], as[2][4];
     for (int k2 = 0; k2 < ns; k2 += 2) {
 #pragma unroll
       for (int odd = 0; odd < 2; ++odd) {
@@ -689,17 +696,16 @@ __global__ __launch_bounds__(512, 2) void gemm_mx4_wide_kernel(Mx4Args g, int64_
         if (!odd) {
           const int late = 8 * k - scale_at(k);   // 8 where the row's last 16 bytes begin a step early
           auto words = [&](int row, uint32_t (&to)[4]) {
-            const uint8_t* at = smem + S::SC + row * 16;
-            u4v v = *(const u4v*)at;
+            u4v v = *(const u4v*)(smem + S::SC + row * 16);
             v[0] = late ? v[2] : v[0];
             v[1] = late ? v[3] : v[1];
 #pragma unroll
             for (int j = 0; j < 4; ++j) to[j] = v[j] >> (8 * h);
           };
 #pragma unroll
-          for (int f = 0; f < 2; ++f) words(wrow + 32 * f, ws[f]);
+          for (int f = 0; f < 4; ++f) words(wrow + 32 * f, ws[f]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) words(arow + 32 * e, as[e]);
+          for (int e = 0; e < 2; ++e) words(arow + 32 * e, as[e]);
         }
         if (k + 1 < ns) {
           if (odd) issue_scales(k + 1);
@@ -708,37 +714,38 @@ __global__ __launch_bounds__(512, 2) void gemm_mx4_wide_kernel(Mx4Args g, int64_
           if (!odd) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // all have read these scales
           aim(next);
           issue_scales(0);
+          issue_bias(turn);
           issue(0, buf ^ 1);
         }
         const uint8_t* st = smem + buf * S::STAGE;
-        u4v w[2], a[4];
+        u4v w[4], a[2];
 #pragma unroll
-        for (int f = 0; f < 2; ++f) w[f] = *(const u4v*)(st + (wrow + 32 * f) * 128 + ((h ^ sw) << 4));
+        for (int e = 0; e < 2; ++e) a[e] = *(const u4v*)(st + (arow + 32 * e) * 128 + ((h ^ sw) << 4));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = *(const u4v*)(st + (arow + 32 * e) * 128 + ((h ^ sw) << 4));
+        for (int f = 0; f < 4; ++f) w[f] = *(const u4v*)(st + (wrow + 32 * f) * 128 + ((h ^ sw) << 4));
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
           const int p = 2 * odd + (s >> 1);
-          u4v wnext[2];
+          u4v anext[2];
           const int at = (((2 * (s + 1) + h) ^ sw) & 7) << 4;
           if (s < 3)
 #pragma unroll
-            for (int f = 0; f < 2; ++f) wnext[f] = *(const u4v*)(st + (wrow + 32 * f) * 128 + at);
+            for (int e = 0; e < 2; ++e) anext[e] = *(const u4v*)(st + (arow + 32 * e) * 128 + at);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const v8i av = v8i{(int)a[e][0], (int)a[e][1], (int)a[e][2], (int)a[e][3], 0, 0, 0, 0};
+          for (int f = 0; f < 4; ++f) {
+            const v8i wv = v8i{(int)w[f][0], (int)w[f][1], (int)w[f][2], (int)w[f][3], 0, 0, 0, 0};
 #pragma unroll
-            for (int f = 0; f < 2; ++f) {
-              const v8i wv = v8i{(int)w[f][0], (int)w[f][1], (int)w[f][2], (int)w[f][3], 0, 0, 0, 0};
+            for (int e = 0; e < 2; ++e) {
+              const v8i av = v8i{(int)a[e][0], (int)a[e][1], (int)a[e][2], (int)a[e][3], 0, 0, 0, 0};
               acc[f][e] = (s & 1) == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv, av, acc[f][e], 4, 4, 0, (int)ws[f][p], 0, (int)as[e][p])
                                        : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv, av, acc[f][e], 4, 4, 2, (int)ws[f][p], 2, (int)as[e][p]);
             }
-            if (s < 3) a[e] = *(const u4v*)(st + (arow + 32 * e) * 128 + at);   // the next step's, in the same registers
+            if (s < 3) w[f] = *(const u4v*)(st + (wrow + 32 * f) * 128 + at);   // the next step's, in the same registers
             __builtin_amdgcn_sched_barrier(0);
           }
           if (s < 3)
 #pragma unroll
-            for (int f = 0; f < 2; ++f) w[f] = wnext[f];
+            for (int e = 0; e < 2; ++e) a[e] = anext[e];
         }
         buf ^= 1;
         // the next step's codes have arrived and every wave is done with this step's.  After the tile's last step this
@@ -747,39 +754,67 @@ __global__ __launch_bounds__(512, 2) void gemm_mx4_wide_kernel(Mx4Args g, int64_
       }
     }
 
-    const int64_t n0 = tile % tiles_n * S::T + wn * 64, m0 = tile / tiles_n * S::T + wm * 128;
-    const bool full = m0 + 128 <= g.M && n0 + 64 <= g.N;
+    // The half of LDS that was just read takes C on its way out, so that a store covers whole lines of the output's
+    // rows: each wave its own 8 KB, which only its own next fetch overwrites.  Chunk c of row r at place c ^ r.
+    uint8_t* const out = smem + (buf ^ 1) * S::STAGE + wave * 8192;
+    const int64_t n0 = tile % tiles_n * S::T + wn * 128, m0 = tile / tiles_n * S::T + wm * 64;
+    const bool full = m0 + 64 <= g.M && n0 + 128 <= g.N;
 #pragma unroll
-    for (int f = 0; f < 2; ++f) {
-      const int64_t nb = n0 + 32 * f;
-      float b[16];
-      tile_bias(g, nb, h, full, b);
+    for (int e = 0; e < 2; ++e) {
+      const int64_t m = m0 + 32 * e + li;
+      uint32_t row_scales4 = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t m = m0 + 32 * e + li;
+      for (int f = 0; f < 4; ++f) {
+        const int64_t nb = n0 + 32 * f;
         __builtin_amdgcn_sched_barrier(0);
-        if (OUT != 1 || !full) {
+        float b[16];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float4_t v = *(const float4_t*)(smem + S::BIAS + (int)((turn - 1) & 1) * 4 * S::T + 4 * (wn * 128 + 32 * f + 8 * j + 4 * h));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) b[4 * j + i] = v[i];
+        }
+        if (OUT == 0 || !full) {
           if (full) store_tile<OUT, true>(g, acc[f][e], b, m, nb, h);
           else store_tile<OUT, false>(g, acc[f][e], b, m, nb, h);
           continue;
         }
         float y[16];
         tile_act(acc[f][e], b, g.relu, y);
+        if constexpr (OUT == 1) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint2 q;
-          q.x = (uint32_t)f2bf(y[4 * j]) | ((uint32_t)f2bf(y[4 * j + 1]) << 16);
-          q.y = (uint32_t)f2bf(y[4 * j + 2]) | ((uint32_t)f2bf(y[4 * j + 3]) << 16);
-          *reinterpret_cast<uint2*>(out + li * 80 + 16 * j + 8 * h) = q;
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = 16 * i + (lane >> 2), q = lane & 3;
-          const u4v v = *reinterpret_cast<const u4v*>(out + r * 80 + 16 * q);
-          *reinterpret_cast<u4_any2*>((bf16_t*)g.C + (m0 + 32 * e + r) * g.ldc + nb + 8 * q) = u4_any2{v[0], v[1], v[2], v[3]};
+          for (int j = 0; j < 4; ++j) {
+            uint2 q;
+            q.x = (uint32_t)f2bf(y[4 * j]) | ((uint32_t)f2bf(y[4 * j + 1]) << 16);
+            q.y = (uint32_t)f2bf(y[4 * j + 2]) | ((uint32_t)f2bf(y[4 * j + 3]) << 16);
+            *reinterpret_cast<uint2*>(out + li * 256 + (((4 * f + j) ^ (li & 15)) << 4) + 8 * h) = q;
+          }
+        } else {
+          uint32_t c[2], sc;
+          tile_codes(y, h, c, sc);
+          *reinterpret_cast<uint2*>(out + li * 64 + ((f ^ (li >> 2 & 3)) << 4) + 8 * h) = make_uint2(c[0], c[1]);
+          row_scales4 |= sc << (8 * f);
         }
       }
+      if (OUT != 0 && full) {
+        constexpr int LANES = OUT == 1 ? 16 : 4;       // lanes to a row
+#pragma unroll
+        for (int i = 0; i < 32 * LANES / 64; ++i) {
+          const int r = i * (64 / LANES) + lane / LANES, q = lane % LANES;
+          const int64_t mr = m0 + 32 * e + r;
+          if constexpr (OUT == 1) {
+            const u4v v = *reinterpret_cast<const u4v*>(out + r * 256 + ((q ^ (r & 15)) << 4));
+            *reinterpret_cast<u4_any2*>((bf16_t*)g.C + mr * g.ldc + n0 + 8 * q) = u4_any2{v[0], v[1], v[2], v[3]};
+          } else {
+            const u4v v = *reinterpret_cast<const u4v*>(out + r * 64 + ((q ^ (r >> 2 & 3)) << 4));
+            *reinterpret_cast<u4v*>((uint8_t*)g.C4.codes + mr * g.C4.ld_codes + n0 / 2 + 16 * q) = v;
+          }
+        }
+        if constexpr (OUT == 2)
+          if (h == 0) *(uint32_t*)((uint8_t*)g.C4.scales + m * g.C4.ld_scales + n0 / 32) = row_scales4;
+      }
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // its own reads of C, before its next fetch into the same place
     tile = next;
   }
 }
