@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 #include <stdlib.h>
 
 #include "llp_common.h"
@@ -22,7 +23,7 @@ __device__ __forceinline__ float as_f32<bf16_t>(bf16_t x) { return bf2f(x); }
 
 typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u4_any2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t u4_any4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u2_any2 __attribute__((ext_vector_type(2), aligned(2)));
 
 // 8 values at any element offset (gfx950's global loads need no alignment), zeros past n
 __device__ __forceinline__ void load8(const float* p, int n, float (&x)[8]) {
@@ -145,10 +146,10 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(int64_t M, int64_t 
 }
 
 // ---------------------------------------------------------------- product
-// The matrix instruction's first operand is W and its second A, so that its 32 x 32 result holds, in
-// lane l, row m = l % 32 of C at the 16 columns 8 (i / 4) + 4 (l / 32) + i % 4: runs of 4 along the row.
-// Operand lane l: row l % 32, the 32 values of block l / 32 of the 64 that one instruction takes, in
-// 4 registers (16 consecutive bytes of codes), and that block's scale byte: a lane's own.
+// The matrix instruction's first operand is W and its second A, so that a lane's results lie along a row of C.
+// v_mfma_scale_f32_32x32x64: operand lane l holds row l % 32 and the 32 values of block l / 32 of 64 in 4
+// registers (16 consecutive bytes of codes), with that block's scale byte; result lane l row l % 32 of C at
+// the 16 columns 8 (i / 4) + 4 (l / 32) + i % 4: runs of 4.
 struct Mx4Args {
   int64_t M, N, K, Kp, Np;   // Kp, Np: K and N up to 128
   const void* A;         // f32 / bf16 rows
@@ -159,139 +160,6 @@ struct Mx4Args {
   const float* bias;
   int relu;
 };
-
-__device__ __forceinline__ void load_block(const llp_mx4& x, int64_t row, int64_t kb, bool ok, v8i& v, int& s) {
-  u4v c = {0, 0, 0, 0};
-  s = 0;
-  if (ok) {
-    c = *(const u4v*)((const uint8_t*)x.codes + row * x.ld_codes + kb * 16);
-    s = ((const uint8_t*)x.scales)[row * x.ld_scales + kb];
-  }
-  v = v8i{(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
-}
-
-// a block of 32 values of an f32 / bf16 row, quantised in the lane that feeds it to the instruction
-template <typename T>
-__device__ __forceinline__ void quantize_block(const T* row, int64_t k, int64_t K, bool ok, v8i& v, int& s) {
-  float x[32];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float y[8];
-    const int64_t left = ok ? K - k - 8 * j : 0;
-    load8(row + k + 8 * j, (int)(left < 0 ? 0 : left > 8 ? 8 : left), y);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[8 * j + i] = y[i];
-  }
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 32; ++i) top = umax(top, abs_bits(x[i]));
-  const uint32_t b = mx4_scale(top);
-  const float f = mx4_scale_f32(b);
-  s = (int)b;
-  v = v8i{0, 0, 0, 0, 0, 0, 0, 0};
-  if (b != 255u) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = (int)mx4_codes(x + 8 * j, f);
-  }
-}
-
-// One workgroup per 32 x 32 tile of C, its K split over 4 waves and joined through LDS in wave order.
-// SRC 0: A in MXFP4, 1: f32, 2: bf16.  OUT 0: f32, 1: bf16, 2: MXFP4.
-template <int SRC, int OUT>
-__global__ __launch_bounds__(256) void gemm_mx4_tile_kernel(Mx4Args g) {
-  __shared__ float part[3][64][17];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t n0 = (int64_t)blockIdx.x * 32, m0 = (int64_t)blockIdx.y * 32;
-  const int64_t wr = n0 + (lane & 31), ar = m0 + (lane & 31);
-  float16_t acc = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-  for (int64_t kb = 2 * wave + (lane >> 5); kb < g.Kp / 32; kb += 8) {
-    v8i w, a;
-    int sw, sa;
-    load_block(g.W, wr, kb, wr < g.N, w, sw);
-    if constexpr (SRC == 0) load_block(g.A4, ar, kb, ar < g.M, a, sa);
-    else if constexpr (SRC == 1) quantize_block((const float*)g.A + ar * g.lda, kb * 32, g.K, ar < g.M, a, sa);
-    else quantize_block((const bf16_t*)g.A + ar * g.lda, kb * 32, g.K, ar < g.M, a, sa);
-    acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, a, acc, 4, 4, 0, sw, 0, sa);
-  }
-  if (wave > 0)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) part[wave - 1][lane][i] = acc[i];
-  __syncthreads();
-  if (wave > 0) return;
-  const int h = lane >> 5;
-  float y[16];
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int64_t n = n0 + 8 * (i >> 2) + 4 * h + (i & 3);
-    float v = ((acc[i] + part[0][lane][i]) + part[1][lane][i]) + part[2][lane][i];
-    if (g.bias) v += n < g.N ? g.bias[n] : 0.f;
-    if (g.relu) v = v < 0.f ? 0.f : v;   // a NaN stays
-    y[i] = n < g.N ? v : 0.f;
-    top = umax(top, abs_bits(y[i]));
-  }
-  if constexpr (OUT == 2) {
-    top = umax(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-    const uint32_t s = mx4_scale(top);
-    const float f = mx4_scale_f32(s);
-    if (ar < g.M) {
-      uint8_t* c = (uint8_t*)g.C4.codes + ar * g.C4.ld_codes + n0 / 2 + 2 * h;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t q = 0;
-        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[4 * j], y[4 * j + 1], f, 0);
-        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[4 * j + 2], y[4 * j + 3], f, 1);
-        *(uint16_t*)(c + 4 * j) = s == 255u ? 0 : (uint16_t)q;
-      }
-      if (h == 0) ((uint8_t*)g.C4.scales)[ar * g.C4.ld_scales + n0 / 32] = (uint8_t)s;
-    }
-  } else {
-    if (ar < g.M)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int64_t n = n0 + 8 * (i >> 2) + 4 * h + (i & 3);
-        if (n < g.N) {
-          if constexpr (OUT == 0) ((float*)g.C)[ar * g.ldc + n] = y[i];
-          else ((bf16_t*)g.C)[ar * g.ldc + n] = f2bf(y[i]);
-        }
-      }
-  }
-}
-
-// ---------------------------------------------------------------- the tiled product
-// A workgroup of 4 waves (2 x 2) computes 64 MI rows x 64 NI columns of C, a wave 32 MI x 32 NI.  128 of K
-// at a time (a step) go through LDS: 64 bytes of codes per row of W and A, by LDS-DMA (global_load_lds)
-// into one of three stages, two of them in flight while one is read, so one barrier a step.  Chunk c (16
-// bytes) of row r lies at place c ^ place(r) of its row, so that the 16 lanes that read LDS together
-// (neighbouring rows at one c) touch all 64 banks.  The scale bytes of 4 steps (16 per row) come at once: 4 of them a step
-// would touch as many cache lines as the codes do.  They are read into registers at the first of
-// the 4 steps, and the next 16 follow into the same LDS once every wave has read.  SHORT: K of at most
-// 3 steps, whose rows hold fewer than 16 scale bytes: 4 bytes at a time, all before the first step.
-__device__ __forceinline__ int place(int r) { return ((r >> 2) & 1) | ((((r >> 1) ^ (r >> 3)) & 1) << 1); }
-template <int MI, int NI>
-struct Mx4Stage {
-  static constexpr int TM = 64 * MI, TN = 64 * NI, ROWS = TM + TN;
-  static constexpr int BYTES = ROWS * 64;
-  static constexpr int DATA = ROWS / 64;                        // 16-byte DMA instructions per wave and step
-  static constexpr int SCALE_ROWS = ROWS / 4;                   // rows whose scales a wave fetches
-  static constexpr int SCALE = (SCALE_ROWS + 63) / 64;          // DMA instructions for them
-  static constexpr int LDS = 3 * BYTES + ROWS * 16 + 16;        // (a read of 16 bytes may begin 12 late)
-};
-
-// LDS-DMA from inline asm: the kernel counts its own outstanding loads (vmcnt)
-__device__ __forceinline__ void dma16(uint32_t voff, const void* base, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory");
-}
-__device__ __forceinline__ void dma4(const void* p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds) : "memory");
-}
-__device__ __forceinline__ void dma16p(const void* p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory");
-}
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
 
 // bias of a lane's 16 columns n0 + 8 j + 4 h + i (zero past N)
 __device__ __forceinline__ void tile_bias(const Mx4Args& g, int64_t n0, int h, bool full, float (&b)[16]) {
@@ -396,6 +264,204 @@ __device__ __forceinline__ void store_tile(const Mx4Args& g, const float16_t& ac
       }
     }
   }
+}
+
+// ---------------------------------------------------------------- few rows
+// 16 MT rows x 32 columns of C per workgroup, K split over its 8 waves (128 at a time) and joined through LDS in
+// wave order.  What counts here is latency: every load of a wave's step is issued before anything is waited for, and for
+// K <= 1024 a wave has one step.  On v_mfma_scale_f32_16x16x128: lane l holds row l % 16 and the 32 values of
+// block l / 16 of 128, so that f32 / bf16 rows are quantised in the lane that feeds them, without an exchange; the result's
+// lane l has row l % 16 of C at columns 4 (l / 16) + i.  (32 x 32 tiles with K over 4 waves in a loop took
+// 11.6 us for 1 x 1024 x 1024.)
+// SRC 0: A in MXFP4, 1: f32, 2: bf16.  OUT 0: f32, 1: bf16, 2: MXFP4.
+template <int SRC>
+__device__ __forceinline__ void load_rows(const Mx4Args& g, int64_t row, int64_t kb, bool ok, u4v (&x)[SRC == 1 ? 8 : SRC == 2 ? 4 : 1],
+                                          int& s) {
+#pragma unroll
+  for (int i = 0; i < (SRC == 1 ? 8 : SRC == 2 ? 4 : 1); ++i) x[i] = u4v{0, 0, 0, 0};
+  s = 0;
+  if (!ok) return;
+  if constexpr (SRC == 0) {
+    x[0] = *(const u4v*)((const uint8_t*)g.A4.codes + row * g.A4.ld_codes + kb * 16);
+    s = ((const uint8_t*)g.A4.scales)[row * g.A4.ld_scales + kb];
+  } else {
+    constexpr int PER = SRC == 1 ? 4 : 8;   // values in 16 bytes
+    using T = typename std::conditional<SRC == 1, float, bf16_t>::type;
+    const T* p = (const T*)g.A + row * g.lda + kb * 32;
+    const int64_t left = g.K - kb * 32;
+    if (left >= 32) {
+#pragma unroll
+      for (int i = 0; i < 32 / PER; ++i) {
+        const u4_any2 v = *reinterpret_cast<const u4_any2*>(p + PER * i);
+        x[i] = u4v{v[0], v[1], v[2], v[3]};
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        if (i < left) {
+          if constexpr (SRC == 1) x[i >> 2][i & 3] = __float_as_uint(p[i]);
+          else x[i >> 3][(i >> 1) & 3] |= (uint32_t)p[i] << (16 * (i & 1));
+        }
+      }
+    }
+  }
+}
+template <int SRC>
+__device__ __forceinline__ v8i as_block(const u4v (&x)[SRC == 1 ? 8 : SRC == 2 ? 4 : 1], int& s) {
+  if constexpr (SRC == 0) {
+    return v8i{(int)x[0][0], (int)x[0][1], (int)x[0][2], (int)x[0][3], 0, 0, 0, 0};
+  } else {
+    float y[32];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      y[i] = SRC == 1 ? __uint_as_float(x[i >> 2][i & 3])
+                      : __uint_as_float(i & 1 ? x[i >> 3][(i >> 1) & 3] & 0xFFFF0000u : x[i >> 3][(i >> 1) & 3] << 16);
+      top = umax(top, abs_bits(y[i]));
+    }
+    const uint32_t b = mx4_scale(top);
+    const float f = mx4_scale_f32(b);
+    s = (int)b;
+    v8i v = v8i{0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = b == 255u ? 0 : (int)mx4_codes(y + 8 * j, f);
+    return v;
+  }
+}
+
+template <int SRC, int OUT, int MT>
+__global__ __launch_bounds__(512) void gemm_mx4_rows_kernel(Mx4Args g) {
+  __shared__ float4_t part[8][2 * MT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, li = lane & 15;
+  const int64_t n0 = (int64_t)blockIdx.x * 32, m0 = (int64_t)blockIdx.y * 16 * MT;
+  // bias of the tile that this wave stores (t = wave modulo 2 MT: rows t / 2, columns t % 2)
+  float4_t bias = {0.f, 0.f, 0.f, 0.f};
+  if (g.bias) {
+    const int64_t n = n0 + 16 * (wave & 1) + 4 * q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bias[i] = n + i < g.N ? g.bias[n + i] : 0.f;
+  }
+  float4_t acc[2][MT];
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int e = 0; e < MT; ++e) acc[c][e] = float4_t{0.f, 0.f, 0.f, 0.f};
+  const int64_t nk = g.Kp / 128;
+  for (int64_t k = wave; k < nk; k += 8) {
+    const int64_t kb = 4 * k + q;
+    u4v w[2], x[MT][SRC == 1 ? 8 : SRC == 2 ? 4 : 1];
+    int ws[2], xs[MT];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int64_t n = n0 + 16 * c + li;
+      w[c] = u4v{0, 0, 0, 0};
+      ws[c] = 0;
+      if (n < g.N) {
+        w[c] = *(const u4v*)((const uint8_t*)g.W.codes + n * g.W.ld_codes + kb * 16);
+        ws[c] = ((const uint8_t*)g.W.scales)[n * g.W.ld_scales + kb];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < MT; ++e) load_rows<SRC>(g, m0 + 16 * e + li, kb, m0 + 16 * e + li < g.M, x[e], xs[e]);
+#pragma unroll
+    for (int e = 0; e < MT; ++e) {
+      const v8i a = as_block<SRC>(x[e], xs[e]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const v8i b = v8i{(int)w[c][0], (int)w[c][1], (int)w[c][2], (int)w[c][3], 0, 0, 0, 0};
+        acc[c][e] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, acc[c][e], 4, 4, 0, ws[c], 0, xs[e]);
+      }
+    }
+  }
+  const int live = (int)(nk < 8 ? nk : 8);   // waves that had a step
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int e = 0; e < MT; ++e) part[wave][2 * e + c][lane] = acc[c][e];
+  __syncthreads();
+  if (OUT != 2 && wave >= 2 * MT) return;
+  const int t = wave % (2 * MT), c = t & 1, e = t >> 1;   // (in MXFP4 the other waves repeat a tile up to the barrier)
+  float4_t y = part[0][t][lane];
+  for (int i = 1; i < live; ++i) y += part[i][t][lane];
+  const int64_t m = m0 + 16 * e + li, n = n0 + 16 * c + 4 * q;
+  const float floor = g.relu ? 0.f : -__builtin_inff();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = relu_or(y[i] + bias[i], floor);
+  if constexpr (OUT == 2) {
+    // a block of 32 columns: the 4 lane groups of two waves, whose largest values meet in LDS
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (n + i >= g.N) y[i] = 0.f;
+      top = umax(top, abs_bits(y[i]));
+    }
+    top = umax(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+    top = umax(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+    __shared__ uint32_t tops[2 * MT][16];
+    if (q == 0) tops[t][li] = top;
+    __syncthreads();
+    const uint32_t sc = mx4_scale(umax(top, tops[t ^ 1][li]));
+    const float f = mx4_scale_f32(sc);
+    uint32_t d = 0;
+    d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, y[0], y[1], f, 0);
+    d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, y[2], y[3], f, 1);
+    if (m < g.M && wave < 2 * MT) {
+      *(uint16_t*)((uint8_t*)g.C4.codes + m * g.C4.ld_codes + n / 2) = sc == 255u ? 0 : (uint16_t)d;
+      if (c == 0 && q == 0) ((uint8_t*)g.C4.scales)[m * g.C4.ld_scales + n0 / 32] = (uint8_t)sc;
+    }
+  } else if (m < g.M) {
+    if constexpr (OUT == 0) {
+      float* o = (float*)g.C + m * g.ldc + n;
+      if (n + 4 <= g.N) *reinterpret_cast<f4_any*>(o) = f4_any{y[0], y[1], y[2], y[3]};
+      else
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n + i < g.N) o[i] = y[i];
+    } else {
+      bf16_t* o = (bf16_t*)g.C + m * g.ldc + n;
+      const uint32_t p0 = (uint32_t)f2bf(y[0]) | ((uint32_t)f2bf(y[1]) << 16), p1 = (uint32_t)f2bf(y[2]) | ((uint32_t)f2bf(y[3]) << 16);
+      if (n + 4 <= g.N) *reinterpret_cast<u2_any2*>(o) = u2_any2{p0, p1};
+      else
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n + i < g.N) o[i] = (bf16_t)((i < 2 ? p0 : p1) >> (16 * (i & 1)));
+    }
+  }
+}
+
+// ---------------------------------------------------------------- the tiled product
+// A workgroup of 4 waves (2 x 2) computes 64 MI rows x 64 NI columns of C, a wave 32 MI x 32 NI.  128 of K
+// at a time (a step) go through LDS: 64 bytes of codes per row of W and A, by LDS-DMA (global_load_lds)
+// into one of three stages, two of them in flight while one is read, so one barrier a step.  Chunk c (16
+// bytes) of row r lies at place c ^ place(r) of its row, so that the 16 lanes that read LDS together
+// (neighbouring rows at one c) touch all 64 banks.  The scale bytes of 4 steps (16 per row) come at once: 4 of them a step
+// would touch as many cache lines as the codes do.  They are read into registers at the first of
+// the 4 steps, and the next 16 follow into the same LDS once every wave has read.  SHORT: K of at most
+// 3 steps, whose rows hold fewer than 16 scale bytes: 4 bytes at a time, all before the first step.
+__device__ __forceinline__ int place(int r) { return ((r >> 2) & 1) | ((((r >> 1) ^ (r >> 3)) & 1) << 1); }
+template <int MI, int NI>
+struct Mx4Stage {
+  static constexpr int TM = 64 * MI, TN = 64 * NI, ROWS = TM + TN;
+  static constexpr int BYTES = ROWS * 64;
+  static constexpr int DATA = ROWS / 64;                        // 16-byte DMA instructions per wave and step
+  static constexpr int SCALE_ROWS = ROWS / 4;                   // rows whose scales a wave fetches
+  static constexpr int SCALE = (SCALE_ROWS + 63) / 64;          // DMA instructions for them
+  static constexpr int LDS = 3 * BYTES + ROWS * 16 + 16;        // (a read of 16 bytes may begin 12 late)
+};
+
+// LDS-DMA from inline asm: the kernel counts its own outstanding loads (vmcnt)
+__device__ __forceinline__ void dma16(uint32_t voff, const void* base, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void dma4(const void* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void dma16p(const void* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
 template <int MI, int NI, int OUT, bool SHORT>
@@ -829,6 +895,35 @@ int launch_wide(const Mx4Args& g, int out, int64_t n_out, hipStream_t s) {
 
 int64_t pad128(int64_t k) { return (k + 127) / 128 * 128; }
 
+template <int MT>
+int launch_rows(const Mx4Args& g, int src, int out, int64_t n_out, hipStream_t s) {
+  // the grid's second dimension ends at 65,535: longer M in slices
+  const int64_t slice = (int64_t)65535 * 16 * MT;
+  for (int64_t r = 0; r < g.M; r += slice) {
+    Mx4Args h = g;
+    h.M = std::min(g.M - r, slice);
+    if (src == 0) h.A4.codes = (char*)h.A4.codes + r * h.A4.ld_codes, h.A4.scales = (char*)h.A4.scales + r * h.A4.ld_scales;
+    else h.A = (const char*)h.A + r * h.lda * (src == 1 ? 4 : 2);
+    if (out == 2) h.C4.codes = (char*)h.C4.codes + r * h.C4.ld_codes, h.C4.scales = (char*)h.C4.scales + r * h.C4.ld_scales;
+    else h.C = (char*)h.C + r * h.ldc * (out == 0 ? 4 : 2);
+    const dim3 grid((unsigned)((n_out + 31) / 32), (unsigned)((h.M + 16 * MT - 1) / (16 * MT)));
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(512), 0, s, h); };
+    switch (src * 3 + out) {
+      case 0: go(gemm_mx4_rows_kernel<0, 0, MT>); break;
+      case 1: go(gemm_mx4_rows_kernel<0, 1, MT>); break;
+      case 2: go(gemm_mx4_rows_kernel<0, 2, MT>); break;
+      case 3: go(gemm_mx4_rows_kernel<1, 0, MT>); break;
+      case 4: go(gemm_mx4_rows_kernel<1, 1, MT>); break;
+      case 5: go(gemm_mx4_rows_kernel<1, 2, MT>); break;
+      case 6: go(gemm_mx4_rows_kernel<2, 0, MT>); break;
+      case 7: go(gemm_mx4_rows_kernel<2, 1, MT>); break;
+      default: go(gemm_mx4_rows_kernel<2, 2, MT>); break;
+    }
+    LLP_LAUNCH_CHECK();
+  }
+  return LLP_OK;
+}
+
 const char* bad_mx4(const llp_mx4* x, int64_t rows, int64_t K) {
   if (!x) return "null";
   if (rows > 0 && (!x->codes || !x->scales)) return "null buffer";
@@ -876,6 +971,7 @@ extern "C" int llp_mx4_dequantize(int64_t M, int64_t K, const llp_mx4* X, int dt
   return LLP_OK;
 }
 
+int64_t g_tiled = getenv("TT") ? atoll(getenv("TT")) : 1024;
 int64_t g_resident_rows = getenv("RR") ? atoll(getenv("RR")) : 8192;
 extern "C" int llp_gemm_nt_mx4(int64_t M, int64_t N, int64_t K, int a_dtype, const llp_operand* A, const llp_mx4* A4,
                                const llp_mx4* W, void* C, int64_t ldc, int c_dtype, const llp_mx4* C4,
@@ -912,36 +1008,11 @@ extern "C" int llp_gemm_nt_mx4(int64_t M, int64_t N, int64_t K, int a_dtype, con
     g.C = C, g.ldc = ldc;
     out = c_dtype == LLP_F32 ? 0 : 1;
   }
-  const int64_t nt = (C4 ? pad128(N) : N + 31) / 32, mt = (M + 31) / 32;
+  const int64_t n_out = C4 ? g.Np : N;
+  hipStream_t s = (hipStream_t)stream;
   // (32-bit row offsets within a tile)
   const bool near = W->ld_codes < (1 << 23) && (!A4 || A4->ld_codes < (1 << 23));
-  if (A4 && near && M >= g_resident_rows && g.Kp >= 512 && g.Kp % 256 == 0) return launch_wide(g, out, C4 ? g.Np : N, (hipStream_t)stream);
-  if (A4 && near && nt * mt >= 1024) return launch_tiled<2, 4>(g, out, C4 ? pad128(N) : N, (hipStream_t)stream);
-  auto go = [&](auto kernel) -> int {
-    // the grid's second dimension ends at 65,535: longer M in slices
-    for (int64_t b = 0; b < mt; b += 65535) {
-      Mx4Args h = g;
-      const int64_t r = b * 32;
-      h.M = std::min<int64_t>(M - r, 65535 * 32);
-      if (h.A) h.A = (const char*)h.A + r * h.lda * (src == 1 ? 4 : 2);
-      if (A4) h.A4.codes = (char*)h.A4.codes + r * h.A4.ld_codes, h.A4.scales = (char*)h.A4.scales + r * h.A4.ld_scales;
-      if (h.C) h.C = (char*)h.C + r * h.ldc * (out == 0 ? 4 : 2);
-      if (C4) h.C4.codes = (char*)h.C4.codes + r * h.C4.ld_codes, h.C4.scales = (char*)h.C4.scales + r * h.C4.ld_scales;
-      hipLaunchKernelGGL(kernel, dim3((unsigned)nt, (unsigned)std::min<int64_t>(mt - b, 65535)), dim3(256), 0,
-                         (hipStream_t)stream, h);
-      LLP_LAUNCH_CHECK();
-    }
-    return LLP_OK;
-  };
-  switch (src * 3 + out) {
-    case 0: return go(gemm_mx4_tile_kernel<0, 0>);
-    case 1: return go(gemm_mx4_tile_kernel<0, 1>);
-    case 2: return go(gemm_mx4_tile_kernel<0, 2>);
-    case 3: return go(gemm_mx4_tile_kernel<1, 0>);
-    case 4: return go(gemm_mx4_tile_kernel<1, 1>);
-    case 5: return go(gemm_mx4_tile_kernel<1, 2>);
-    case 6: return go(gemm_mx4_tile_kernel<2, 0>);
-    case 7: return go(gemm_mx4_tile_kernel<2, 1>);
-    default: return go(gemm_mx4_tile_kernel<2, 2>);
-  }
+  if (A4 && near && M >= g_resident_rows && g.Kp >= 512 && g.Kp % 256 == 0) return launch_wide(g, out, n_out, s);
+  if (A4 && near && (n_out + 31) / 32 * ((M + 31) / 32) >= g_tiled) return launch_tiled<2, 4>(g, out, n_out, s);
+  return M <= 16 ? launch_rows<1>(g, src, out, n_out, s) : launch_rows<4>(g, src, out, n_out, s);
 }

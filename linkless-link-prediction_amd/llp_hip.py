@@ -927,23 +927,18 @@ def descs_to_device(descs, device):
     return host.to(device)
 
 
-class on_device:
-    """The launch context of ``dev``: its current stream's handle, with ``dev`` the current device
-    (a kernel launches on the current device; a tensor may live on another)."""
-    __slots__ = ("dev", "prev")
-
-    def __init__(self, dev):
-        self.dev = dev.index
-
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.dev:
-            torch.cuda.set_device(self.dev)
-        return torch.cuda.current_stream(self.dev).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.prev != self.dev:
-            torch.cuda.set_device(self.prev)
+def launch(what, dev, *args):
+    """Entry point ``what`` with ``args`` and the current stream of ``dev``, with ``dev`` the current device (a
+    kernel launches on the current device; the tensors may live on another)."""
+    fn = getattr(_lib or lib(), what)
+    i = dev.index
+    if torch._C._cuda_getDevice() == i:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc != 0:
+        check(rc, what)
 
 
 def relu_bwd(gy, y, alpha, out):

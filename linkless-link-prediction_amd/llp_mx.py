@@ -24,6 +24,7 @@ import llp_hip as K
 # f32 / bf16 inputs of up to this many rows are quantised inside the product (one launch); more rows
 # are quantised first, once, instead of once for each 32 columns of the result.
 DIRECT_ROWS = 64
+_FLOATS = (torch.float32, torch.bfloat16)
 
 
 def _pad(k):
@@ -49,8 +50,12 @@ class MX4:
     @staticmethod
     def empty(rows, cols, device):
         p = _pad(cols)
-        return MX4(torch.empty(rows, p // 2, dtype=torch.uint8, device=device),
-                   torch.empty(rows, p // 32, dtype=torch.uint8, device=device), cols)
+        q = object.__new__(MX4)
+        q.codes = torch.empty((rows, p // 2), dtype=torch.uint8, device=device)
+        q.scales = torch.empty((rows, p // 32), dtype=torch.uint8, device=device)
+        q.cols = cols
+        q.c = K.Mx4(q.codes.data_ptr(), q.scales.data_ptr(), p // 2, p // 32)
+        return q
 
     @property
     def rows(self):
@@ -68,11 +73,11 @@ class MX4:
 def _rows2d(x, what):
     if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
         raise ValueError(f"{what}: a 2-D tensor with contiguous rows")
-    if x.dtype not in (torch.float32, torch.bfloat16):
+    if x.dtype not in _FLOATS:
         raise TypeError(f"{what}: f32 or bf16, not {x.dtype}")
     if not x.is_cuda:
         raise RuntimeError("LLP ops run only on the MI355X HIP device (got a CPU tensor; no CPU fallback)")
-    if torch.is_grad_enabled() and x.requires_grad:
+    if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{what}: MXFP4 has no gradient; call it under torch.no_grad()")
 
 
@@ -111,10 +116,7 @@ def quantize(x, idx=None, x2=None, idx2=None, out=None):
         out = MX4.empty(rows, x.shape[1], x.device)
     elif out.shape != (rows, x.shape[1]) or out.device != x.device:
         raise ValueError(f"quantize: out is {out.shape} on {out.device}, the rows are {(rows, x.shape[1])} on {x.device}")
-    L = K.lib()
-    with K.on_device(x.device) as stream:
-        K.check(L.llp_mx4_quantize(K.dtype_code(x.dtype), rows, x.shape[1], C.byref(op), C.byref(out.c), stream),
-                "llp_mx4_quantize")
+    K.launch("llp_mx4_quantize", x.device, K.dtype_code(x.dtype), rows, x.shape[1], C.byref(op), C.byref(out.c))
     return out
 
 
@@ -124,10 +126,8 @@ def dequantize(q, dtype=torch.float32, out=None):
         out = torch.empty(q.rows, q.cols, dtype=dtype, device=q.device)
     elif tuple(out.shape) != q.shape or out.device != q.device or (q.cols > 1 and out.stride(1) != 1):
         raise ValueError("dequantize: out needs q's shape, on its device, with contiguous rows")
-    L = K.lib()
-    with K.on_device(q.device) as stream:
-        K.check(L.llp_mx4_dequantize(q.rows, q.cols, C.byref(q.c), K.dtype_code(out.dtype), out.data_ptr(),
-                                     max(out.stride(0), q.cols), stream), "llp_mx4_dequantize")
+    K.launch("llp_mx4_dequantize", q.device, q.rows, q.cols, C.byref(q.c), K.dtype_code(out.dtype), out.data_ptr(),
+             max(out.stride(0), q.cols))
     return out
 
 
@@ -135,44 +135,45 @@ def linear(x, w, bias=None, relu=False, out_dtype=None, out=None):
     """act(Q(x) w^T + bias): x [..., cols] in f32 / bf16 or an MX4, w an MX4 [N, cols], bias [N].
     out_dtype torch.float32 / torch.bfloat16 / "mx4" (default x's dtype; bf16 for an MX4 x); ``out``: a
     2-D tensor with contiguous rows, or an MX4, written in place of a new one."""
-    lead = None
-    if isinstance(x, MX4):
-        rows, dt = x.rows, torch.bfloat16
-        width, dev = x.cols, x.device
-    else:
+    lead = op = None
+    four_in = isinstance(x, MX4)
+    if not four_in:
         if x.dim() != 2:
             lead = x.shape[:-1]
             x = x.reshape(-1, x.shape[-1])
         _rows2d(x, "linear")
-        rows, dt = x.shape[0], x.dtype
-        width, dev = x.shape[1], x.device
+    rows, width = x.shape
+    N, dev = w.rows, x.device
     if width != w.cols or dev != w.device:
         raise ValueError(f"linear: x has {width} columns on {dev}, w has {w.cols} on {w.device}")
-    N = w.rows
     if bias is not None:
-        if torch.is_grad_enabled() and bias.requires_grad:
+        if bias.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("linear: MXFP4 has no gradient; call it under torch.no_grad()")
         if bias.shape != (N,) or bias.device != dev:
             raise ValueError(f"linear: bias of {N} values on {dev}")
-        bias = bias.detach().float().contiguous()
+        if bias.dtype != torch.float32 or not bias.is_contiguous():
+            bias = bias.detach().float().contiguous()
     if out is None:
-        out_dtype = dt if out_dtype is None else out_dtype
-        out = MX4.empty(rows, N, dev) if out_dtype == "mx4" else torch.empty(rows, N, dtype=out_dtype, device=dev)
+        if out_dtype is None:
+            out_dtype = torch.bfloat16 if four_in else x.dtype
+        out = MX4.empty(rows, N, dev) if out_dtype == "mx4" else torch.empty((rows, N), dtype=out_dtype, device=dev)
     elif tuple(out.shape) != (rows, N) or out.device != dev or lead is not None:
         raise ValueError(f"linear: out is {tuple(out.shape)} on {out.device}, the result is {(rows, N)} on {dev}")
-    four = isinstance(out, MX4)
-    if not four and (out.dtype not in (torch.float32, torch.bfloat16) or (N > 1 and out.stride(1) != 1)):
+    four_out = isinstance(out, MX4)
+    if not four_out and (out.dtype not in _FLOATS or (N > 1 and out.stride(1) != 1)):
         raise TypeError("linear: out in f32 or bf16 with contiguous rows")
-    if not isinstance(x, MX4) and rows > DIRECT_ROWS:
-        x = quantize(x)
-    L = K.lib()
-    op, code = None, 0
-    if not isinstance(x, MX4):
-        op = C.byref(K.Operand(x.data_ptr(), None, None, None, x.stride(0), 0, None))
-        code = K.dtype_code(x.dtype)
-    with K.on_device(dev) as stream:
-        K.check(L.llp_gemm_nt_mx4(rows, N, width, code, op, None if op else C.byref(x.c), C.byref(w.c),
-                                  None if four else out.data_ptr(), 0 if four else max(out.stride(0), N),
-                                  0 if four else K.dtype_code(out.dtype), C.byref(out.c) if four else None,
-                                  K.ptr(bias), K.ACT_RELU if relu else K.ACT_NONE, stream), "llp_gemm_nt_mx4")
-    return out if lead is None or four else out.reshape(*lead, N)
+    code = 0
+    if not four_in:
+        if rows > DIRECT_ROWS:
+            x, four_in = quantize(x), True
+        else:
+            op, code = C.byref(K.Operand(x.data_ptr(), None, None, None, x.stride(0), 0, None)), K.dtype_code(x.dtype)
+    act = K.ACT_RELU if relu else K.ACT_NONE
+    b = None if bias is None else bias.data_ptr()
+    if four_out:
+        K.launch("llp_gemm_nt_mx4", dev, rows, N, width, code, op, C.byref(x.c) if four_in else None, C.byref(w.c), None, 0, 0,
+                 C.byref(out.c), b, act)
+        return out
+    K.launch("llp_gemm_nt_mx4", dev, rows, N, width, code, op, C.byref(x.c) if four_in else None, C.byref(w.c),
+             out.data_ptr(), max(out.stride(0), N), K.dtype_code(out.dtype), None, b, act)
+    return out if lead is None else out.reshape(*lead, N)

@@ -128,6 +128,7 @@ class AdamWTable:
         self._descs = K.descs_to_device(descs, dev)
         self._work = torch.cat(work).to(dev)
         self._work_t = torch.cat(work_t).to(dev) if work_t else None
+        self._args = (self._descs.data_ptr(), self.n, self._work.data_ptr(), self._work.shape[0])
         self._keep = (ins, outs, grads, copies, copies_t, values)
 
     @staticmethod
@@ -195,24 +196,18 @@ class AdamWTable:
         if sumsq is not None and (sumsq.dtype != torch.float32 or sumsq.device != self.device
                                   or sumsq.numel() < self.n_groups or not sumsq.is_contiguous()):
             raise TypeError(f"AdamWTable.step: sumsq as f32[{self.n_groups}] on {self.device}")
-        L = K.lib()
-        with K.on_device(self.device) as stream:
-            K.check(L.llp_adamw_step(self._descs.data_ptr(), self.n, self._work.data_ptr(), self._work.shape[0],
-                                     self.bits, self.param_code, self.grad_code, K.ptr(sumsq), max_norm, lr, betas[0],
-                                     betas[1], eps, weight_decay, step.data_ptr(), int(seed) & 0xFFFFFFFFFFFFFFFF,
-                                     stream), "llp_adamw_step")
-            if self._work_t is not None:
-                K.check(L.llp_adamw_copy_t(self._descs.data_ptr(), self._work_t.data_ptr(), self._work_t.shape[0],
-                                           self.param_code, stream), "llp_adamw_copy_t")
+        K.launch("llp_adamw_step", self.device, *self._args, self.bits, self.param_code, self.grad_code, K.ptr(sumsq),
+                 max_norm, lr, betas[0], betas[1], eps, weight_decay, step.data_ptr(), int(seed) & 0xFFFFFFFFFFFFFFFF)
+        if self._work_t is not None:
+            K.launch("llp_adamw_copy_t", self.device, self._descs.data_ptr(), self._work_t.data_ptr(),
+                     self._work_t.shape[0], self.param_code)
 
     def values(self):
         """Fill the ``values`` lists with the values of the 8-bit moments that the last step wrote."""
         if self.values_dtype is None:
             raise RuntimeError("AdamWTable: built without values")
-        L = K.lib()
-        with K.on_device(self.device) as stream:
-            K.check(L.llp_adamw_values(self._descs.data_ptr(), self._work.data_ptr(), self._work.shape[0],
-                                       K.dtype_code(self.values_dtype), stream), "llp_adamw_values")
+        K.launch("llp_adamw_values", self.device, self._args[0], self._args[2], self._args[3],
+                 K.dtype_code(self.values_dtype))
 
 
 class AdamW(torch.optim.Optimizer):
@@ -283,8 +278,7 @@ class AdamW(torch.optim.Optimizer):
             _, table, ctr = at
             table.step(ctr, lr=float(group["lr"]), betas=group["betas"], eps=float(group["eps"]),
                        weight_decay=float(group["weight_decay"]), seed=self.seed + (i << 48))
-            with K.on_device(ctr.device):
-                K.increment(ctr)
+            K.launch("llp_increment", ctr.device, ctr.data_ptr())
         return loss
 
     def _sync_steps(self):
