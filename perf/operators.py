@@ -139,10 +139,13 @@ _TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "mx4": torch.bfloat16}
 
 
 def _llp(name):
-    at = os.path.join(os.getcwd(), "linkless-link-prediction_amd")
-    if at not in sys.path:
-        sys.path.insert(0, at)
-    return __import__(name)
+    """A module of the package, imported on first use."""
+    if name not in sys.modules:
+        at = os.path.join(os.getcwd(), "linkless-link-prediction_amd")
+        if at not in sys.path:
+            sys.path.insert(0, at)
+        __import__(name)
+    return sys.modules[name]
 
 
 def prepare(c, seed):
