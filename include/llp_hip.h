@@ -685,8 +685,8 @@ int llp_adamw_copy_t(const llp_adamw_desc* descs, const int32_t* work, int64_t n
  *   ties to even, saturated at 6.  X->rows_dev must be NULL.
  * llp_mx4_dequantize: the values, as f32 or bf16 (exact in both), [M, K] with row stride ldy.
  * llp_gemm_nt_mx4: C[m, n] = act(sum_k A[m, k] W[n, k] + bias[n]) with W in MXFP4 and A in MXFP4 (A4) or
- *   f32 / bf16 rows (A, plain; quantised on the way as llp_mx4_quantize does: for few rows).  Exactly one
- *   of A and A4.  Products exact, f32 sums.  act NONE or RELU; bias f32[N] or NULL.  Out: C (f32 or bf16)
+ *   f32 / bf16 rows (A, plain; quantised on the way as llp_mx4_quantize does: for few rows).  Both: A is first
+ *   quantised into A4 (scratch).  Products exact, f32 sums.  act NONE or RELU; bias f32[N] or NULL.  Out: C (f32 or bf16)
  *   or C4 (MXFP4 with K := N, the values quantised from f32; padding written), exactly one of them.
  *   Inference only: there is no gradient through it. */
 typedef struct llp_mx4 {

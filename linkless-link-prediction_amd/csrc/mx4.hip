@@ -77,30 +77,56 @@ __device__ __forceinline__ uint32_t quad_umax(uint32_t x) {
 }
 
 // ---------------------------------------------------------------- quantise
+// u / d and u % d for u < 2^31 by a multiplication (Granlund and Montgomery): with 2^(l-1) < d <= 2^l and
+// m = ceil(2^(31+l) / d) < 2^32, floor(u / d) = floor(u m / 2^(31+l)).  (A 64-bit division for each 8 values made the
+// conversions compute-bound.)
+struct FastDiv {
+  uint32_t d, m, shift;   // shift = l - 1 of the product's upper word
+};
+inline FastDiv fast_div(uint32_t d) {
+  uint32_t l = 0;
+  while ((1ull << l) < d) ++l;
+  if (l == 0) return FastDiv{1, 0, 0};
+  return FastDiv{d, (uint32_t)(((1ull << (31 + l)) + d - 1) / d), l - 1};
+}
+__device__ __forceinline__ uint32_t divided(uint32_t u, const FastDiv& f) {
+  return f.m ? __umulhi(u, f.m) >> f.shift : u;
+}
+
 // 8 values per lane, a block of 32 per quad: the block's largest by two quad exchanges, 4 bytes of
-// codes per lane, one scale byte per quad.  Bound by memory: 4 or 2 B read, 17/32 B written per value.
+// codes per lane, one scale byte per quad.  Four such units per thread, 256 apart, all loaded before the first is
+// used.  Bound by memory: 4 or 2 B read, 17/32 B written per value.
 template <typename T, bool PAIRS>
-__global__ __launch_bounds__(256) void mx4_quantize_kernel(int64_t M, int64_t K, int64_t per_row, llp_operand X,
+__global__ __launch_bounds__(256) void mx4_quantize_kernel(uint32_t units, int K, FastDiv per_row, llp_operand X,
                                                            llp_mx4 out) {
-  const int64_t units = M * per_row;
-  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < units; u += (int64_t)gridDim.x * 256) {
-    const int64_t r = u / per_row, c = (u - r * per_row) * 8;
-    const int n = (int)(K - c < 8 ? (K - c < 0 ? 0 : K - c) : 8);
-    float x[8];
-    load8((const T*)X.ptr + (X.idx ? (int64_t)X.idx[r] : r) * X.ld + c, n, x);
-    if constexpr (PAIRS) {
-      float y[8];
-      load8((const T*)X.ptr2 + (X.idx2 ? (int64_t)X.idx2[r] : r) * X.ld2 + c, n, y);
+  constexpr int U = 4;
+  const uint32_t u0 = blockIdx.x * (256u * U) + threadIdx.x;
+  float x[U][8], y[U][8];
+  uint32_t row[U];
+  int col[U];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] *= y[i];
-    }
+  for (int i = 0; i < U; ++i) {
+    const uint32_t u = u0 + 256 * i < units ? u0 + 256 * i : units - 1;
+    row[i] = divided(u, per_row);
+    col[i] = (int)(u - row[i] * per_row.d) * 8;
+    const int n = K - col[i] < 8 ? (K - col[i] < 0 ? 0 : K - col[i]) : 8;
+    load8((const T*)X.ptr + (X.idx ? (int64_t)X.idx[row[i]] : (int64_t)row[i]) * X.ld + col[i], n, x[i]);
+    if constexpr (PAIRS)
+      load8((const T*)X.ptr2 + (X.idx2 ? (int64_t)X.idx2[row[i]] : (int64_t)row[i]) * X.ld2 + col[i], n, y[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    if (u0 + 256 * i >= units) break;   // (whole quads: units is a multiple of 16)
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = umax(top, abs_bits(x[i]));
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (PAIRS) x[i][j] *= y[i][j];
+      top = umax(top, abs_bits(x[i][j]));
+    }
     const uint32_t s = mx4_scale(quad_umax(top));
-    const uint32_t codes = s == 255u ? 0u : mx4_codes(x, mx4_scale_f32(s));
-    *(uint32_t*)((uint8_t*)out.codes + r * out.ld_codes + (c >> 1)) = codes;
-    if ((threadIdx.x & 3) == 0) ((uint8_t*)out.scales)[r * out.ld_scales + (c >> 5)] = (uint8_t)s;
+    const uint32_t codes = s == 255u ? 0u : mx4_codes(x[i], mx4_scale_f32(s));
+    *(uint32_t*)((uint8_t*)out.codes + (int64_t)row[i] * out.ld_codes + (col[i] >> 1)) = codes;
+    if ((threadIdx.x & 3) == 0) ((uint8_t*)out.scales)[(int64_t)row[i] * out.ld_scales + (col[i] >> 5)] = (uint8_t)s;
   }
 }
 
@@ -111,19 +137,29 @@ __device__ __forceinline__ float mx4_value(uint32_t c, float scale) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void mx4_dequantize_kernel(int64_t M, int64_t K, int64_t per_row, llp_mx4 X,
+__global__ __launch_bounds__(256) void mx4_dequantize_kernel(uint32_t units, int K, FastDiv per_row, llp_mx4 X,
                                                              T* __restrict__ Y, int64_t ldy) {
-  const int64_t units = M * per_row;
-  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < units; u += (int64_t)gridDim.x * 256) {
-    const int64_t r = u / per_row, c = (u - r * per_row) * 8;
-    const int64_t n = K - c;
-    const uint32_t codes = *(const uint32_t*)((const uint8_t*)X.codes + r * X.ld_codes + (c >> 1));
-    const uint32_t s = ((const uint8_t*)X.scales)[r * X.ld_scales + (c >> 5)];
-    const float f = s == 255u ? __uint_as_float(0x7FC00000u) : mx4_scale_f32(s);
-    T* y = Y + r * ldy + c;
+  constexpr int U = 4;
+  const uint32_t u0 = blockIdx.x * (256u * U) + threadIdx.x;
+  uint32_t row[U], codes[U], s[U];
+  int col[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const uint32_t u = u0 + 256 * i < units ? u0 + 256 * i : units - 1;
+    row[i] = divided(u, per_row);
+    col[i] = (int)(u - row[i] * per_row.d) * 8;
+    codes[i] = *(const uint32_t*)((const uint8_t*)X.codes + (int64_t)row[i] * X.ld_codes + (col[i] >> 1));
+    s[i] = ((const uint8_t*)X.scales)[(int64_t)row[i] * X.ld_scales + (col[i] >> 5)];
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    if (u0 + 256 * i >= units) break;
+    const int n = K - col[i];
+    const float f = s[i] == 255u ? __uint_as_float(0x7FC00000u) : mx4_scale_f32(s[i]);
+    T* y = Y + (int64_t)row[i] * ldy + col[i];
     float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = mx4_value(codes >> (4 * i), f);
+    for (int j = 0; j < 8; ++j) v[j] = mx4_value(codes[i] >> (4 * j), f);
     if (n >= 8) {
       if constexpr (sizeof(T) == 4) {
         *reinterpret_cast<f4_any*>(y) = f4_any{v[0], v[1], v[2], v[3]};
@@ -131,15 +167,15 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(int64_t M, int64_t 
       } else {
         u4_any2 o;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = (uint32_t)f2bf(v[2 * i]) | ((uint32_t)f2bf(v[2 * i + 1]) << 16);
+        for (int j = 0; j < 4; ++j) o[j] = (uint32_t)f2bf(v[2 * j]) | ((uint32_t)f2bf(v[2 * j + 1]) << 16);
         *reinterpret_cast<u4_any2*>(y) = o;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n) {
-          if constexpr (sizeof(T) == 4) y[i] = v[i];
-          else y[i] = f2bf(v[i]);
+      for (int j = 0; j < 8; ++j)
+        if (j < n) {
+          if constexpr (sizeof(T) == 4) y[j] = v[j];
+          else y[j] = f2bf(v[j]);
         }
     }
   }
@@ -295,12 +331,22 @@ __device__ __forceinline__ void load_rows(const Mx4Args& g, int64_t row, int64_t
         const u4_any2 v = *reinterpret_cast<const u4_any2*>(p + PER * i);
         x[i] = u4v{v[0], v[1], v[2], v[3]};
       }
-    } else {
+    } else if (left > 0) {   // the row's end: whole pieces of 16 bytes, then one by its elements
+      const int whole = (int)left / PER;
+      u4v tail = {0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        if (i < left) {
-          if constexpr (SRC == 1) x[i >> 2][i & 3] = __float_as_uint(p[i]);
-          else x[i >> 3][(i >> 1) & 3] |= (uint32_t)p[i] << (16 * (i & 1));
+      for (int i = 0; i < PER - 1; ++i)
+        if (whole * PER + i < left) {
+          if constexpr (SRC == 1) tail[i] = __float_as_uint(p[whole * PER + i]);
+          else tail[i >> 1] |= (uint32_t)p[whole * PER + i] << (16 * (i & 1));
+        }
+#pragma unroll
+      for (int i = 0; i < 32 / PER; ++i) {
+        if (i < whole) {
+          const u4_any2 v = *reinterpret_cast<const u4_any2*>(p + PER * i);
+          x[i] = u4v{v[0], v[1], v[2], v[3]};
+        } else if (i == whole) {
+          x[i] = tail;
         }
       }
     }
@@ -932,42 +978,69 @@ const char* bad_mx4(const llp_mx4* x, int64_t rows, int64_t K) {
   return nullptr;
 }
 
+// rows of a launch: fewer than 2^31 units of 8 values
+int64_t slice_rows(int64_t per_row) { return std::max<int64_t>(1, ((1ll << 31) - 1) / per_row); }
+
+int quantize(int dtype, int64_t M, int64_t K, llp_operand X, llp_mx4 out, hipStream_t s) {
+  const int64_t per_row = pad128(K) / 8, slice = slice_rows(per_row);
+  const int64_t size = dtype == LLP_F32 ? 4 : 2;
+  for (int64_t r = 0; r < M; r += slice) {
+    const int64_t n = std::min(M - r, slice);
+    llp_operand x = X;
+    llp_mx4 o = out;
+    if (x.idx) x.idx += r;
+    else x.ptr = (const char*)x.ptr + r * x.ld * size;
+    if (x.ptr2) {
+      if (x.idx2) x.idx2 += r;
+      else x.ptr2 = (const char*)x.ptr2 + r * x.ld2 * size;
+    }
+    o.codes = (char*)o.codes + r * o.ld_codes, o.scales = (char*)o.scales + r * o.ld_scales;
+    const uint32_t units = (uint32_t)(n * per_row);
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((units + 1023u) / 1024u), dim3(256), 0, s, units, (int)K, fast_div((uint32_t)per_row), x, o);
+    };
+    if (dtype == LLP_F32) x.ptr2 ? go(mx4_quantize_kernel<float, true>) : go(mx4_quantize_kernel<float, false>);
+    else x.ptr2 ? go(mx4_quantize_kernel<bf16_t, true>) : go(mx4_quantize_kernel<bf16_t, false>);
+    LLP_LAUNCH_CHECK();
+  }
+  return LLP_OK;
+}
+
 }  // namespace
 
 extern "C" int llp_mx4_quantize(int dtype, int64_t M, int64_t K, const llp_operand* X, const llp_mx4* out, void* stream) {
   LLP_CHECK_ARG(dtype == LLP_F32 || dtype == LLP_BF16, "llp_mx4_quantize: rows in f32 or bf16");
-  LLP_CHECK_ARG(M >= 0 && K >= 1 && K < (1ll << 31), "llp_mx4_quantize: M >= 0, 1 <= K < 2^31");
+  LLP_CHECK_ARG(M >= 0 && K >= 1 && K < (1ll << 31) - 128, "llp_mx4_quantize: M >= 0, 1 <= K < 2^31 - 128");
   if (M == 0) return LLP_OK;
   LLP_CHECK_ARG(X && X->ptr, "llp_mx4_quantize: null pointer");
   LLP_CHECK_ARG(!X->rows_dev, "llp_mx4_quantize: no device row count");
   LLP_CHECK_ARG(!X->idx2 || X->ptr2, "llp_mx4_quantize: idx2 without ptr2");
   const char* why = bad_mx4(out, M, K);
   LLP_CHECK_ARG(!why, "llp_mx4_quantize: out: %s", why);
-  const int64_t per_row = pad128(K) / 8;
-  const unsigned nb = (unsigned)std::min<int64_t>((M * per_row + 255) / 256, 1 << 20);
-  auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(nb), dim3(256), 0, (hipStream_t)stream, M, K, per_row, *X, *out);
-  };
-  if (dtype == LLP_F32) X->ptr2 ? go(mx4_quantize_kernel<float, true>) : go(mx4_quantize_kernel<float, false>);
-  else X->ptr2 ? go(mx4_quantize_kernel<bf16_t, true>) : go(mx4_quantize_kernel<bf16_t, false>);
-  LLP_LAUNCH_CHECK();
-  return LLP_OK;
+  return quantize(dtype, M, K, *X, *out, (hipStream_t)stream);
 }
 
 extern "C" int llp_mx4_dequantize(int64_t M, int64_t K, const llp_mx4* X, int dtype, void* Y, int64_t ldy, void* stream) {
   LLP_CHECK_ARG(dtype == LLP_F32 || dtype == LLP_BF16, "llp_mx4_dequantize: values in f32 or bf16");
-  LLP_CHECK_ARG(M >= 0 && K >= 1 && K < (1ll << 31) && ldy >= K, "llp_mx4_dequantize: M >= 0, 1 <= K < 2^31, ldy >= K");
+  LLP_CHECK_ARG(M >= 0 && K >= 1 && K < (1ll << 31) - 128 && ldy >= K,
+                "llp_mx4_dequantize: M >= 0, 1 <= K < 2^31 - 128, ldy >= K");
   if (M == 0) return LLP_OK;
   LLP_CHECK_ARG(Y, "llp_mx4_dequantize: null pointer");
   const char* why = bad_mx4(X, M, K);
   LLP_CHECK_ARG(!why, "llp_mx4_dequantize: X: %s", why);
-  const int64_t per_row = (K + 7) / 8;
-  const unsigned nb = (unsigned)std::min<int64_t>((M * per_row + 255) / 256, 1 << 20);
-  if (dtype == LLP_F32)
-    hipLaunchKernelGGL(mx4_dequantize_kernel<float>, dim3(nb), dim3(256), 0, (hipStream_t)stream, M, K, per_row, *X, (float*)Y, ldy);
-  else
-    hipLaunchKernelGGL(mx4_dequantize_kernel<bf16_t>, dim3(nb), dim3(256), 0, (hipStream_t)stream, M, K, per_row, *X, (bf16_t*)Y, ldy);
-  LLP_LAUNCH_CHECK();
+  const int64_t per_row = (K + 7) / 8, slice = slice_rows(per_row);
+  for (int64_t r = 0; r < M; r += slice) {
+    const int64_t n = std::min(M - r, slice);
+    llp_mx4 x = *X;
+    x.codes = (char*)x.codes + r * x.ld_codes, x.scales = (char*)x.scales + r * x.ld_scales;
+    const uint32_t units = (uint32_t)(n * per_row);
+    const dim3 grid((units + 1023u) / 1024u);
+    if (dtype == LLP_F32)
+      hipLaunchKernelGGL(mx4_dequantize_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, units, (int)K, fast_div((uint32_t)per_row), x, (float*)Y + r * ldy, ldy);
+    else
+      hipLaunchKernelGGL(mx4_dequantize_kernel<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, units, (int)K, fast_div((uint32_t)per_row), x, (bf16_t*)Y + r * ldy, ldy);
+    LLP_LAUNCH_CHECK();
+  }
   return LLP_OK;
 }
 
@@ -979,7 +1052,7 @@ extern "C" int llp_gemm_nt_mx4(int64_t M, int64_t N, int64_t K, int a_dtype, con
   LLP_CHECK_ARG(M >= 0 && N >= 0 && K >= 1 && M < (1ll << 31) && N < (1ll << 31) && K < (1ll << 31),
                 "llp_gemm_nt_mx4: M, N >= 0, K >= 1, each < 2^31");
   LLP_CHECK_ARG(act == LLP_ACT_NONE || act == LLP_ACT_RELU, "llp_gemm_nt_mx4: act must be NONE or RELU");
-  LLP_CHECK_ARG((A != nullptr) != (A4 != nullptr), "llp_gemm_nt_mx4: exactly one of A and A4");
+  LLP_CHECK_ARG(A || A4, "llp_gemm_nt_mx4: one of A and A4");
   if (M == 0 || N == 0) return LLP_OK;
   LLP_CHECK_ARG((C != nullptr) != (C4 != nullptr), "llp_gemm_nt_mx4: exactly one of C and C4");
   const char* why = bad_mx4(W, N, K);
@@ -991,12 +1064,13 @@ extern "C" int llp_gemm_nt_mx4(int64_t M, int64_t N, int64_t K, int a_dtype, con
     why = bad_mx4(A4, M, K);
     LLP_CHECK_ARG(!why, "llp_gemm_nt_mx4: A4: %s", why);
     g.A4 = *A4;
-  } else {
+  }
+  if (A) {
     LLP_CHECK_ARG(a_dtype == LLP_F32 || a_dtype == LLP_BF16, "llp_gemm_nt_mx4: A in f32 or bf16");
     LLP_CHECK_ARG(A->ptr && !A->idx && !A->ptr2 && !A->idx2 && !A->rows_dev, "llp_gemm_nt_mx4: A must be plain rows");
     LLP_CHECK_ARG(M == 1 || A->ld >= K, "llp_gemm_nt_mx4: A's rows overlap");
     g.A = A->ptr, g.lda = A->ld;
-    src = a_dtype == LLP_F32 ? 1 : 2;
+    if (!A4) src = a_dtype == LLP_F32 ? 1 : 2;
   }
   if (C4) {
     why = bad_mx4(C4, M, N);
@@ -1010,6 +1084,10 @@ extern "C" int llp_gemm_nt_mx4(int64_t M, int64_t N, int64_t K, int a_dtype, con
   }
   const int64_t n_out = C4 ? g.Np : N;
   hipStream_t s = (hipStream_t)stream;
+  if (A && A4) {
+    const int rc = quantize(a_dtype, M, K, *A, *A4, s);
+    if (rc != LLP_OK) return rc;
+  }
   // (32-bit row offsets within a tile)
   const bool near = W->ld_codes < (1 << 23) && (!A4 || A4->ld_codes < (1 << 23));
   if (A4 && near && M >= g_resident_rows && g.Kp >= 512 && g.Kp % 256 == 0) return launch_wide(g, out, n_out, s);

@@ -34,7 +34,7 @@ def _pad(k):
 class MX4:
     """A [rows, cols] matrix in MXFP4: ``codes`` uint8 [rows, pad / 2] (even element in the low half) and
     ``scales`` uint8 [rows, pad / 32] with pad = cols rounded up to 128 (zero codes behind cols)."""
-    __slots__ = ("codes", "scales", "cols", "c")
+    __slots__ = ("rows", "cols", "device", "c", "_codes", "_scales", "_both")
 
     def __init__(self, codes, scales, cols):
         for name, t, per in (("codes", codes, 2), ("scales", scales, 32)):
@@ -44,30 +44,38 @@ class MX4:
                 raise ValueError(f"MX4 {name}: rows of {_pad(cols) // per} contiguous bytes for {cols} columns")
         if cols < 1 or codes.shape[0] != scales.shape[0] or codes.device != scales.device:
             raise ValueError("MX4: codes and scales of the same rows, on the same device")
-        self.codes, self.scales, self.cols = codes, scales, int(cols)
+        self.rows, self.cols, self.device = codes.shape[0], int(cols), codes.device
+        self._codes, self._scales, self._both = codes, scales, None
         self.c = K.Mx4(codes.data_ptr(), scales.data_ptr(), codes.stride(0), scales.stride(0))
 
     @staticmethod
     def empty(rows, cols, device):
         p = _pad(cols)
         q = object.__new__(MX4)
-        q.codes = torch.empty((rows, p // 2), dtype=torch.uint8, device=device)
-        q.scales = torch.empty((rows, p // 32), dtype=torch.uint8, device=device)
-        q.cols = cols
-        q.c = K.Mx4(q.codes.data_ptr(), q.scales.data_ptr(), p // 2, p // 32)
+        # one allocation, codes first; the two views are made when they are asked for
+        q._both = torch.empty(rows * (p // 32) * 17, dtype=torch.uint8, device=device)
+        q.rows, q.cols, q.device, q._codes, q._scales = rows, cols, q._both.device, None, None
+        at = q._both.data_ptr()
+        q.c = K.Mx4(at, at + rows * (p // 2), p // 2, p // 32)
         return q
 
     @property
-    def rows(self):
-        return self.codes.shape[0]
+    def codes(self):
+        if self._codes is None:
+            p = _pad(self.cols)
+            self._codes = self._both[:self.rows * (p // 2)].view(self.rows, p // 2)
+        return self._codes
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            p = _pad(self.cols)
+            self._scales = self._both[self.rows * (p // 2):].view(self.rows, p // 32)
+        return self._scales
 
     @property
     def shape(self):
-        return (self.codes.shape[0], self.cols)
-
-    @property
-    def device(self):
-        return self.codes.device
+        return (self.rows, self.cols)
 
 
 def _rows2d(x, what):
@@ -162,18 +170,18 @@ def linear(x, w, bias=None, relu=False, out_dtype=None, out=None):
     four_out = isinstance(out, MX4)
     if not four_out and (out.dtype not in _FLOATS or (N > 1 and out.stride(1) != 1)):
         raise TypeError("linear: out in f32 or bf16 with contiguous rows")
-    code = 0
+    code, x4 = 0, x if four_in else None
     if not four_in:
+        op, code = C.byref(K.Operand(x.data_ptr(), None, None, None, x.stride(0), 0, None)), K.dtype_code(x.dtype)
         if rows > DIRECT_ROWS:
-            x, four_in = quantize(x), True
-        else:
-            op, code = C.byref(K.Operand(x.data_ptr(), None, None, None, x.stride(0), 0, None)), K.dtype_code(x.dtype)
+            x4 = MX4.empty(rows, width, dev)      # scratch: the call quantises x into it first
+    c4 = None if x4 is None else C.byref(x4.c)
     act = K.ACT_RELU if relu else K.ACT_NONE
     b = None if bias is None else bias.data_ptr()
     if four_out:
-        K.launch("llp_gemm_nt_mx4", dev, rows, N, width, code, op, C.byref(x.c) if four_in else None, C.byref(w.c), None, 0, 0,
+        K.launch("llp_gemm_nt_mx4", dev, rows, N, width, code, op, c4, C.byref(w.c), None, 0, 0,
                  C.byref(out.c), b, act)
         return out
-    K.launch("llp_gemm_nt_mx4", dev, rows, N, width, code, op, C.byref(x.c) if four_in else None, C.byref(w.c),
+    K.launch("llp_gemm_nt_mx4", dev, rows, N, width, code, op, c4, C.byref(w.c),
              out.data_ptr(), max(out.stride(0), N), K.dtype_code(out.dtype), None, b, act)
     return out if lead is None else out.reshape(*lead, N)

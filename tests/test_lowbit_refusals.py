@@ -61,7 +61,8 @@ def test_mx4_c_entries_refuse():
         assert rc == 10001 and why in msg, msg
     for args, why in (
             ((2, 2, 128, 0, None, None, C.byref(ok), 4096, 2, 0, None, None, 0, None), "one of A"),
-            ((2, 2, 128, 0, C.byref(op), C.byref(ok), C.byref(ok), 4096, 2, 0, None, None, 0, None), "one of A"),
+            ((2, 2, 128, 0, C.byref(K.Operand(4096, 4096, None, None, 128, 0, None)), C.byref(ok), C.byref(ok), 4096, 2, 0, None,
+              None, 0, None), "plain rows"),
             ((2, 2, 128, 0, None, C.byref(ok), C.byref(ok), None, 2, 0, None, None, 0, None), "one of C"),
             ((2, 2, 128, 0, None, C.byref(ok), C.byref(ok), 4096, 2, 0, C.byref(ok), None, 0, None), "one of C"),
             ((2, 2, 128, 0, None, C.byref(ok), C.byref(ok), 4096, 2, 0, None, None, 2, None), "act"),
