@@ -5,7 +5,6 @@
 
 #include <algorithm>
 #include <type_traits>
-#include <stdlib.h>
 
 #include "llp_common.h"
 
@@ -392,31 +391,54 @@ __global__ __launch_bounds__(512) void gemm_mx4_rows_kernel(Mx4Args g) {
   for (int c = 0; c < 2; ++c)
 #pragma unroll
     for (int e = 0; e < MT; ++e) acc[c][e] = float4_t{0.f, 0.f, 0.f, 0.f};
-  const int64_t nk = g.Kp / 128;
-  for (int64_t k = wave; k < nk; k += 8) {
-    const int64_t kb = 4 * k + q;
-    u4v w[2], x[MT][SRC == 1 ? 8 : SRC == 2 ? 4 : 1];
+  const int nk = (int)(g.Kp / 128);
+  constexpr int XR = SRC == 1 ? 8 : SRC == 2 ? 4 : 1;
+  struct Step {
+    u4v w[2], x[MT][XR];
     int ws[2], xs[MT];
+  };
+  auto load = [&](int k, Step& t) {
+    const int64_t kb = 4 * (int64_t)k + q;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int64_t n = n0 + 16 * c + li;
-      w[c] = u4v{0, 0, 0, 0};
-      ws[c] = 0;
+      t.w[c] = u4v{0, 0, 0, 0};
+      t.ws[c] = 0;
       if (n < g.N) {
-        w[c] = *(const u4v*)((const uint8_t*)g.W.codes + n * g.W.ld_codes + kb * 16);
-        ws[c] = ((const uint8_t*)g.W.scales)[n * g.W.ld_scales + kb];
+        t.w[c] = *(const u4v*)((const uint8_t*)g.W.codes + n * g.W.ld_codes + kb * 16);
+        t.ws[c] = ((const uint8_t*)g.W.scales)[n * g.W.ld_scales + kb];
       }
     }
 #pragma unroll
-    for (int e = 0; e < MT; ++e) load_rows<SRC>(g, m0 + 16 * e + li, kb, m0 + 16 * e + li < g.M, x[e], xs[e]);
+    for (int e = 0; e < MT; ++e) load_rows<SRC>(g, m0 + 16 * e + li, kb, m0 + 16 * e + li < g.M, t.x[e], t.xs[e]);
+  };
+  auto compute = [&](Step& t) {
 #pragma unroll
     for (int e = 0; e < MT; ++e) {
-      const v8i a = as_block<SRC>(x[e], xs[e]);
+      const v8i a = as_block<SRC>(t.x[e], t.xs[e]);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const v8i b = v8i{(int)w[c][0], (int)w[c][1], (int)w[c][2], (int)w[c][3], 0, 0, 0, 0};
-        acc[c][e] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, acc[c][e], 4, 4, 0, ws[c], 0, xs[e]);
+        const v8i b = v8i{(int)t.w[c][0], (int)t.w[c][1], (int)t.w[c][2], (int)t.w[c][3], 0, 0, 0, 0};
+        acc[c][e] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, acc[c][e], 4, 4, 0, t.ws[c], 0, t.xs[e]);
       }
+    }
+  };
+  if constexpr (MT == 1) {   // the next step's loads in flight under this step's work
+    Step t[2];
+    if (wave < nk) load(wave, t[0]);
+    for (int k = wave; k < nk; k += 16) {
+      if (k + 8 < nk) load(k + 8, t[1]);
+      compute(t[0]);
+      if (k + 8 < nk) {
+        if (k + 16 < nk) load(k + 16, t[0]);
+        compute(t[1]);
+      }
+    }
+  } else {
+    for (int k = wave; k < nk; k += 8) {
+      Step t;
+      load(k, t);
+      compute(t);
     }
   }
   const int live = (int)(nk < 8 ? nk : 8);   // waves that had a step
@@ -1044,8 +1066,6 @@ extern "C" int llp_mx4_dequantize(int64_t M, int64_t K, const llp_mx4* X, int dt
   return LLP_OK;
 }
 
-int64_t g_tiled = getenv("TT") ? atoll(getenv("TT")) : 1024;
-int64_t g_resident_rows = getenv("RR") ? atoll(getenv("RR")) : 8192;
 extern "C" int llp_gemm_nt_mx4(int64_t M, int64_t N, int64_t K, int a_dtype, const llp_operand* A, const llp_mx4* A4,
                                const llp_mx4* W, void* C, int64_t ldc, int c_dtype, const llp_mx4* C4,
                                const float* bias, int act, void* stream) {
@@ -1088,9 +1108,16 @@ extern "C" int llp_gemm_nt_mx4(int64_t M, int64_t N, int64_t K, int a_dtype, con
     const int rc = quantize(a_dtype, M, K, *A, *A4, s);
     if (rc != LLP_OK) return rc;
   }
-  // (32-bit row offsets within a tile)
+  // Which kernel, by the tiles there are (us, rows in MXFP4, bf16 out; 32-bit row offsets within a tile):
+  //   few 32 x 32 tiles: the rows kernel, K over a workgroup's waves (1024 x 1024 x 1024: 9.1, tiled 10.2;
+  //     2048 rows: 15.4 / 10.4; 4096 x 1433 -> 257: 12.9 / 15.4; 8192: 19.6 / 15.7), 16 rows at a time while that
+  //     makes no more than two workgroups a CU (256 x 1024 x 1024: 5.7, 64 at a time 6.3; 512 rows: 9.7 / 6.3);
+  //   no more 128 x 256 tiles than CUs: tiled (8192 x 1024 x 1024: 12.3, wide 13.4; 4096 x 2048 x 2048: 17.2 / 19.0);
+  //   more, and K in whole steps of 256: wide (16384 x 1024 x 1024: 15.5, tiled 18.1; 262144 x 2048 x 2048: 651 / 830).
   const bool near = W->ld_codes < (1 << 23) && (!A4 || A4->ld_codes < (1 << 23));
-  if (A4 && near && M >= g_resident_rows && g.Kp >= 512 && g.Kp % 256 == 0) return launch_wide(g, out, n_out, s);
-  if (A4 && near && (n_out + 31) / 32 * ((M + 31) / 32) >= g_tiled) return launch_tiled<2, 4>(g, out, n_out, s);
-  return M <= 16 ? launch_rows<1>(g, src, out, n_out, s) : launch_rows<4>(g, src, out, n_out, s);
+  if (A4 && near && (n_out + 31) / 32 * ((M + 31) / 32) > 1024) {
+    if (g.Kp >= 512 && g.Kp % 256 == 0 && (n_out + 255) / 256 * ((M + 127) / 128) > 256) return launch_wide(g, out, n_out, s);
+    return launch_tiled<2, 4>(g, out, n_out, s);
+  }
+  return (n_out + 31) / 32 * ((M + 15) / 16) <= 512 ? launch_rows<1>(g, src, out, n_out, s) : launch_rows<4>(g, src, out, n_out, s);
 }

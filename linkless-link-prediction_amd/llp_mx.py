@@ -21,9 +21,14 @@ import torch
 
 import llp_hip as K
 
-# f32 / bf16 inputs of up to this many rows are quantised inside the product (one launch); more rows
-# are quantised first, once, instead of once for each 32 columns of the result.
-DIRECT_ROWS = 64
+def _direct(rows, cols):
+    """Whether rows in f32 / bf16 are quantised inside the product (one launch) or first, once, instead of
+    once for each 32 columns of the result.  GPU time in us, inside / first, bf16 rows: 256 x 1024 -> 1024 8.3 / 8.6,
+    512 rows 9.9 / 9.4; 64 x 2048 -> 2048 7.3 / 8.6, 128 rows 12.0 / 11.3; 64 x 4096 -> 64 10.3 / 11.0;
+    1 x 8415 -> 256 10.6 / 10.8, 16 rows 27.7 / 13.3; 512 x 128 -> 1024 5.6 / 6.5, 1024 rows 9.3 / 7.0."""
+    return rows <= 512 and rows * cols <= (1 << 18 if cols <= 4096 else 1 << 15)
+
+
 _FLOATS = (torch.float32, torch.bfloat16)
 
 
@@ -173,7 +178,7 @@ def linear(x, w, bias=None, relu=False, out_dtype=None, out=None):
     code, x4 = 0, x if four_in else None
     if not four_in:
         op, code = C.byref(K.Operand(x.data_ptr(), None, None, None, x.stride(0), 0, None)), K.dtype_code(x.dtype)
-        if rows > DIRECT_ROWS:
+        if not _direct(rows, width):
             x4 = MX4.empty(rows, width, dev)      # scratch: the call quantises x into it first
     c4 = None if x4 is None else C.byref(x4.c)
     act = K.ACT_RELU if relu else K.ACT_NONE

@@ -145,7 +145,7 @@ def _check_linear(x, xv, w, wv, b, relu, out_dtype, **kw):
     return y
 
 
-# rows: single tokens, around the tile sizes, above the direct rows; K and N odd and around the tiles
+# rows: single ones, around the tile sizes and each kernel's range; K and N odd and around the tiles
 SHAPES = [(1, 16, 8), (1, 1024, 1024), (1, 1433, 257), (2, 33, 1), (3, 128, 33), (16, 300, 130), (31, 64, 32), (32, 129, 64),
           (33, 256, 128), (47, 1433, 257), (64, 8415, 40), (65, 128, 96), (129, 1000, 129), (255, 512, 256), (257, 384, 300),
           (300, 2048, 64), (513, 128, 513), (1030, 257, 1024), (4099, 64, 72), (2050, 129, 513),
@@ -217,7 +217,7 @@ def test_linear_same_for_any_number_of_rows():
     wv = Q.mx4_values(w.codes.cpu().numpy(), w.scales.cpu().numpy(), 320)
     _, size = Q.mx4_linear(_f64(x), wv)
     full = _f64(m.linear(x, w))
-    for n in (1, 5, 64, 65, 128):
+    for n in (1, 5, 64, 65, 128, 400):
         assert (np.abs(_f64(m.linear(x[:n], w)) - full[:n]) <= 2 * 321 * 2.0 ** -23 * size[:n]).all()
         assert (np.abs(_f64(m.linear(m.quantize(x[:n]), w, out_dtype=torch.float32)) - full[:n]) <= 2 * 321 * 2.0 ** -23 * size[:n]).all()
 
