@@ -29,6 +29,7 @@ import torch
 import torch.distributed as dist
 
 import llp_hip as K
+import llp_optim
 
 # Philox streams per step (csrc/llp_common.h LLP_STREAMS_PER_STEP): a draw of step s at
 # offset o uses stream STREAMS_PER_STEP * s + o.  Offsets under self.seed: the context
@@ -40,6 +41,7 @@ DENSE_NEG_STREAM = STREAMS_PER_STEP - 2
 MAX_RW_STEP = STREAMS_PER_STEP - 3          # walks + negatives below DENSE_NEG_STREAM
 # dropout Philox keys (EngineBase._dropout): one per module, one stream per layer and step
 DROP_ENCODER, DROP_PREDICTOR, DROP_TEACHER_PRED = 0, 1, 2
+_ADAMW_KEY = 0xADA << 44      # Philox key of the 8-bit moments' rounding, beside self.seed
 # x at most this dense runs the full-batch student's first layer sparse (llp_spmm_rows): a
 # gathered 512-B weight row per nonzero against a dense 256-wide MFMA pass over every column
 SPARSE_X_MAX_DENSITY = 0.05
@@ -287,17 +289,25 @@ class EngineBase:
     # ------------------------------------------------------------------ setup
     def _init_optimizer_state(self):
         opt = self.optimizer
-        if not isinstance(opt, torch.optim.Adam):
-            raise NotImplementedError("the LLP engine implements torch.optim.Adam (src/main.py:400-402)")
+        if not isinstance(opt, (torch.optim.Adam, llp_optim.AdamW)):
+            raise NotImplementedError("the LLP engine implements torch.optim.Adam (src/main.py:400-402) and AdamW")
         g = opt.param_groups
-        if len(g) != 1 or g[0]["weight_decay"] != 0 or g[0]["amsgrad"] or g[0].get("maximize", False):
-            raise NotImplementedError("Adam with one param group, no weight decay / amsgrad / maximize")
+        # decoupled decay (torch.optim.AdamW with one, llp_optim.AdamW) takes the AdamW step
+        self.adamw = None
+        self._use_adamw = isinstance(opt, llp_optim.AdamW) or (g[0].get("decoupled_weight_decay", False)
+                                                               and g[0]["weight_decay"] != 0)
+        if len(g) != 1 or (g[0]["weight_decay"] != 0 and not self._use_adamw) or g[0].get("amsgrad", False) \
+                or g[0].get("maximize", False):
+            raise NotImplementedError("Adam with one param group, no weight decay / amsgrad / maximize "
+                                      "(weight decay: torch.optim.AdamW or llp_optim.AdamW)")
         ids = {id(p) for p in g[0]["params"]}
         if ids != {id(p) for p in self.all_params}:
             raise ValueError("optimizer must hold exactly model.parameters() + predictor.parameters()")
         step0 = 0
+        if isinstance(opt, llp_optim.AdamW):
+            opt.hand_over()
         for p in self.all_params:
-            st = opt.state[p]
+            st = opt.init_state(p) if isinstance(opt, llp_optim.AdamW) else opt.state[p]
             if "exp_avg" not in st:
                 st["step"] = torch.tensor(0.0)
                 st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
@@ -326,6 +336,17 @@ class EngineBase:
         self.ws_sumsq = torch.empty(K.grad_sumsq_ws_bytes(self.n_desc, self.max_numel) // 4 + 1, dtype=torch.float32,
                                     device=self.dev)
         K.refresh_shadows(self.descs_dev, self.n_desc, self.max_numel)
+        if self._use_adamw:
+            sh = [self._shadows.get(id(p), (None, None, 0, 0)) for p in self.all_params]
+            params, grads = [p.data for p in self.all_params], [p.grad for p in self.all_params]
+            more = dict(groups=self.param_groups_of, copies=[(a, ld) for a, _, ld, _ in sh],
+                        copies_t=[(b, ld) for _, b, _, ld in sh])
+            if isinstance(opt, llp_optim.AdamW):
+                self.adamw = opt.table(self.all_params, grads, **more)
+            else:
+                sts = [opt.state[p] for p in self.all_params]
+                self.adamw = llp_optim.AdamWTable(params, grads, [t["exp_avg"] for t in sts],
+                                                  [t["exp_avg_sq"] for t in sts], **more)
 
     def refresh_weights(self):
         """Call after loading weights into the modules (reset_parameters, load_state_dict)."""
@@ -732,6 +753,11 @@ class EngineBase:
         K.grad_sumsq(self.descs_dev, self.n_desc, self.max_numel, self.n_groups, self.sumsq, self.ws_sumsq,
                      ticket=self.sumsq_ticket, n_work=self.n_work_sumsq)
         b1, b2 = g["betas"]
+        if self.adamw is not None:   # (the gradients stay unclipped: the coefficient is applied as they are read)
+            self.adamw.step(self.adam_step, lr=float(g["lr"]), betas=(float(b1), float(b2)), eps=float(g["eps"]),
+                            weight_decay=float(g["weight_decay"]), sumsq=self.sumsq, max_norm=1.0,
+                            seed=self.seed ^ _ADAMW_KEY)
+            return
         # the one-launch Adam reads the step counter; the step-end launch advances it
         K.adam_step(self.descs_dev, self.n_desc, self.max_numel, self.sumsq, 1.0, float(g["lr"]), float(b1),
                     float(b2), float(g["eps"]), self.adam_step, fused=True, n_work=self.n_work_adam)
@@ -856,7 +882,7 @@ class DistillEngine(EngineBase):
     student ``model`` (MLP), ``predictor`` (LinkPredictor), the frozen
     ``teacher_predictor`` and teacher embeddings ``t_h``; ``x`` the node
     features; ``row``/``col`` the sampler graph (data.adj_t, src/main.py:56);
-    ``optimizer`` a torch.optim.Adam over model+predictor parameters whose
+    ``optimizer`` a torch.optim.Adam (or AdamW, llp_optim.AdamW) over model+predictor parameters whose
     hyper-parameters and state this engine uses.
     """
 

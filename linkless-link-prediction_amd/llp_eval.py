@@ -11,12 +11,17 @@ Scores are computed by ``EdgeScorer``: the predictor's first GEMM reads
 ``h[e0] * h[e1]`` through a gathered operand (no materialised pair tensor),
 hidden layers keep bias+ReLU in the epilogue, and the Linear(H,1)+sigmoid
 head is one reduction kernel.  Chunks of ``chunk`` edges bound the scratch.
+
+dtype "mxfp4": the student answers in 4 bits (llp_mx).  Node features, pair products and hidden
+activations are quantised (a hidden layer hands MXFP4 rows to the next), weights too; embeddings are
+bf16 and the Linear(H, 1) head works on the last hidden layer in bf16.
 """
 from __future__ import annotations
 
 import torch
 
 import llp_hip as K
+import llp_mx
 
 TRANSDUCTIVE_KS = (10, 20, 30, 50)          # src/train_teacher_gnn.py:118
 COLLAB_KS = (10, 50, 100)                   # src/train_teacher_gnn.py:132
@@ -34,14 +39,15 @@ class EdgeScorer:
 
     def __init__(self, predictor, dtype=torch.float32, chunk: int = 1 << 18):
         self.predictor = predictor
-        self.dtype = dtype
+        self.mx = dtype == "mxfp4"
+        self.dtype = torch.bfloat16 if self.mx else dtype
         self.chunk = int(chunk)
         self.kind = predictor.predictor
 
     def _weights(self):
         lins = list(self.predictor.lins)
-        hid = [(l.weight.detach().to(self.dtype).contiguous(), l.bias.detach().float().contiguous())
-               for l in lins[:-1]]
+        hid = [(llp_mx.quantize(l.weight.detach()) if self.mx else l.weight.detach().to(self.dtype).contiguous(),
+                l.bias.detach().float().contiguous()) for l in lins[:-1]]
         head = (lins[-1].weight.detach().float().reshape(-1).contiguous(), lins[-1].bias.detach().float().contiguous())
         return hid, head
 
@@ -65,6 +71,12 @@ class EdgeScorer:
         for s in range(0, E, self.chunk):
             n = min(self.chunk, E - s)
             i0, i1 = e0[s:s + n], e1[s:s + n]
+            if self.mx:
+                z = llp_mx.quantize(h, i0, h, i1)
+                for l, (W, b) in enumerate(hid):
+                    z = llp_mx.linear(z, W, b, relu=True, out_dtype="mx4" if l + 1 < len(hid) else torch.bfloat16)
+                K.head_fwd(z, n, z.shape[1], w2, b2, prob=out[s:s + n])
+                continue
             A = K.operand(h, i0, h, i1)
             z = None
             for W, b in hid:
@@ -75,6 +87,31 @@ class EdgeScorer:
         return out
 
 
+def _norm_relu(nm, h):
+    """relu(norm(h)) in place, in eval mode."""
+    batch = isinstance(nm, torch.nn.BatchNorm1d)
+    stats = torch.empty(2, h.shape[1] if batch else h.shape[0], dtype=torch.float32, device=h.device)
+    K.norm_fwd(K.NORM_BATCH if batch else K.NORM_LAYER, h, h, stats,
+               None if nm.weight is None else nm.weight.detach(), None if nm.bias is None else nm.bias.detach(),
+               float(nm.eps), not batch, running_mean=getattr(nm, "running_mean", None),
+               running_var=getattr(nm, "running_var", None), relu=True)
+
+
+def _embed_mlp_mx(layers, norms, x):
+    """embed_mlp in MXFP4: hidden layers hand MXFP4 rows on (bf16 through a norm), the embedding is bf16."""
+    h = x if x.dtype in (torch.float32, torch.bfloat16) else x.float()
+    h = h.contiguous()
+    for l, lin in enumerate(layers):
+        W, b = llp_mx.quantize(lin.weight.detach()), lin.bias.detach().float()
+        last = l == len(layers) - 1
+        if norms and not last:
+            h = llp_mx.linear(h, W, b, out_dtype=torch.bfloat16)
+            _norm_relu(norms[l], h)
+        else:
+            h = llp_mx.linear(h, W, b, relu=not last, out_dtype=torch.bfloat16 if last else "mx4")
+    return h
+
+
 @torch.no_grad()
 def embed_mlp(model, x: torch.Tensor, dtype=torch.float32) -> torch.Tensor:
     """model(x) for the student MLP in eval mode (no dropout, src/models.py:45-54; with
@@ -82,10 +119,12 @@ def embed_mlp(model, x: torch.Tensor, dtype=torch.float32) -> torch.Tensor:
     statistics)."""
     if x.device.type != "cuda":
         raise RuntimeError("embed_mlp runs only on a HIP device (no CPU fallback)")
-    dc = K.dtype_code(dtype)
-    A = K.operand(x.to(dtype).contiguous())
     layers = list(model.layers)
     norms = list(getattr(model, "norms", []))
+    if dtype == "mxfp4":
+        return _embed_mlp_mx(layers, norms, x)
+    dc = K.dtype_code(dtype)
+    A = K.operand(x.to(dtype).contiguous())
     h = None
     M = x.shape[0]
     for l, lin in enumerate(layers):
@@ -96,13 +135,7 @@ def embed_mlp(model, x: torch.Tensor, dtype=torch.float32) -> torch.Tensor:
         K.gemm_nt(A, K.operand(W), M, W.shape[0], W.shape[1], h, dc, bias=lin.bias.detach().float(),
                   act=K.ACT_NONE if (last or normed) else K.ACT_RELU)
         if normed:
-            nm = norms[l]
-            batch = isinstance(nm, torch.nn.BatchNorm1d)
-            stats = torch.empty(2, W.shape[0] if batch else M, dtype=torch.float32, device=x.device)
-            K.norm_fwd(K.NORM_BATCH if batch else K.NORM_LAYER, h, h, stats,
-                       None if nm.weight is None else nm.weight.detach(), None if nm.bias is None else nm.bias.detach(),
-                       float(nm.eps), not batch, running_mean=getattr(nm, "running_mean", None),
-                       running_var=getattr(nm, "running_var", None), relu=True)
+            _norm_relu(norms[l], h)
         A = K.operand(h)
     return h
 

@@ -21,6 +21,7 @@ import torch
 
 import llp_hip as K
 
+
 def _direct(rows, cols):
     """Whether rows in f32 / bf16 are quantised inside the product (one launch) or first, once, instead of
     once for each 32 columns of the result.  GPU time in us, inside / first, bf16 rows: 256 x 1024 -> 1024 8.3 / 8.6,
@@ -83,13 +84,17 @@ class MX4:
         return (self.rows, self.cols)
 
 
+def _on_gpu(dev):
+    if dev.type != "cuda":
+        raise RuntimeError("LLP ops run only on the MI355X HIP device (got a CPU tensor; no CPU fallback)")
+
+
 def _rows2d(x, what):
     if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
         raise ValueError(f"{what}: a 2-D tensor with contiguous rows")
     if x.dtype not in _FLOATS:
         raise TypeError(f"{what}: f32 or bf16, not {x.dtype}")
-    if not x.is_cuda:
-        raise RuntimeError("LLP ops run only on the MI355X HIP device (got a CPU tensor; no CPU fallback)")
+    _on_gpu(x.device)
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{what}: MXFP4 has no gradient; call it under torch.no_grad()")
 
@@ -135,6 +140,7 @@ def quantize(x, idx=None, x2=None, idx2=None, out=None):
 
 def dequantize(q, dtype=torch.float32, out=None):
     """The values of q (exact in f32; in bf16 too, down to 2^-133)."""
+    _on_gpu(q.device)
     if out is None:
         out = torch.empty(q.rows, q.cols, dtype=dtype, device=q.device)
     elif tuple(out.shape) != q.shape or out.device != q.device or (q.cols > 1 and out.stride(1) != 1):
@@ -155,6 +161,7 @@ def linear(x, w, bias=None, relu=False, out_dtype=None, out=None):
             lead = x.shape[:-1]
             x = x.reshape(-1, x.shape[-1])
         _rows2d(x, "linear")
+    _on_gpu(x.device)
     rows, width = x.shape
     N, dev = w.rows, x.device
     if width != w.cols or dev != w.device:

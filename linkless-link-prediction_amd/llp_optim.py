@@ -94,6 +94,12 @@ class AdamWTable:
             raise ValueError("AdamWTable: a clip group in 0..7 for each param")
         self.n_groups = max(groups) + 1
         copies, copies_t = self._copies(copies, params, dev), self._copies(copies_t, params, dev)
+        shapes = [(p.shape[0], p.shape[1]) if p.dim() == 2 else (1, p.numel()) for p in params]
+        for i, (c, ct) in enumerate(zip(copies, copies_t)):
+            if c[0] is not None and ct[0] is not None and c[0].dtype != ct[0].dtype:
+                raise TypeError("AdamWTable: a param's copies in one dtype")
+            self._fits(c, *shapes[i], i)
+            self._fits(ct, *shapes[i][::-1], i)
         if not params[0].is_cuda:
             raise RuntimeError("AdamWTable runs only on the MI355X HIP device (got CPU tensors; no CPU fallback)")
         self._apart(ins, outs, grads, copies, copies_t, values)
@@ -104,11 +110,9 @@ class AdamWTable:
             return None if ts is None else ts[i].data_ptr()
 
         for i, p in enumerate(params):
-            rows, cols = (p.shape[0], p.shape[1]) if p.dim() == 2 else (1, p.numel())
+            rows, cols = shapes[i]
             c, ct = copies[i], copies_t[i]
             kinds = {t.dtype for t, _ in (c, ct) if t is not None}
-            if len(kinds) > 1:
-                raise TypeError("AdamWTable: a param's copies in one dtype")
             descs.append(K.AdamWDesc(
                 p.data_ptr(), grads[i].data_ptr(), exp_avg[i].data_ptr(), exp_avg_sq[i].data_ptr(),
                 at(ins.get("exp_avg_scale"), i), at(ins.get("exp_avg_sq_scale"), i), outs["params"][i].data_ptr(),
@@ -153,6 +157,18 @@ class AdamWTable:
                     raise ValueError("AdamWTable: copies contiguous, or given with their row stride")
             got.append((t, int(ld)))
         return got
+
+    @staticmethod
+    def _fits(copy, rows, cols, i):
+        """A copy of [rows, cols] lies within its tensor's storage."""
+        t, ld = copy
+        if t is None:
+            return
+        if not ld and t.numel() != rows * cols:
+            raise ValueError(f"AdamWTable: a copy of param {i} has {t.numel()} elements, {rows * cols} are needed")
+        room = t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
+        if ld and (ld < cols or (rows - 1) * ld + cols > room):
+            raise ValueError(f"AdamWTable: rows {ld} apart of a copy of param {i} ([{rows}, {cols}]) leave its storage")
 
     @staticmethod
     def _apart(ins, outs, grads, copies, copies_t, values):
@@ -210,15 +226,33 @@ class AdamWTable:
                  K.dtype_code(self.values_dtype))
 
 
+def add_flags(parser):
+    """--optimizer / --weight_decay / --optim_bits of the training commands."""
+    parser.add_argument('--optimizer', type=str, default='adam', choices=['adam', 'adamw'])
+    parser.add_argument('--weight_decay', type=float, default=0.01, help="decoupled decay of --optimizer=adamw")
+    parser.add_argument('--optim_bits', type=int, default=32, choices=[32, 8],
+                        help="bits of the moments of --optimizer=adamw")
+
+
+def from_args(args, params):
+    """The optimizer that those flags name."""
+    if getattr(args, "optimizer", "adam") == "adam":
+        if getattr(args, "optim_bits", 32) != 32:
+            raise ValueError("--optim_bits=8 needs --optimizer=adamw")
+        return torch.optim.Adam(params, lr=args.lr)
+    return AdamW(params, lr=args.lr, weight_decay=args.weight_decay, state_bits=args.optim_bits)
+
+
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW on the HIP step: ``lr``, ``betas``, ``eps``, ``weight_decay`` as there (no amsgrad,
     no maximize); ``state_bits`` 32 or 8; ``seed`` of the 8-bit moments' rounding.
 
     Params in f32 or bf16 on the GPU, dense gradients of one dtype in a group.  ``state[p]`` holds
     ``step`` and exp_avg / exp_avg_sq (f32, or uint8 codes with exp_avg_scale / exp_avg_sq_scale).  A
-    param without a gradient is left as it is; the update number is the group's, as long as its
-    params always step together.  After a first eager step on the same gradients' storage ``step()`` can
-    be captured into a graph (``zero_grad(set_to_none=False)``)."""
+    param without a gradient is left as it is; the update number is the group's, so params that step
+    together must always have done so (refused else).  After a first eager step on the same gradients'
+    storage ``step()`` can be captured into a graph (``zero_grad(set_to_none=False)``); a graph works on the
+    state that was there, so ``load_state_dict`` asks for a new capture."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
         if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and 0 <= betas[0] < 1 and 0 <= betas[1] < 1):
@@ -227,7 +261,18 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("AdamW: state_bits 32 or 8")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
         self.state_bits, self.seed = int(state_bits), int(seed)
-        self._tables = {}      # per group: (addresses, table, device step counter)
+        self._tables = {}      # per group: (addresses, table, device step counter, params)
+        self._counters, self._captured = {}, []
+
+    def __getstate__(self):
+        self._sync_steps()
+        return {**super().__getstate__(), "state_bits": self.state_bits, "seed": self.seed}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._tables = {}
+        self.__dict__.setdefault("_counters", {})
+        self.__dict__.setdefault("_captured", [])
 
     def init_state(self, p):
         """state[p], made on first use."""
@@ -267,26 +312,38 @@ class AdamW(torch.optim.Optimizer):
             where = tuple((p.data_ptr(), g.data_ptr(), p.numel(), p.dtype, g.dtype,
                            self.init_state(p)["exp_avg"].data_ptr()) for p, g in zip(params, grads))
             at = self._tables.get(i)
+            capturing = params[0].is_cuda and torch.cuda.is_current_stream_capturing()
             if at is None or at[0] != where:
-                if params[0].is_cuda and torch.cuda.is_current_stream_capturing():
+                if capturing:
                     raise RuntimeError("AdamW: run one eager step on these gradients before a capture")
-                steps = {float(self.state[p]["step"]) for p in params} if at is None else {float(at[2].item())}
+                if at is not None:
+                    self._sync_steps()
+                steps = {float(self.state[p]["step"]) for p in params}
                 if len(steps) != 1:
                     raise RuntimeError("AdamW: a group's params must have taken the same number of steps")
-                ctr = torch.full((1,), int(steps.pop()), dtype=torch.int64, device=params[0].device)
-                at = self._tables[i] = (where, self.table(params, grads), ctr)
-            _, table, ctr = at
+                table = self.table(params, grads)
+                ctr = self._counters.setdefault(i, torch.zeros(1, dtype=torch.int64, device=params[0].device))
+                ctr.fill_(int(steps.pop()))
+                at = self._tables[i] = (where, table, ctr, params)
+            if capturing:
+                self._captured.append(at)      # a replay reads the table
+            _, table, ctr, _ = at
             table.step(ctr, lr=float(group["lr"]), betas=group["betas"], eps=float(group["eps"]),
                        weight_decay=float(group["weight_decay"]), seed=self.seed + (i << 48))
             K.launch("llp_increment", ctr.device, ctr.data_ptr())
         return loss
 
+    def hand_over(self):
+        """state[p]["step"] brought up to date, for whoever takes over the state's tensors (the training
+        engines); a later ``step`` continues from what state[p]["step"] then holds."""
+        self._sync_steps()
+        self._tables = {}
+
     def _sync_steps(self):
-        for i, (_, _, ctr) in self._tables.items():
+        for _, _, ctr, params in self._tables.values():
             n = float(ctr.item())
-            for p in self.param_groups[i]["params"]:
-                if "step" in self.state[p]:
-                    self.state[p]["step"] = torch.tensor(n)
+            for p in params:
+                self.state[p]["step"] = torch.tensor(n)
 
     def state_dict(self):
         self._sync_steps()

@@ -17,7 +17,9 @@ Each epoch runs on a cached engine (llp_engine.DistillEngine /
 llp_teacher.TeacherEngine) bound to the given modules and optimizer: the
 modules' parameters stay the masters (state_dict / torch.save unchanged), the
 optimizer's Adam state is the engine's.  ``args.dtype`` ('fp32' default, as
-the reference; 'bf16' for the MFMA fast path) is an additive option.
+the reference; 'bf16' for the MFMA fast path) is an additive option, as are an
+llp_optim.AdamW / torch.optim.AdamW in place of Adam and ``args.eval_dtype``
+('fp32' default, 'bf16', 'mxfp4': the MLP's evaluation, llp_eval).
 
 Shuffling: the reference's DataLoader(shuffle=True) permutations come from
 torch's global generator; here one seed is drawn from that generator per
@@ -236,9 +238,14 @@ def _train_teacher_mlp(model, predictor, data, pos_train_edge, mp_edges, optimiz
     return eng.end_epoch(E)
 
 
-def _embed(model, data, x, adj, encoder_name):
+def _eval_dtype(args):
+    """args.eval_dtype ('fp32' default, 'bf16', 'mxfp4') as llp_eval takes it."""
+    return {"fp32": torch.float32, "bf16": torch.bfloat16, "mxfp4": "mxfp4"}[getattr(args, "eval_dtype", "fp32")]
+
+
+def _embed(model, data, x, adj, encoder_name, dtype=torch.float32):
     if encoder_name == "mlp":
-        return llp_eval.embed_mlp(model, x)
+        return llp_eval.embed_mlp(model, x, dtype)
     for k, eng in _ENGINES.items():
         if k[0] == "teacher" and k[1] == id(model) and k[4] == id(data):
             return eng.embed()       # the engine's resident graph is this data's graph
@@ -253,22 +260,24 @@ def test_transductive(model, predictor, data, split_edge, evaluator, batch_size,
     model.eval()
     predictor.eval()
     x = data.x if data.x.is_cuda else data.x.to("cuda")
-    h = _embed(model, data, x, getattr(data, "adj_t", None), encoder_name)
-    return llp_eval.test_transductive(h, predictor, split_edge, dataset)
+    dt = _eval_dtype(args)
+    h = _embed(model, data, x, getattr(data, "adj_t", None), encoder_name, dt)
+    return llp_eval.test_transductive(h, predictor, split_edge, dataset, dt)
 
 
 @torch.no_grad()
 def test_production(model, predictor, val_data, inference_data, test_edge_bundle, negative_samples, evaluator,
-                    batch_size, encoder_name, dataset):
+                    batch_size, encoder_name, dataset, args=None):
     """src/train_teacher_gnn.py:157-268 -> (results, h of val_data)."""
     model.eval()
     predictor.eval()
-    hv = _embed(model, val_data, val_data.x.to("cuda"), val_data.edge_index.to("cuda"), encoder_name)
+    dt = _eval_dtype(args)
+    hv = _embed(model, val_data, val_data.x.to("cuda"), val_data.edge_index.to("cuda"), encoder_name, dt)
     hi = _embed(model, inference_data, inference_data.x.to("cuda"), inference_data.edge_index.to("cuda"),
-                encoder_name)
+                encoder_name, dt)
     ve = val_data.edge_label_index.t()
     lab = val_data.edge_label.bool()
-    return llp_eval.test_production(hv, hi, predictor, ve[lab], ve[~lab], test_edge_bundle, negative_samples)
+    return llp_eval.test_production(hv, hi, predictor, ve[lab], ve[~lab], test_edge_bundle, negative_samples, dt)
 
 
 __all__ = ["train_minibatch", "train", "train_teacher", "test_transductive", "test_production", "K"]

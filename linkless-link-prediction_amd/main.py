@@ -5,6 +5,11 @@ file :465-513).  Same flags and outputs; additive flags only:
   --dtype {fp32,bf16}   compute dtype of the HIP engine (fp32 = the reference's)
   --synthetic           seeded graph of the dataset's shape when no dataset
                         file exists (no network here; see llp_datasets.py)
+  --optimizer {adam,adamw} --weight_decay D --optim_bits {32,8}
+                        AdamW with decoupled decay, its moments in f32 or in 8 bits
+                        (llp_optim); default the reference's Adam
+  --eval_dtype {fp32,bf16,mxfp4}
+                        what the student answers in when it is evaluated (llp_eval)
 
 Training runs in llp_train (DistillEngine, hand-written gfx950 kernels);
 evaluation in llp_eval (device Hits@K / AUC).  Teacher artefacts are read
@@ -20,6 +25,7 @@ import numpy as np
 import torch
 
 import llp_datasets
+import llp_optim
 import llp_split
 import llp_train
 from logger import Logger, ProductionLogger
@@ -70,6 +76,9 @@ def build_parser():
     # additive
     p.add_argument('--dtype', type=str, default='fp32', choices=['fp32', 'bf16'])
     p.add_argument('--synthetic', action='store_true')
+    llp_optim.add_flags(p)
+    p.add_argument('--eval_dtype', type=str, default='fp32', choices=['fp32', 'bf16', 'mxfp4'],
+                   help="what the student answers in when it is evaluated")
     return p
 
 
@@ -189,7 +198,7 @@ def main(argv=None):
         seed_everything(run + 1)
         model.reset_parameters()
         predictor.reset_parameters()
-        optimizer = torch.optim.Adam(list(model.parameters()) + list(predictor.parameters()), lr=args.lr)
+        optimizer = llp_optim.from_args(args, list(model.parameters()) + list(predictor.parameters()))
         cnt_wait = 0
         best_val = 0.0
         for epoch in range(1, 1 + args.epochs):
@@ -203,7 +212,7 @@ def main(argv=None):
                                        args, device)
                 results, h = llp_train.test_production(model, predictor, val_data, inference_data,
                                                        test_edge_bundle, negative_samples, None,
-                                                       args.link_batch_size, 'mlp', args.datasets)
+                                                       args.link_batch_size, 'mlp', args.datasets, args)
             if results[args.metric][0] >= best_val:
                 best_val = results[args.metric][0]
                 cnt_wait = 0

@@ -8,7 +8,8 @@ main.py (and the reference's main.py) read.
 Encoders: 'sage' (SAGEConv; SAGEConv_updated for coauthor-physics, :376-383)
 and 'gcn' (:384-387) on llp_teacher.TeacherEngine, 'mlp' on the full-batch
 engine.  Additive
-flags: --dtype {fp32,bf16}, --synthetic (see main.py).
+flags: --dtype {fp32,bf16}, --synthetic, --optimizer / --weight_decay /
+--optim_bits (see main.py).
 """
 import argparse
 import os
@@ -16,6 +17,7 @@ import os
 import torch
 
 import llp_datasets
+import llp_optim
 import llp_split
 import llp_train
 from llp_sage import SAGEConv, SAGEConv_updated
@@ -49,6 +51,7 @@ def build_parser():
     # additive
     p.add_argument('--dtype', type=str, default='fp32', choices=['fp32', 'bf16'])
     p.add_argument('--synthetic', action='store_true')
+    llp_optim.add_flags(p)
     return p
 
 
@@ -105,7 +108,7 @@ def main(argv=None):
         seed_everything(run)
         model.reset_parameters()
         predictor.reset_parameters()
-        optimizer = torch.optim.Adam(list(model.parameters()) + list(predictor.parameters()), lr=args.lr)
+        optimizer = llp_optim.from_args(args, list(model.parameters()) + list(predictor.parameters()))
         cnt_wait = 0
         best_val = 0.0
         for epoch in range(1, 1 + args.epochs):

@@ -1,0 +1,371 @@
+"""The low-bit operators where the framework uses them: AdamW (moments in 32 or 8 bits) in the training
+engines, MXFP4 in the evaluation, the commands' flags, and all of them in one run.
+
+The engines' update is compared with the formula in 64 bits on the gradient that the step left; its
+tolerances are those of tests/test_gpu_adamw.py (u = 2^-24; p' off by at most 3 u |p| + 24 u of the update's
+terms), the product's those of tests/test_gpu_mx4.py.
+"""
+import contextlib
+import copy
+import io
+import os
+import types
+
+import numpy as np
+import pytest
+import torch
+
+import golden_io as G
+from oracle import llp_oracle as O
+from oracle import lowbit_oracle as Q
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _lib():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    import llp_hip
+    llp_hip.lib()
+
+
+def _f64(t):
+    return t.detach().float().cpu().numpy().astype(np.float64)
+
+
+# ---------------------------------------------------------------- AdamW in the engines
+def _optimizer(kind, params):
+    import llp_optim
+    if kind == "torch":
+        return torch.optim.AdamW(params, lr=0.01, weight_decay=0.1)
+    return llp_optim.AdamW(params, lr=0.01, weight_decay=0.1, state_bits=8 if kind == "8bit" else 32, seed=0)
+
+
+def _moments(st):
+    if "exp_avg_scale" not in st:
+        return _f64(st["exp_avg"]).reshape(-1), _f64(st["exp_avg_sq"]).reshape(-1)
+    m, ms, v, vs = (st[k].cpu().numpy().reshape(-1) for k in ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale"))
+    return Q.values8(m, ms, True), Q.values8(v, vs, False) ** 2
+
+
+def _step_follows_the_formula(eng, opt, do_step):
+    """One step of the engine; returns the largest change of a parameter."""
+    params = eng.all_params
+    before = [(_f64(p).reshape(-1), *_moments(opt.state[p])) for p in params]
+    t = int(eng.adam_step) + 1
+    do_step()
+    torch.cuda.synchronize()
+    assert int(eng.adam_step) == t
+    g0 = opt.param_groups[0]
+    b1, b2 = g0["betas"]
+    sumsq, moved = _f64(eng.sumsq), 0.0
+    for p, grp, (p0, m0, v0) in zip(params, eng.param_groups_of, before):
+        g, ss = _f64(p.grad).reshape(-1), float(sumsq[grp])
+        rp, rm, rv = Q.adamw(p0, g, m0, v0, t, g0["lr"], (b1, b2), g0["eps"], g0["weight_decay"], ss)
+        terms = b1 * np.abs(m0) + (1 - b1) * min(1.0, 1.0 / (np.sqrt(ss) + 1e-6)) * np.abs(g)
+        upd = g0["lr"] / (1 - b1 ** t) * terms / (np.sqrt(rv) / np.sqrt(1 - b2 ** t) + g0["eps"])
+        assert (np.abs(_f64(p).reshape(-1) - rp) <= 3 * U * np.abs(p0) + 24 * U * upd).all()
+        m1, v1 = _moments(opt.state[p])
+        if "exp_avg_scale" in opt.state[p]:     # within one code of the exact value: steps of 32 (m), 16 (r) scales
+            s = np.exp2(np.repeat(_f64(opt.state[p]["exp_avg_scale"]) - 127, 32))[:m1.size]
+            assert (np.abs(m1 - rm) <= 32 * s * (1 + 1e-5)).all()
+            s = np.exp2(np.repeat(_f64(opt.state[p]["exp_avg_sq_scale"]) - 127, 32))[:m1.size]
+            assert (np.abs(np.sqrt(v1) - np.sqrt(rv)) <= 16 * s * (1 + 1e-5)).all()
+        else:
+            assert (np.abs(m1 - rm) <= 8 * U * terms).all() and (np.abs(v1 - rv) <= 13 * U * rv).all()
+        moved = max(moved, np.abs(rp - p0).max())
+        shadow, shadow_t, ld, ld_t = eng._shadows.get(id(p), (None, None, 0, 0))
+        if shadow is not None:
+            r, c = p.shape
+            assert torch.equal(shadow.as_strided((r, c), (ld or c, 1)), p.detach().to(shadow.dtype))
+        if shadow_t is not None:
+            r, c = p.shape
+            assert torch.equal(shadow_t.as_strided((c, r), (ld_t or r, 1)), p.detach().t().to(shadow_t.dtype))
+    return moved
+
+
+def _student(kind, dtype, N=600, F_=70, H=64):
+    import llp_engine
+    import models
+    args = types.SimpleNamespace(rw_step=3, hops=2, ns_rate=2, ps_method="nb", dropout=0.0, margin=0.05, LLP_D=1.0, LLP_R=1.0,
+                                 True_label=1.0, predictor="mlp", lr=0.01, minibatch=True)
+    torch.manual_seed(2)
+    model = models.MLP(3, F_, H, H, 0.0).to(DEV)
+    pred = models.LinkPredictor("mlp", H, H, 1, 3, 0.0).to(DEV)
+    tpred = models.LinkPredictor("mlp", 256, 256, 1, 2, 0.0).to(DEV)
+    for p in tpred.parameters():
+        p.requires_grad = False
+    g = torch.Generator().manual_seed(0)
+    pairs = torch.randint(0, N, (4000, 2), generator=g)
+    pairs = pairs[pairs[:, 0] != pairs[:, 1]]
+    ei = torch.stack([pairs, pairs.flip(1)], 1).reshape(-1, 2).t()
+    x, t_h = torch.randn(N, F_, generator=g) * 0.3, torch.randn(N, 256, generator=g) * 0.3
+    opt = _optimizer(kind, list(model.parameters()) + list(pred.parameters()))
+    eng = llp_engine.DistillEngine(model, pred, tpred, x.to(DEV), t_h.to(DEV), ei[0].numpy(), ei[1].numpy(), N, args, opt,
+                                   dtype=dtype, seed=5)
+    anchors = torch.randperm(N, generator=g)[:64].to(torch.int32).to(DEV)
+    links = torch.randperm(pairs.size(0), generator=g)[:512].to(torch.int32).to(DEV)
+    return eng, opt, model, pred, (anchors, links, pairs.to(torch.int32).to(DEV).contiguous())
+
+
+@pytest.mark.parametrize("kind", ["torch", "32bit", "8bit"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_student_step_with_adamw(kind, dtype):
+    """Eager steps, then a captured one replayed between eager work: each is the update of its own gradient."""
+    eng, opt, _, _, batch = _student(kind, dtype)
+    eng.begin_epoch()
+    for _ in range(2):
+        assert _step_follows_the_formula(eng, opt, lambda: eng.step_minibatch(*batch)) > 0
+    graph = eng.capture_minibatch(*batch)
+    for _ in range(3):
+        assert _step_follows_the_formula(eng, opt, graph.replay) > 0
+        eng.end_epoch(512)
+        eng.begin_epoch()
+    assert all(float(opt.state[p]["step"]) == 5 for p in eng.all_params)
+
+
+@pytest.mark.parametrize("kind", ["torch", "32bit", "8bit"])
+@pytest.mark.parametrize("name,dtype", [("teacher_sage_small", "fp32"), ("teacher_sage_small", "bf16"),
+                                        ("teacher_gcn_small", "bf16"), ("teacher_updated_production_small", "bf16")])
+def test_teacher_step_with_adamw(kind, name, dtype):
+    """The teacher's weights keep their copies in wider operands ([Wl | Wr], side by side and transposed)."""
+    import llp_sage
+    import llp_teacher
+    import models
+    c = G.load_teacher_case(name)
+    if c.encoder == "gcn":
+        model = models.GCN(c.F, c.H, c.H, c.L, 0.0).to(DEV)
+    else:
+        model = models.SAGE(c.dataset, c.F, c.H, c.H, c.L, 0.0, llp_sage.SAGEConv_updated if c.updated else llp_sage.SAGEConv,
+                            c.norm_type).to(DEV)
+    pred = models.LinkPredictor("mlp", c.H, c.H, 1, 2, 0.0).to(DEV)
+    opt = _optimizer(kind, list(model.parameters()) + list(pred.parameters()))
+    eng = llp_teacher.TeacherEngine(model, pred, c.x.to(DEV), c.edge_index, c.N, opt, dtype=dtype, seed=3)
+    pairs = c.pos_train_edge.to(torch.int32).to(DEV).contiguous()
+    eng.begin_epoch()
+    for st in c.steps[:3]:
+        link = st.link_perm.to(torch.int32).to(DEV)
+        neg = st.neg_edge.to(DEV)
+        assert _step_follows_the_formula(eng, opt, lambda: eng.step(link, pairs, neg=neg)) > 0
+
+
+def test_adamw_without_decay_is_the_adam_path():
+    """torch.optim.AdamW with no decay takes the same step as torch.optim.Adam, as before."""
+    runs = []
+    for cls in (torch.optim.Adam, torch.optim.AdamW):
+        eng, _, model, pred, batch = _student("torch", "bf16")
+        kw = {} if cls is torch.optim.Adam else {"weight_decay": 0.0}
+        eng.optimizer = cls(eng.all_params, lr=0.01, **kw)
+        eng._init_optimizer_state()
+        eng._build_descs()
+        assert eng.adamw is None
+        eng.begin_epoch()
+        eng.step_minibatch(*batch)
+        runs.append([p.detach().clone() for p in eng.all_params])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_engine_refuses_other_optimizers():
+    import llp_optim
+    eng, _, _, _, _ = _student("torch", "bf16")
+    ps = list(eng.all_params)
+    for opt in (torch.optim.SGD(ps, lr=0.1), torch.optim.Adam(ps, weight_decay=0.1), torch.optim.AdamW(ps, amsgrad=True),
+                torch.optim.AdamW(ps, maximize=True), torch.optim.AdamW([{"params": ps[:1]}, {"params": ps[1:]}]),
+                llp_optim.AdamW([{"params": ps[:1]}, {"params": ps[1:]}])):
+        eng.optimizer = opt
+        with pytest.raises(NotImplementedError):
+            eng._init_optimizer_state()
+    eng.optimizer = llp_optim.AdamW(ps[:-1])
+    with pytest.raises(ValueError, match="exactly"):
+        eng._init_optimizer_state()
+
+
+def test_engine_takes_over_a_stepped_optimizer():
+    """Eager llp_optim steps, then the engine, then eager again: one count of steps throughout."""
+    eng, opt, _, _, batch = _student("8bit", "fp32")
+    eng.begin_epoch()
+    eng.step_minibatch(*batch)
+    eng.end_epoch(512)
+    opt.step()
+    opt.step()
+    assert float(opt.state_dict()["state"][0]["step"]) == 3
+    opt.step()
+    eng._init_optimizer_state()
+    eng._build_descs()
+    assert int(eng.adam_step) == 4
+    _step_follows_the_formula(eng, opt, lambda: eng.step_minibatch(*batch))
+
+
+# ---------------------------------------------------------------- MXFP4 in the evaluation
+class _Spy:
+    """Records the operands and results of llp_mx.linear."""
+
+    def __init__(self, monkeypatch):
+        import llp_mx
+        self.calls, real = [], llp_mx.linear
+
+        def linear(x, w, bias=None, relu=False, out_dtype=None, out=None):
+            y = real(x, w, bias, relu, out_dtype, out)
+            keep = y if isinstance(y, llp_mx.MX4) else y.clone()
+            self.calls.append((x if isinstance(x, llp_mx.MX4) else x.clone(), w, bias, relu, keep))
+            return y
+        monkeypatch.setattr(llp_mx, "linear", linear)
+
+
+def _values(q):
+    return Q.mx4_values(q.codes.cpu().numpy(), q.scales.cpu().numpy(), q.cols)
+
+
+def _check_call(call, weight):
+    """A recorded product against the definition, from its own input's values; weight: the module's."""
+    import llp_mx
+    x, w, b, relu, y = call
+    assert np.array_equal(_values(w), Q.mx4_round(_f64(weight)))
+    xv = _values(x) if isinstance(x, llp_mx.MX4) else Q.mx4_round(_f64(x))
+    ref = xv @ _values(w).T + _f64(b)
+    size = np.abs(xv) @ np.abs(_values(w)).T + np.abs(_f64(b))
+    ref = np.maximum(ref, 0) if relu else ref
+    tol = (xv.shape[1] + 1) * 2.0 ** -23 * size
+    if isinstance(y, llp_mx.MX4):
+        # rounded to a code of the block: half a step of the exponent e - 2 of its largest value, which saturates
+        # at 6 (of less than 8): at most 2 scales
+        s = np.exp2(np.repeat(y.scales.cpu().numpy().astype(np.float64) - 127, 32, 1))[:, :ref.shape[1]]
+        assert (np.abs(_values(y) - ref) <= tol + 2 * s).all()
+    else:
+        assert (np.abs(_f64(y) - ref) <= tol + 2.0 ** -8 * (np.abs(ref) + tol)).all()
+
+
+@pytest.mark.parametrize("norm", ["none", "layer", "batch"])
+@pytest.mark.parametrize("N,F_,H,L", [(700, 96, 128, 3), (1, 33, 64, 2), (5000, 70, 96, 3), (40, 128, 64, 1)])
+def test_embed_mlp_mxfp4(monkeypatch, norm, N, F_, H, L):
+    import llp_eval as E
+    import models
+    torch.manual_seed(0)
+    mlp = models.MLP(L, F_, H, H, 0.3, norm).to(DEV).eval()
+    for m in getattr(mlp, "norms", []):      # other than the identity
+        with torch.no_grad():
+            m.weight.uniform_(0.5, 1.5)
+            m.bias.uniform_(-0.5, 0.5)
+            if norm == "batch":
+                m.running_mean.uniform_(-0.1, 0.1)
+                m.running_var.uniform_(0.5, 1.5)
+    x = torch.randn(N, F_, device=DEV)
+    spy = _Spy(monkeypatch)
+    h = E.embed_mlp(mlp, x, "mxfp4")
+    assert h.dtype == torch.bfloat16 and h.shape == (N, H) and len(spy.calls) == L
+    assert torch.equal(spy.calls[0][0], x) and torch.equal(spy.calls[-1][4], h)
+    for l, call in enumerate(spy.calls):
+        _check_call(call, mlp.layers[l].weight)
+        if l and norm == "none":
+            assert call[0] is spy.calls[l - 1][4]
+        elif l:        # the norm of the bf16 result, in 64 bits; its statistics and products in f32, the result in bf16
+            m, z = mlp.norms[l - 1], spy.calls[l - 1][4].double()
+            with torch.no_grad():
+                want = torch.relu(copy.deepcopy(m).double()(z))
+            assert ((call[0].double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-4 * (1 + want.abs())).all()
+
+
+@pytest.mark.parametrize("hd", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("L,H,E_,chunk", [(2, 64, 5000, 1536), (3, 128, 5000, 1536), (3, 96, 1, 1536), (2, 256, 40000, 1 << 18)])
+def test_scorer_mxfp4(monkeypatch, hd, L, H, E_, chunk):
+    """Pair products, hidden layers and the head; scores of f32 embeddings are those of their bf16 values."""
+    import llp_eval as E
+    import models
+    torch.manual_seed(1)
+    N = 900
+    pred = models.LinkPredictor("mlp", H, H, 1, L, 0.3).to(DEV).eval()
+    h = torch.randn(N, H, device=DEV).to(hd)
+    edges = torch.randint(0, N, (E_, 2))
+    spy = _Spy(monkeypatch)
+    s = E.EdgeScorer(pred, dtype="mxfp4", chunk=chunk)(h, edges.to(DEV))
+    assert s.shape == (E_,) and s.dtype == torch.float32
+    hv, per = _f64(h.to(torch.bfloat16)), L - 1
+    w2, b2 = _f64(pred.lins[-1].weight).reshape(-1), float(pred.lins[-1].bias)
+    for k, lo in enumerate(range(0, E_, chunk)):
+        e = edges[lo:lo + chunk].numpy()
+        for l in range(per):
+            call = spy.calls[k * per + l]
+            _check_call(call, pred.lins[l].weight)
+            if l == 0:        # a product of two bf16 numbers is exact in f32
+                assert np.array_equal(_values(call[0]), Q.mx4_round(hv[e[:, 0]] * hv[e[:, 1]]))
+            else:
+                assert call[0] is spy.calls[k * per + l - 1][4]
+        z = _f64(spy.calls[k * per + per - 1][4])
+        logit, size = z @ w2 + b2, np.abs(z) @ np.abs(w2) + abs(b2)
+        # f32 sums, then a sigmoid of slope 1/4 in f32 (off by a few u)
+        assert (np.abs(_f64(s[lo:lo + chunk]) - 1 / (1 + np.exp(-logit))) <= (H + 2) * U * size / 4 + 16 * U).all()
+
+
+def test_scorer_mxfp4_inner_and_empty():
+    import llp_eval as E
+    import models
+    h = torch.randn(50, 64, device=DEV)
+    edges = torch.randint(0, 50, (300, 2), device=DEV)
+    pred = models.LinkPredictor("inner", 64, 64, 1, 2, 0.0).to(DEV).eval()
+    # the inner product has no layer: it is the bf16 path's
+    assert torch.equal(E.EdgeScorer(pred, dtype="mxfp4")(h, edges), E.EdgeScorer(pred, dtype=torch.bfloat16)(h, edges))
+    pred = models.LinkPredictor("mlp", 64, 64, 1, 2, 0.0).to(DEV).eval()
+    assert E.EdgeScorer(pred, dtype="mxfp4")(h, edges[:0]).shape == (0,)
+
+
+# ---------------------------------------------------------------- together
+def test_distil_with_8bit_adamw_then_answer_in_mxfp4():
+    """A student trained with 8-bit moments, saved, loaded and evaluated in MXFP4 through the training API:
+    the Hits@K are those of the MXFP4 scores."""
+    import llp_eval as E
+    import llp_optim
+    import llp_train
+    eng, opt, model, pred, batch = _student("8bit", "bf16", N=600, F_=70, H=64)
+    eng.begin_epoch()
+    for _ in range(4):
+        eng.step_minibatch(*batch)
+    assert np.isfinite(eng.end_epoch(4 * 512))
+    again = llp_optim.AdamW(list(model.parameters()) + list(pred.parameters()), lr=0.01, state_bits=8)
+    again.load_state_dict(opt.state_dict())
+    assert float(again.state_dict()["state"][0]["step"]) == 4
+    x = torch.randn(600, 70)
+    g = torch.Generator().manual_seed(8)
+    split = {s: {"edge": torch.randint(0, 600, (300, 2), generator=g), "edge_neg": torch.randint(0, 600, (900, 2), generator=g)}
+             for s in ("valid", "test")}
+    args = types.SimpleNamespace(eval_dtype="mxfp4", dataset="cora")
+    data = types.SimpleNamespace(x=x)
+    res, h = llp_train.test_transductive(model, pred, data, split, None, 1024, "mlp", "cora", args)
+    assert h.dtype == torch.bfloat16
+    model.eval(), pred.eval()
+    want = E.embed_mlp(model, x.to(DEV), "mxfp4")
+    assert torch.equal(h, want)
+    sc = E.EdgeScorer(pred, dtype="mxfp4")
+    for i, s in enumerate(("valid", "test")):
+        p, n = (sc(want, split[s][k].to(DEV)).cpu() for k in ("edge", "edge_neg"))
+        for k in (10, 20, 30, 50):
+            assert res[f"Hits@{k}"][i] == O.hits_at_k(p, n, k)
+    # and near the full-precision answer's ranking: nothing is claimed but that scores are probabilities
+    assert ((p > 0) & (p < 1)).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("setting", ["transductive", "production"])
+def test_commands_with_the_flags(tmp_path, bits, setting):
+    import main as student_cli
+    import train_teacher_gnn as teacher_cli
+    w = tmp_path / "src"
+    w.mkdir()
+    old = os.getcwd()
+    os.chdir(w)
+    try:
+        def run(mod, argv):
+            buf = io.StringIO()
+            with contextlib.redirect_stdout(buf):
+                mod.main(["--datasets=cora", "--encoder=sage", "--runs=1", "--epochs=1", "--synthetic", "--optimizer=adamw",
+                          f"--optim_bits={bits}", "--weight_decay=0.02", f"--transductive={setting}"] + argv)
+            return buf.getvalue()
+        assert "Run: 01, Epoch: 01" in run(teacher_cli, [])
+        out = run(student_cli, ["--LLP_D=1", "--LLP_R=1", "--True_label=1", "--dropout=0.5", "--hops=2", "--rw_step=2",
+                                "--ns_rate=1", "--eval_dtype=mxfp4"])
+        assert len([l for l in out.splitlines() if l.startswith("Run: 01, Epoch: 01")]) == 5, out
+    finally:
+        os.chdir(old)

@@ -180,3 +180,55 @@ def test_oracle_round_trips():
     d = Q.draws16(20, 3, 5, 99)
     from oracle import llp_oracle as O
     assert d[9] == (int(O.philox_u32(99, 65536 * 5 + 3, np.array([4]))[0]) >> 16) & 0xFFFF
+
+
+def test_adamw_copies_are_bounded():
+    """A copy has the param's size, or rows that stay within its storage."""
+    fits = llp_optim.AdamWTable._fits
+    t = torch.zeros(6, 20)
+    fits((None, 0), 3, 4, 0)
+    fits((t, 0), 6, 20, 0)
+    fits((t, 20), 6, 10, 0)
+    fits((t[:, 10:], 20), 6, 10, 0)
+    fits((t[5:], 20), 1, 20, 0)
+    for copy, r, c in (((t, 0), 6, 19), ((t, 20), 7, 20), ((t[:, 11:], 20), 6, 10), ((t, 8), 6, 10), ((t[1:], 20), 6, 20)):
+        with pytest.raises(ValueError):
+            fits(copy, r, c, 0)
+    p, g, m, v = [[torch.zeros(6, 20)] for _ in range(4)]
+    with pytest.raises(ValueError, match="copy"):
+        llp_optim.AdamWTable(p, g, m, v, copies=[torch.zeros(6, 19)])
+    with pytest.raises(ValueError, match="copy"):
+        llp_optim.AdamWTable(p, g, m, v, copies_t=[(torch.zeros(20, 5), 6)])
+
+
+def test_mx4_on_the_cpu_is_refused():
+    q = llp_mx.MX4(_u8(3, 64), _u8(3, 4), 100)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        llp_mx.dequantize(q)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        llp_mx.linear(q, q)
+
+
+def test_commands_optimizer_flags():
+    import main
+    import train_teacher_gnn
+    for mod in (main, train_teacher_gnn):
+        a = mod.build_parser().parse_args([])
+        assert (a.optimizer, a.weight_decay, a.optim_bits) == ("adam", 0.01, 32)
+        p = [torch.nn.Parameter(torch.zeros(3))]
+        assert type(llp_optim.from_args(a, p)) is torch.optim.Adam
+        a = mod.build_parser().parse_args(["--optimizer=adamw", "--optim_bits=8", "--weight_decay=0.5", "--lr=0.25"])
+        opt = llp_optim.from_args(a, p)
+        assert isinstance(opt, llp_optim.AdamW) and opt.state_bits == 8
+        assert (opt.param_groups[0]["lr"], opt.param_groups[0]["weight_decay"]) == (0.25, 0.5)
+        with pytest.raises(ValueError, match="adamw"):
+            llp_optim.from_args(mod.build_parser().parse_args(["--optim_bits=8"]), p)
+    assert main.build_parser().parse_args([]).eval_dtype == "fp32"
+
+
+def test_adamw_optimizer_copies():
+    """copy.deepcopy (as pickling) keeps the settings and starts with no device tables."""
+    import copy
+    opt = llp_optim.AdamW([torch.nn.Parameter(torch.zeros(4))], lr=0.5, state_bits=8, seed=9)
+    got = copy.deepcopy(opt)
+    assert (got.state_bits, got.seed, got.param_groups[0]["lr"], got._tables) == (8, 9, 0.5, {})
