@@ -15,8 +15,12 @@
 // a code is 3 to 6 % wide, and v would never move down.
 // The update of p uses m' and v' before they are rounded.
 //
-// Bound by memory: per element 8 B of p, 4 (2) of g, and 16 B of f32 moments or 4.1 B of 8-bit ones.
+// Bound by memory: per element 8 B of p, 4 (2) of g, and 16 B of f32 moments or 4.1 B of 8-bit ones.  36 M f32
+// elements with a bf16 copy: 200 us at 5.1 TB/s with f32 moments, 1e8 with 8-bit ones 342 us at 5.3 TB/s (a large copy
+// reaches 4.8); 500,000 elements 5.0 and 5.6 us, where the launch is what counts.
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "llp_common.h"
 
@@ -32,12 +36,22 @@ typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u4_any2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u2_any1 __attribute__((ext_vector_type(2), aligned(1)));
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int64_t e, int n, float (&x)[8]);
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, int64_t e, int n, float (&x)[8]) {
+// ONCE: nontemporal, past the caches
+template <bool ONCE, typename V>
+__device__ __forceinline__ V load_as(const void* p) {
+  if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+  else return *reinterpret_cast<const V*>(p);
+}
+template <bool ONCE, typename V>
+__device__ __forceinline__ void store_as(void* p, V v) {
+  if constexpr (ONCE) __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
+  else *reinterpret_cast<V*>(p) = v;
+}
+
+template <bool ONCE>
+__device__ __forceinline__ void load8(const float* p, int64_t e, int n, float (&x)[8]) {
   if (n == 8) {
-    const f4_any a = *reinterpret_cast<const f4_any*>(p + e), b = *reinterpret_cast<const f4_any*>(p + e + 4);
+    const f4_any a = load_as<ONCE, f4_any>(p + e), b = load_as<ONCE, f4_any>(p + e + 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
   } else {
@@ -45,10 +59,10 @@ __device__ __forceinline__ void load8<float>(const float* p, int64_t e, int n, f
     for (int i = 0; i < 8; ++i) x[i] = i < n ? p[e + i] : 0.f;
   }
 }
-template <>
-__device__ __forceinline__ void load8<bf16_t>(const bf16_t* p, int64_t e, int n, float (&x)[8]) {
+template <bool ONCE>
+__device__ __forceinline__ void load8(const bf16_t* p, int64_t e, int n, float (&x)[8]) {
   if (n == 8) {
-    const u4_any2 a = *reinterpret_cast<const u4_any2*>(p + e);
+    const u4_any2 a = load_as<ONCE, u4_any2>(p + e);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       x[2 * i] = __uint_as_float(a[i] << 16);
@@ -60,26 +74,24 @@ __device__ __forceinline__ void load8<bf16_t>(const bf16_t* p, int64_t e, int n,
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void store8(T* p, int64_t e, int n, const float (&x)[8]);
-template <>
-__device__ __forceinline__ void store8<float>(float* p, int64_t e, int n, const float (&x)[8]) {
+template <bool ONCE>
+__device__ __forceinline__ void store8(float* p, int64_t e, int n, const float (&x)[8]) {
   if (n == 8) {
-    *reinterpret_cast<f4_any*>(p + e) = f4_any{x[0], x[1], x[2], x[3]};
-    *reinterpret_cast<f4_any*>(p + e + 4) = f4_any{x[4], x[5], x[6], x[7]};
+    store_as<ONCE>(p + e, f4_any{x[0], x[1], x[2], x[3]});
+    store_as<ONCE>(p + e + 4, f4_any{x[4], x[5], x[6], x[7]});
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (i < n) p[e + i] = x[i];
   }
 }
-template <>
-__device__ __forceinline__ void store8<bf16_t>(bf16_t* p, int64_t e, int n, const float (&x)[8]) {
+template <bool ONCE>
+__device__ __forceinline__ void store8(bf16_t* p, int64_t e, int n, const float (&x)[8]) {
   if (n == 8) {
     u4_any2 a;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = (uint32_t)f2bf(x[2 * i]) | ((uint32_t)f2bf(x[2 * i + 1]) << 16);
-    *reinterpret_cast<u4_any2*>(p + e) = a;
+    for (int i = 0; i < 4; ++i) a[i] = bf16_pair(x[2 * i], x[2 * i + 1]);
+    store_as<ONCE>(p + e, a);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -98,9 +110,10 @@ __device__ __forceinline__ void load_codes(const uint8_t* p, int64_t e, int n, u
       if (i < n) w[i >> 2] |= (uint32_t)p[e + i] << (8 * (i & 3));
   }
 }
+template <bool ONCE>
 __device__ __forceinline__ void store_codes(uint8_t* p, int64_t e, int n, const uint32_t (&w)[2]) {
   if (n == 8) {
-    *reinterpret_cast<u2_any1*>(p + e) = u2_any1{w[0], w[1]};
+    store_as<ONCE>(p + e, u2_any1{w[0], w[1]});
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -175,10 +188,11 @@ __device__ __forceinline__ uint32_t round_r(float y, float x, uint32_t w) {
 }
 
 // the working copy, rows copy_ld apart (0: as the parameter)
+template <bool ONCE>
 __device__ __forceinline__ void store_copy(const llp_adamw_desc& d, int64_t e, int n, const float (&p)[8]) {
   if (d.copy_ld == 0 || d.copy_ld == d.cols) {
-    if (d.copy_dtype == LLP_BF16) store8((bf16_t*)d.copy, e, n, p);
-    else store8((float*)d.copy, e, n, p);
+    if (d.copy_dtype == LLP_BF16) store8<ONCE>((bf16_t*)d.copy, e, n, p);
+    else store8<ONCE>((float*)d.copy, e, n, p);
     return;
   }
 #pragma unroll
@@ -207,7 +221,7 @@ struct AdamWArgs {
   uint64_t seed;
 };
 
-template <int BITS, typename P, typename G>
+template <int BITS, bool ONCE, typename P, typename G>
 __global__ __launch_bounds__(256) void adamw_kernel(const llp_adamw_desc* __restrict__ descs,
                                                     const int32_t* __restrict__ work, int64_t n_work,
                                                     const float* __restrict__ sumsq, AdamWArgs a,
@@ -228,11 +242,11 @@ __global__ __launch_bounds__(256) void adamw_kernel(const llp_adamw_desc* __rest
       coef = (q != q) ? q : fminf(q, 1.f);
     }
     float g[8], p[8], m[8], v[8], r[8];
-    load8((const G*)d.grad, e, n, g);
-    load8((const P*)d.param, e, n, p);
+    load8<ONCE>((const G*)d.grad, e, n, g);
+    load8<ONCE>((const P*)d.param, e, n, p);
     if constexpr (BITS == 32) {
-      load8((const float*)d.exp_avg, e, n, m);
-      load8((const float*)d.exp_avg_sq, e, n, v);
+      load8<false>((const float*)d.exp_avg, e, n, m);
+      load8<false>((const float*)d.exp_avg_sq, e, n, v);
     } else {
       uint32_t cm[2], cr[2];
       load_codes((const uint8_t*)d.exp_avg, e, n, cm);
@@ -253,11 +267,11 @@ __global__ __launch_bounds__(256) void adamw_kernel(const llp_adamw_desc* __rest
       r[i] = sqrtf(v[i]);
       p[i] = p[i] * keep - size * (m[i] / (r[i] * inv_bc2 + eps));
     }
-    store8((P*)d.param_out, e, n, p);
-    if (d.copy) store_copy(d, e, n, p);
+    store8<ONCE>((P*)d.param_out, e, n, p);
+    if (d.copy) store_copy<ONCE>(d, e, n, p);
     if constexpr (BITS == 32) {
-      store8((float*)d.exp_avg_out, e, n, m);
-      store8((float*)d.exp_avg_sq_out, e, n, v);
+      store8<false>((float*)d.exp_avg_out, e, n, m);
+      store8<false>((float*)d.exp_avg_sq_out, e, n, v);
     } else {
       uint32_t tm = 0, tr = 0;
 #pragma unroll
@@ -280,8 +294,8 @@ __global__ __launch_bounds__(256) void adamw_kernel(const llp_adamw_desc* __rest
       }
       if (sm == 255u) cm[0] = cm[1] = 0;
       if (sr == 255u) cr[0] = cr[1] = 0;
-      store_codes((uint8_t*)d.exp_avg_out, e, n, cm);
-      store_codes((uint8_t*)d.exp_avg_sq_out, e, n, cr);
+      store_codes<ONCE>((uint8_t*)d.exp_avg_out, e, n, cm);
+      store_codes<ONCE>((uint8_t*)d.exp_avg_sq_out, e, n, cr);
       if (n && (threadIdx.x & 3) == 0) {
         d.exp_avg_scale_out[e >> 5] = (uint8_t)sm;
         d.exp_avg_sq_scale_out[e >> 5] = (uint8_t)sr;
@@ -307,8 +321,8 @@ __global__ __launch_bounds__(256) void adamw_values_kernel(const llp_adamw_desc*
     decode_r(cr, d.exp_avg_sq_scale_out[e >> 5], r);
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] *= r[i];
-    if (d.exp_avg_value) store8((T*)d.exp_avg_value, e, n, m);
-    if (d.exp_avg_sq_value) store8((T*)d.exp_avg_sq_value, e, n, r);
+    if (d.exp_avg_value) store8<true>((T*)d.exp_avg_value, e, n, m);
+    if (d.exp_avg_sq_value) store8<true>((T*)d.exp_avg_sq_value, e, n, r);
   }
 }
 
@@ -324,7 +338,8 @@ __global__ __launch_bounds__(256) void adamw_copy_t_kernel(const llp_adamw_desc*
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
   const P* p = (const P*)d.param_out;
 #pragma unroll
-  for (int i = ty; i < 64; i += 4) {
+  for (int j = 0; j < 16; ++j) {
+    const int i = ty + 4 * j;
     const int64_t r = r0 + i, c = c0 + tx;
     if (r < d.rows && c < d.cols) {
       if constexpr (sizeof(P) == 4) tile[i][tx] = p[r * d.cols + c];
@@ -333,7 +348,8 @@ __global__ __launch_bounds__(256) void adamw_copy_t_kernel(const llp_adamw_desc*
   }
   __syncthreads();
 #pragma unroll
-  for (int i = ty; i < 64; i += 4) {
+  for (int j = 0; j < 16; ++j) {
+    const int i = ty + 4 * j;
     const int64_t c = c0 + i, r = r0 + tx;
     if (c < d.cols && r < d.rows) {
       if (d.copy_dtype == LLP_BF16) ((bf16_t*)d.copy_t)[c * ldt + r] = f2bf(tile[tx][i]);
@@ -367,13 +383,19 @@ extern "C" int llp_adamw_step(const llp_adamw_desc* descs, int n_tensors, const 
     hipLaunchKernelGGL(kernel, dim3(aw_grid(n_work)), dim3(256), 0, (hipStream_t)stream, descs, work, n_work, sumsq, a,
                        step);
   };
-  if (state_bits == 32) {
-    if (param_dtype == LLP_F32) grad_dtype == LLP_F32 ? go(adamw_kernel<32, float, float>) : go(adamw_kernel<32, float, bf16_t>);
-    else grad_dtype == LLP_F32 ? go(adamw_kernel<32, bf16_t, float>) : go(adamw_kernel<32, bf16_t, bf16_t>);
-  } else {
-    if (param_dtype == LLP_F32) grad_dtype == LLP_F32 ? go(adamw_kernel<8, float, float>) : go(adamw_kernel<8, float, bf16_t>);
-    else grad_dtype == LLP_F32 ? go(adamw_kernel<8, bf16_t, float>) : go(adamw_kernel<8, bf16_t, bf16_t>);
-  }
+  auto types = [&](auto bits, auto once) {
+    constexpr int B = bits;
+    constexpr bool O = once;
+    if (param_dtype == LLP_F32) grad_dtype == LLP_F32 ? go(adamw_kernel<B, O, float, float>) : go(adamw_kernel<B, O, float, bf16_t>);
+    else grad_dtype == LLP_F32 ? go(adamw_kernel<B, O, bf16_t, float>) : go(adamw_kernel<B, O, bf16_t, bf16_t>);
+  };
+  constexpr std::integral_constant<int, 32> b32{};
+  constexpr std::integral_constant<int, 8> b8{};
+  // 8-bit steps of more than 32 M elements (580 MB, twice the last-level cache) pass by the caches: 4e7 elements 148 -> 138 us,
+  // 1e8 367 -> 342; 2e7 would go from 64 to 69.  With f32 moments it only costs (1e8 / 2.8: 200 -> 210).
+  if (state_bits == 32) types(b32, std::false_type{});
+  else if (n_work >= 16384) types(b8, std::true_type{});
+  else types(b8, std::false_type{});
   LLP_LAUNCH_CHECK();
   return LLP_OK;
 }

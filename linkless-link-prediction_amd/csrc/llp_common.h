@@ -53,6 +53,13 @@ __device__ __forceinline__ bf16_t f2bf(float f) {
   return *reinterpret_cast<bf16_t*>(&h);
 }
 
+// two values to bf16 in one instruction, a in the low half
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
+}
+
 // Philox streams per training step: a draw of step s at offset o uses stream
 // LLP_STREAMS_PER_STEP * s + o (walks 0 .. rw_step-1, context negatives rw_step, PyG-dense
 // negatives STREAMS-2 under their own key, randint negatives STREAMS-1; dropout layers 1 + l

@@ -384,3 +384,52 @@ def test_optimizer_uses_the_current_stream():
         opt.step()
     torch.cuda.current_stream().wait_stream(side)
     assert torch.allclose(p, torch.full_like(p, 0.5), atol=1e-5)
+
+
+def test_adamw_8bit_large_tensor():
+    """Past 32 M elements the step streams; p, the codes and what lies around a slice of the tensor."""
+    o = _opt()
+    n = (1 << 25) + 45
+    gen = torch.Generator(device=DEV).manual_seed(12)
+    p = torch.randn(n, device=DEV, generator=gen)
+    g = 1e-3 * torch.randn(n, device=DEV, generator=gen)
+    (m, ms), (v, vs) = o.AdamWTable.state8(n, DEV), o.AdamWTable.state8(n, DEV)
+    tab = o.AdamWTable([p], [g], [m], [v], exp_avg_scale=[ms], exp_avg_sq_scale=[vs])
+    ctr = torch.zeros(1, dtype=torch.int64, device=DEV)
+    at = [slice(0, 4096), slice(n // 64 * 32, n // 64 * 32 + 4096), slice((n - 4096) // 32 * 32, n)]
+    for t in range(2):
+        ctr.fill_(t)
+        before = [(_f64(p[s]), m[s].cpu().numpy(), ms[s.start // 32:-(-s.stop // 32)].cpu().numpy(), v[s].cpu().numpy(),
+                   vs[s.start // 32:-(-s.stop // 32)].cpu().numpy()) for s in at]
+        tab.step(ctr, seed=5, **HYPER)
+        for s, (p0, m0, ms0, v0, vs0) in zip(at, before):
+            m0, r0, g0 = Q.values8(m0, ms0, True), Q.values8(v0, vs0, False), _f64(g[s])
+            rp, rm, rv = Q.adamw(p0, g0, m0, r0 * r0, t + 1, HYPER["lr"], HYPER["betas"], HYPER["eps"], HYPER["weight_decay"])
+            terms = 0.9 * np.abs(m0) + 0.1 * np.abs(g0)
+            upd = HYPER["lr"] / (1 - 0.9 ** (t + 1)) * terms / (np.sqrt(rv) / np.sqrt(1 - 0.999 ** (t + 1)) + 1e-8)
+            assert (np.abs(_f64(p[s]) - rp) <= 3 * U * np.abs(p0) + 24 * U * upd).all()
+            for x, codes, scales, signed in ((rm, m, ms, True), (np.sqrt(rv), v, vs, False)):
+                b = scales[s.start // 32:-(-s.stop // 32)].cpu().numpy()
+                got = Q.values8(codes[s].cpu().numpy(), b, signed)
+                f = np.repeat(np.exp2(b.astype(np.float64) - 127), 32)[:got.size]
+                # within one code of the value: the codes' largest step is 32 (16) scales
+                assert (np.abs(got - x) <= (32 if signed else 16) * f * (1 + 1e-5)).all()
+
+
+def test_adamw_step_as_the_tables_grow():
+    """The same tensor in a table of its own and as the first of a table of 40 M elements: the same result."""
+    o = _opt()
+    n, gen = 5000, torch.Generator().manual_seed(3)
+    p0, g0 = torch.randn(n, generator=gen), torch.randn(n, generator=gen) * 1e-2
+    got = []
+    for more in (0, 40_000_000):
+        ps, gs = [p0.to(DEV)], [g0.to(DEV)]
+        if more:
+            ps.append(torch.zeros(more, device=DEV)), gs.append(torch.ones(more, device=DEV))
+        st = [o.AdamWTable.state8(t.numel(), DEV) for t in ps for _ in (0, 1)]
+        tab = o.AdamWTable(ps, gs, [s[0] for s in st[::2]], [s[0] for s in st[1::2]], [s[1] for s in st[::2]],
+                           [s[1] for s in st[1::2]])
+        for t in range(3):
+            tab.step(torch.full((1,), t, dtype=torch.int64, device=DEV), seed=9, **HYPER)
+        got.append([ps[0], *st[0], *st[1]])
+    assert all(torch.equal(a, b) for a, b in zip(*got))

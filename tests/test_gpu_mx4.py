@@ -298,3 +298,48 @@ def test_two_streams_at_once():
                 got[k] = m.linear(xs[k], w)
         torch.cuda.synchronize()
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("K,N", [(128, 1024), (512, 1040), (300, 1024)])
+def test_linear_large_result(K, N):
+    """A bf16 result of 2^27 values and more is stored past the caches: the f32 result, rounded."""
+    m = mx()
+    g = torch.Generator(device=DEV).manual_seed(K)
+    M = (1 << 17) + 37
+    q = m.quantize(torch.randn(M, K, generator=g, device=DEV))
+    w, b = m.quantize(torch.randn(N, K, generator=g, device=DEV)), torch.randn(N, generator=g, device=DEV)
+    y = m.linear(q, w, b, relu=True, out_dtype=torch.float32)
+    assert torch.equal(m.linear(q, w, b, relu=True), y.bfloat16())
+    rows = torch.tensor([0, 1, M // 2, M - 38, M - 1], device=DEV)
+    part = m.MX4(q.codes[rows], q.scales[rows], K)
+    xv, wv = _f64(m.dequantize(part)), _f64(m.dequantize(w))
+    ref, size = np.maximum(xv @ wv.T + _f64(b), 0), np.abs(xv) @ np.abs(wv).T + np.abs(_f64(b))
+    assert (np.abs(_f64(y[rows]) - ref) <= (K + 1) * 2.0 ** -23 * size).all()
+
+
+def test_offsets_past_32_bits():
+    """Rows whose bytes, elements and results lie past 2^31 and 2^32; conversions in more than one launch."""
+    m = mx()
+    K, M = 1024, (1 << 24) + 5
+    g = torch.Generator(device=DEV).manual_seed(0)
+    h = torch.randn(1000, K, generator=g, device=DEV).bfloat16()
+    idx = torch.randint(0, 1000, (M,), generator=g, device=DEV, dtype=torch.int32)
+    q = m.quantize(h, idx)
+    x = m.dequantize(q, torch.bfloat16)
+    hq = m.dequantize(m.quantize(h), torch.bfloat16)
+    at = [0, 1 << 21, (1 << 22) - 1, 1 << 22, (1 << 23) + 7, (1 << 24) - 2, (1 << 24) - 1, 1 << 24, M - 1]
+    for i in at:
+        assert torch.equal(x[i], hq[idx[i].long()]), i
+    lo = 0
+    while lo < M:        # and every row, in pieces
+        n = min(1 << 21, M - lo)
+        assert torch.equal(x[lo:lo + n], hq[idx[lo:lo + n].long()]), lo
+        lo += n
+    del x
+    w = m.quantize(torch.randn(264, K, generator=g, device=DEV))
+    hy = m.linear(m.quantize(h), w, out_dtype=torch.float32)
+    y = m.linear(q, w)            # 16.8 M x 264 in bf16: 8.9 GB, of codes of 8.6 GB
+    size = (hq.float().abs() @ m.dequantize(w).abs().T)
+    for i in at:                  # another kernel's sums: the order differs
+        r = int(idx[i])
+        assert ((y[i].float() - hy[r]).abs() <= 2 * K * 2.0 ** -23 * size[r] + 2.0 ** -8 * (hy[r].abs() + K * 2.0 ** -23 * size[r])).all(), i
