@@ -52,7 +52,9 @@ class MX4:
             raise ValueError("MX4: codes and scales of the same rows, on the same device")
         self.rows, self.cols, self.device = codes.shape[0], int(cols), codes.device
         self._codes, self._scales, self._both = codes, scales, None
-        self.c = K.Mx4(codes.data_ptr(), scales.data_ptr(), codes.stride(0), scales.stride(0))
+        p, one = _pad(self.cols), self.rows <= 1       # (the stride of a single row says nothing)
+        self.c = K.Mx4(codes.data_ptr(), scales.data_ptr(), p // 2 if one else codes.stride(0),
+                       p // 32 if one else scales.stride(0))
 
     @staticmethod
     def empty(rows, cols, device):
@@ -82,6 +84,36 @@ class MX4:
     @property
     def shape(self):
         return (self.rows, self.cols)
+
+
+def _row_stride(out, what):
+    """The row stride of a given 2-D output, whose rows must not share memory."""
+    rows, cols = out.shape
+    if rows > 1 and out.stride(0) < cols:
+        raise ValueError(f"{what}: the rows of out overlap")
+    return out.stride(0) if rows > 1 else cols
+
+
+def _spans(t):
+    """Where the rows of a matrix lie: [(first byte, byte past the last)]."""
+    rows, cols = t.shape
+    if not rows:
+        return []
+    if isinstance(t, MX4):
+        p = _pad(cols)
+        return [(t.c.codes, t.c.codes + (rows - 1) * t.c.ld_codes + p // 2),
+                (t.c.scales, t.c.scales + (rows - 1) * t.c.ld_scales + p // 32)]
+    at, size = t.data_ptr(), t.element_size()
+    return [(at, at + ((rows - 1) * t.stride(0) + cols) * size)]
+
+
+def _apart(what, out, *inputs):
+    """A given output shares no memory with what the call reads."""
+    mine = _spans(out)
+    for t in inputs:
+        for a, b in _spans(t):
+            if any(a < hi and lo < b for lo, hi in mine):
+                raise ValueError(f"{what}: out overlaps an input")
 
 
 def _on_gpu(dev):
@@ -134,6 +166,8 @@ def quantize(x, idx=None, x2=None, idx2=None, out=None):
         out = MX4.empty(rows, x.shape[1], x.device)
     elif out.shape != (rows, x.shape[1]) or out.device != x.device:
         raise ValueError(f"quantize: out is {out.shape} on {out.device}, the rows are {(rows, x.shape[1])} on {x.device}")
+    else:
+        _apart("quantize", out, x, *([] if x2 is None else [x2]))
     K.launch("llp_mx4_quantize", x.device, K.dtype_code(x.dtype), rows, x.shape[1], C.byref(op), C.byref(out.c))
     return out
 
@@ -145,8 +179,10 @@ def dequantize(q, dtype=torch.float32, out=None):
         out = torch.empty(q.rows, q.cols, dtype=dtype, device=q.device)
     elif tuple(out.shape) != q.shape or out.device != q.device or (q.cols > 1 and out.stride(1) != 1):
         raise ValueError("dequantize: out needs q's shape, on its device, with contiguous rows")
+    else:
+        _apart("dequantize", out, q)
     K.launch("llp_mx4_dequantize", q.device, q.rows, q.cols, C.byref(q.c), K.dtype_code(out.dtype), out.data_ptr(),
-             max(out.stride(0), q.cols))
+             _row_stride(out, "dequantize"))
     return out
 
 
@@ -179,6 +215,8 @@ def linear(x, w, bias=None, relu=False, out_dtype=None, out=None):
         out = MX4.empty(rows, N, dev) if out_dtype == "mx4" else torch.empty((rows, N), dtype=out_dtype, device=dev)
     elif tuple(out.shape) != (rows, N) or out.device != dev or lead is not None:
         raise ValueError(f"linear: out is {tuple(out.shape)} on {out.device}, the result is {(rows, N)} on {dev}")
+    else:
+        _apart("linear", out, x, w, *([] if bias is None else [bias.view(1, N)]))
     four_out = isinstance(out, MX4)
     if not four_out and (out.dtype not in _FLOATS or (N > 1 and out.stride(1) != 1)):
         raise TypeError("linear: out in f32 or bf16 with contiguous rows")
@@ -195,5 +233,5 @@ def linear(x, w, bias=None, relu=False, out_dtype=None, out=None):
                  C.byref(out.c), b, act)
         return out
     K.launch("llp_gemm_nt_mx4", dev, rows, N, width, code, op, c4, C.byref(w.c),
-             out.data_ptr(), max(out.stride(0), N), K.dtype_code(out.dtype), None, b, act)
+             out.data_ptr(), _row_stride(out, "linear"), K.dtype_code(out.dtype), None, b, act)
     return out if lead is None else out.reshape(*lead, N)

@@ -251,8 +251,8 @@ class AdamW(torch.optim.Optimizer):
     ``step`` and exp_avg / exp_avg_sq (f32, or uint8 codes with exp_avg_scale / exp_avg_sq_scale).  A
     param without a gradient is left as it is; the update number is the group's, so params that step
     together must always have done so (refused else).  After a first eager step on the same gradients'
-    storage ``step()`` can be captured into a graph (``zero_grad(set_to_none=False)``); a graph works on the
-    state that was there, so ``load_state_dict`` asks for a new capture."""
+    storage ``step()`` can be captured into a graph (``zero_grad(set_to_none=False)``); a graph keeps the
+    hyper-parameters and the state that were there, so ``load_state_dict`` asks for a new capture."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
         if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and 0 <= betas[0] < 1 and 0 <= betas[1] < 1):

@@ -200,6 +200,65 @@ def test_engine_takes_over_a_stepped_optimizer():
     _step_follows_the_formula(eng, opt, lambda: eng.step_minibatch(*batch))
 
 
+def _rank(rank, world, port, q):
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    sys.path[:0] = [here, os.path.join(os.path.dirname(here), "linkless-link-prediction_amd")]
+    import torch.distributed as dist
+
+    import llp_engine
+    import llp_optim
+    import models
+    import test_gpu_multirank as T
+    dev = torch.device("cuda", 0)
+    torch.cuda.set_device(dev)
+    os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", str(port)
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    N, F_, H, L, pairs, ei, x, t_h, anchors, links, args = T._problem()
+    torch.manual_seed(3)
+    model = models.MLP(L, F_, H, H, 0.0).to(dev)
+    pred = models.LinkPredictor("mlp", H, H, 1, L, 0.0).to(dev)
+    tpred = models.LinkPredictor("mlp", 256, 256, 1, 2, 0.0).to(dev)
+    for p in tpred.parameters():
+        p.requires_grad = False
+    opt = llp_optim.AdamW(list(model.parameters()) + list(pred.parameters()), lr=args.lr, state_bits=8)
+    eng = llp_engine.DistillEngine(model, pred, tpred, x.to(dev), t_h.to(dev), ei[0].numpy(), ei[1].numpy(), N, args, opt,
+                                   dtype="bf16", seed=11)
+    b0, b1, p0, p1, kw = T._part(eng, rank, world, anchors.numel(), links.numel())
+    pr = pairs.to(torch.int32).to(dev).contiguous()
+    a_dev, l_dev = anchors[b0:b1].to(dev), links[p0:p1].to(dev)
+    before = [p.detach().clone() for p in eng.all_params]
+    eng.begin_epoch()
+    eng.step_minibatch(a_dev, l_dev, pr, **kw)
+    graph = eng.capture_minibatch(a_dev, l_dev, pr, **kw)
+    graph.replay()
+    eng.end_epoch(2 * links.numel())
+    torch.cuda.synchronize()
+    assert any(not torch.equal(a, b) for a, b in zip(before, eng.all_params))
+    out = [p.detach().cpu().numpy() for p in eng.all_params]
+    out += [opt.state[p][k].cpu().numpy() for p in eng.all_params for k in ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale")]
+    q.put((rank, out))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_two_ranks_keep_the_same_8bit_state():
+    """Every rank rounds its copy of the moments with the same draws: weights and codes stay replicas."""
+    import torch.multiprocessing as mp
+
+    import test_gpu_multirank as T
+    ctx = mp.get_context("spawn")
+    q, port = ctx.Queue(), T._free_port()
+    procs = [ctx.Process(target=_rank, args=(r, 2, port, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    got = dict(q.get(timeout=100) for _ in procs)
+    for p in procs:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    assert len(got[0]) == len(got[1]) and all(np.array_equal(a, b) for a, b in zip(got[0], got[1]))
+
+
 # ---------------------------------------------------------------- MXFP4 in the evaluation
 class _Spy:
     """Records the operands and results of llp_mx.linear."""

@@ -343,3 +343,20 @@ def test_offsets_past_32_bits():
     for i in at:                  # another kernel's sums: the order differs
         r = int(idx[i])
         assert ((y[i].float() - hy[r]).abs() <= 2 * K * 2.0 ** -23 * size[r] + 2.0 ** -8 * (hy[r].abs() + K * 2.0 ** -23 * size[r])).all(), i
+
+
+def test_given_outputs_that_overlap_are_refused():
+    m = mx()
+    x = torch.randn(64, 128, device=DEV)
+    q, w = m.quantize(x), m.quantize(torch.randn(128, 128, device=DEV))
+    with pytest.raises(ValueError, match="overlaps"):
+        m.linear(q, w, out=q)
+    with pytest.raises(ValueError, match="overlaps"):
+        m.linear(x, w, out=x)
+    with pytest.raises(ValueError, match="rows of out overlap"):
+        m.dequantize(q, out=torch.empty(1, 128, device=DEV).expand(64, 128))
+    with pytest.raises(ValueError, match="rows of out overlap"):
+        m.linear(x, w, out=torch.empty(1, 128, device=DEV).expand(64, 128))
+    before = m.dequantize(q)
+    y = m.linear(q, w, out_dtype="mx4")
+    assert torch.equal(m.dequantize(q), before) and m.linear(q, w, out=m.MX4.empty(64, 128, DEV)).shape == y.shape

@@ -232,3 +232,31 @@ def test_adamw_optimizer_copies():
     opt = llp_optim.AdamW([torch.nn.Parameter(torch.zeros(4))], lr=0.5, state_bits=8, seed=9)
     got = copy.deepcopy(opt)
     assert (got.state_bits, got.seed, got.param_groups[0]["lr"], got._tables) == (8, 9, 0.5, {})
+
+
+def test_mx4_overlaps_are_found():
+    flat = torch.zeros(4096, dtype=torch.uint8)
+    a = llp_mx.MX4(flat[:640].view(10, 64), flat[640:680].view(10, 4), 100)
+    b = llp_mx.MX4(flat[1024:1664].view(10, 64), flat[1664:1704].view(10, 4), 100)
+    llp_mx._apart("x", a, b)
+    x = flat[2048:].view(torch.float32).view(4, 128)
+    llp_mx._apart("x", a, x, b)
+    llp_mx._apart("x", a, llp_mx.MX4(_u8(0, 64), _u8(0, 4), 100))
+    for bad in (a, llp_mx.MX4(flat[576:1216].view(10, 64), flat[1664:1704].view(10, 4), 100),
+                llp_mx.MX4(flat[1024:1664].view(10, 64), flat[676:716].view(10, 4), 100),
+                flat[:1024].view(torch.float32).view(2, 128), flat[:640].view(torch.bfloat16).view(10, 32)[:, 8:]):
+        with pytest.raises(ValueError, match="overlaps"):
+            llp_mx._apart("x", a, bad)
+
+
+def test_mx4_of_one_row_has_no_stride():
+    q = llp_mx.MX4(_u8(5, 64)[2:3], _u8(5, 4).expand(5, 4)[2:3].as_strided((1, 4), (999, 1)), 100)
+    assert (q.c.ld_codes, q.c.ld_scales) == (64, 4)
+
+
+def test_rows_of_a_given_output_do_not_overlap():
+    assert llp_mx._row_stride(torch.zeros(4, 12)[:, :10], "x") == 12
+    assert llp_mx._row_stride(torch.zeros(1, 10).as_strided((1, 10), (3, 1)), "x") == 10
+    for bad in (torch.zeros(1, 10).expand(4, 10), torch.zeros(100).as_strided((4, 10), (9, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            llp_mx._row_stride(bad, "x")
