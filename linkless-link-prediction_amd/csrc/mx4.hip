@@ -542,12 +542,12 @@ __device__ __forceinline__ void wait_vm() {
 }
 
 template <int MI, int NI, int OUT, bool SHORT>
-__global__ __launch_bounds__(256, 2) void gemm_mx4_kernel(Mx4Args g, int64_t tiles_n, int64_t tiles) {
+__global__ __launch_bounds__(256, 2) void gemm_mx4_kernel(Mx4Args g, FastDiv tiles_n, uint32_t tiles) {
   using S = Mx4Stage<MI, NI>;
   __shared__ __align__(16) uint8_t smem[S::LDS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t tile = llp_xcd_block(blockIdx.x, tiles);
-  const int64_t n0 = tile % tiles_n * S::TN, m0 = tile / tiles_n * S::TM;
+  const uint32_t tile = (uint32_t)llp_xcd_block(blockIdx.x, tiles), tile_m = divided(tile, tiles_n);
+  const int64_t n0 = (int64_t)(tile - tile_m * tiles_n.d) * S::TN, m0 = (int64_t)tile_m * S::TM;
 
   // this wave's DMA sources: 16 rows per data instruction (all of W's or all of A's), clamped to the last
   // valid row (what lies past it is not stored)
@@ -740,7 +740,10 @@ template <int MI, int NI>
 int launch_tiled(const Mx4Args& g, int out, int64_t n_out, hipStream_t s) {
   using S = Mx4Stage<MI, NI>;
   const int64_t tn = (n_out + S::TN - 1) / S::TN, tiles = tn * ((g.M + S::TM - 1) / S::TM);
-  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(256), 0, s, g, tn, tiles); };
+  LLP_CHECK_ARG(tiles < (1ll << 31), "llp_gemm_nt_mx4: C has too many tiles");
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(256), 0, s, g, fast_div((uint32_t)tn), (uint32_t)tiles);
+  };
   if (g.Kp <= 384) out == 0 ? go(gemm_mx4_kernel<MI, NI, 0, true>) : out == 1 ? go(gemm_mx4_kernel<MI, NI, 1, true>) : go(gemm_mx4_kernel<MI, NI, 2, true>);
   else out == 0 ? go(gemm_mx4_kernel<MI, NI, 0, false>) : out == 1 ? go(gemm_mx4_kernel<MI, NI, 1, false>) : go(gemm_mx4_kernel<MI, NI, 2, false>);
   LLP_LAUNCH_CHECK();
@@ -762,7 +765,7 @@ static_assert(Mx4Wide::LDS <= 163840, "LDS of a CU");
 __device__ __forceinline__ int place8(int r) { return (r >> 1) & 7; }
 
 template <int OUT>
-__global__ __launch_bounds__(512, 2) void gemm_mx4_wide_kernel(Mx4Args g, int64_t tiles_n, int64_t tiles) {
+__global__ __launch_bounds__(512, 2) void gemm_mx4_wide_kernel(Mx4Args g, FastDiv tiles_n, uint32_t tiles) {
   using S = Mx4Wide;
   __shared__ __align__(16) uint8_t smem[S::LDS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -770,7 +773,10 @@ __global__ __launch_bounds__(512, 2) void gemm_mx4_wide_kernel(Mx4Args g, int64_
   const int ns = (int)(g.Kp / 256), row_scales = (int)(g.Kp / 32);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
   // tiles are dealt in turns of gridDim.x; within a turn each XCD has a contiguous range of them
-  auto tile_of = [&](int64_t turn) { return turn * gridDim.x + llp_xcd_block(blockIdx.x, gridDim.x); };
+  uint32_t tile = (uint32_t)llp_xcd_block(blockIdx.x, gridDim.x);
+  if (tile >= tiles) return;
+  auto tile_m = [&](uint32_t t) { return (int64_t)divided(t, tiles_n) * S::T; };
+  auto tile_n = [&](uint32_t t) { return (int64_t)(t - divided(t, tiles_n) * tiles_n.d) * S::T; };
 
   // DMA sources of the tile that is being fetched: waves 0 .. 3 W's rows, 4 .. 7 A's, 64 each, 8 rows of 128 bytes an
   // instruction; rows past the last valid one repeat it
@@ -784,8 +790,8 @@ __global__ __launch_bounds__(512, 2) void gemm_mx4_wide_kernel(Mx4Args g, int64_
   int last = 0;
   const uint8_t *base = nullptr, *sp = nullptr;
   const float* bp = nullptr;
-  auto aim = [&](int64_t tile) {
-    const int64_t r0 = isw ? tile % tiles_n * S::T : tile / tiles_n * S::T, left = (isw ? g.N : g.M) - 1 - r0;
+  auto aim = [&](uint32_t t) {
+    const int64_t r0 = isw ? tile_n(t) : tile_m(t), left = (isw ? g.N : g.M) - 1 - r0;
     last = __builtin_amdgcn_readfirstlane((int)(left < S::T ? left : S::T));
     const int r = (wave & 3) * 64 + lane;
     base = codes + r0 * ldc;
@@ -793,7 +799,7 @@ __global__ __launch_bounds__(512, 2) void gemm_mx4_wide_kernel(Mx4Args g, int64_
     bp = isw && g.bias ? g.bias + r0 + (r < last ? r : last) : nullptr;
   };
   // the tile's 256 bias values, in one of two places in turn
-  auto issue_bias = [&](int64_t of) {
+  auto issue_bias = [&](uint32_t of) {
     if (isw && g.bias) dma4(bp, lds0 + S::BIAS + (int)(of & 1) * 4 * S::T + wave * 256);
   };
   auto issue = [&](int k, int buf) {
@@ -812,8 +818,6 @@ __global__ __launch_bounds__(512, 2) void gemm_mx4_wide_kernel(Mx4Args g, int64_
 
   const int wn = wave & 1, wm = wave >> 1;
   const int wrow = wn * 128 + li, arow = S::T + wm * 64 + li, sw = place8(li);
-  int64_t turn = 0, tile = tile_of(0);
-  if (tile >= tiles) return;
   if (!g.bias) *(float*)(smem + S::BIAS + 4 * threadIdx.x) = 0.f;
   aim(tile);
   issue_scales(0);
@@ -821,8 +825,8 @@ __global__ __launch_bounds__(512, 2) void gemm_mx4_wide_kernel(Mx4Args g, int64_
   issue(0, 0);
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   int buf = 0;
-  for (; tile < tiles;) {
-    const int64_t next = tile_of(++turn);
+  for (uint32_t turn = 1; tile < tiles; ++turn) {
+    const uint32_t next = tile + gridDim.x;
     float16_t acc[4][2];
 #pragma unroll
     for (int f = 0; f < 4; ++f)
@@ -900,15 +904,15 @@ __global__ __launch_bounds__(512, 2) void gemm_mx4_wide_kernel(Mx4Args g, int64_
     // The half of LDS that was just read takes C on its way out, so that a store covers whole lines of the output's
     // rows: each wave its own 8 KB, which only its own next fetch overwrites.  Chunk c of row r at place c ^ r.
     uint8_t* const out = smem + (buf ^ 1) * S::STAGE + wave * 8192;
-    const int64_t n0 = tile % tiles_n * S::T + wn * 128, m0 = tile / tiles_n * S::T + wm * 64;
-    const bool full = m0 + 64 <= g.M && n0 + 128 <= g.N;
+    const int64_t nc = tile_n(tile) + wn * 128, mc = tile_m(tile) + wm * 64;
+    const bool full = mc + 64 <= g.M && nc + 128 <= g.N;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int64_t m = m0 + 32 * e + li;
+      const int64_t m = mc + 32 * e + li;
       uint32_t row_scales4 = 0;
 #pragma unroll
       for (int f = 0; f < 4; ++f) {
-        const int64_t nb = n0 + 32 * f;
+        const int64_t nb = nc + 32 * f;
         __builtin_amdgcn_sched_barrier(0);
         float b[16];
 #pragma unroll
@@ -944,17 +948,17 @@ __global__ __launch_bounds__(512, 2) void gemm_mx4_wide_kernel(Mx4Args g, int64_
 #pragma unroll
         for (int i = 0; i < 32 * LANES / 64; ++i) {
           const int r = i * (64 / LANES) + lane / LANES, q = lane % LANES;
-          const int64_t mr = m0 + 32 * e + r;
+          const int64_t mr = mc + 32 * e + r;
           if constexpr (OUT == 1) {
             const u4v v = *reinterpret_cast<const u4v*>(out + r * 256 + ((q ^ (r & 15)) << 4));
-            store_c8(g, mr, n0 + 8 * q, v);
+            store_c8(g, mr, nc + 8 * q, v);
           } else {
             const u4v v = *reinterpret_cast<const u4v*>(out + r * 64 + ((q ^ (r >> 2 & 3)) << 4));
-            *reinterpret_cast<u4v*>((uint8_t*)g.C4.codes + mr * g.C4.ld_codes + n0 / 2 + 16 * q) = v;
+            *reinterpret_cast<u4v*>((uint8_t*)g.C4.codes + mr * g.C4.ld_codes + nc / 2 + 16 * q) = v;
           }
         }
         if constexpr (OUT == 2)
-          if (h == 0) *(uint32_t*)((uint8_t*)g.C4.scales + m * g.C4.ld_scales + n0 / 32) = row_scales4;
+          if (h == 0) *(uint32_t*)((uint8_t*)g.C4.scales + m * g.C4.ld_scales + nc / 32) = row_scales4;
       }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // its own reads of C, before its next fetch into the same place
@@ -964,7 +968,10 @@ __global__ __launch_bounds__(512, 2) void gemm_mx4_wide_kernel(Mx4Args g, int64_
 
 int launch_wide(const Mx4Args& g, int out, int64_t n_out, hipStream_t s) {
   const int64_t tn = (n_out + 255) / 256, tiles = tn * ((g.M + 255) / 256);
-  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>(tiles, 256)), dim3(512), 0, s, g, tn, tiles); };
+  LLP_CHECK_ARG(tiles < (1ll << 31), "llp_gemm_nt_mx4: C has too many tiles");
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>(tiles, 256)), dim3(512), 0, s, g, fast_div((uint32_t)tn), (uint32_t)tiles);
+  };
   out == 0 ? go(gemm_mx4_wide_kernel<0>) : out == 1 ? go(gemm_mx4_wide_kernel<1>) : go(gemm_mx4_wide_kernel<2>);
   LLP_LAUNCH_CHECK();
   return LLP_OK;
