@@ -93,12 +93,14 @@ __device__ __forceinline__ uint32_t divided(uint32_t u, const FastDiv& f) {
 }
 
 // 8 values per lane, a block of 32 per quad: the block's largest by two quad exchanges, 4 bytes of
-// codes per lane, one scale byte per quad.  Four such units per thread, 256 apart, all loaded before the first is
-// used.  Bound by memory: 4 or 2 B read, 17/32 B written per value.
+// codes per lane, one scale byte per quad.  Two such units per thread, 256 apart, both loaded before the first is
+// used: 262144 pairs of 235868 rows of 1024 in bf16 196 us, one unit 216, four 227, eight 354.  Bound by memory: 4 or 2 B
+// read, 17/32 B written per value: 235868 rows of 1024 in bf16 101 us, 6.1 TB/s (a large copy reaches 4.8).
+constexpr int QUANTIZE_UNITS = 2;
 template <typename T, bool PAIRS>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(uint32_t units, int K, FastDiv per_row, llp_operand X,
                                                            llp_mx4 out) {
-  constexpr int U = 4;
+  constexpr int U = QUANTIZE_UNITS;
   const uint32_t u0 = blockIdx.x * (256u * U) + threadIdx.x;
   float x[U][8], y[U][8];
   uint32_t row[U];
@@ -129,16 +131,25 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(uint32_t units, int K
   }
 }
 
+template <bool ONCE, typename V>
+__device__ __forceinline__ void store_as(void* p, V v) {   // ONCE: nontemporal, past the caches
+  if constexpr (ONCE) __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
+  else *reinterpret_cast<V*>(p) = v;
+}
+
 // the value of code c (E2M1 has f32's fields but for the bias: 2 exponent bits, 1 mantissa bit)
 __device__ __forceinline__ float mx4_value(uint32_t c, float scale) {
   const float m = __uint_as_float((c & 7u) << 22) * 0x1p126f;
   return __uint_as_float(__float_as_uint(m) | ((c & 8u) << 28)) * scale;
 }
 
-template <typename T>
+// 16 bytes of a row per lane and unit, so that a store covers whole lines: 8 bf16 or 4 f32 values; two units a thread.
+// 262144 x 1024 to bf16: 93 us, 7.3 TB/s (a fill reaches 6.8).
+constexpr int DEQUANTIZE_UNITS = 2;
+template <typename T, bool ONCE>
 __global__ __launch_bounds__(256) void mx4_dequantize_kernel(uint32_t units, int K, FastDiv per_row, llp_mx4 X,
                                                              T* __restrict__ Y, int64_t ldy) {
-  constexpr int U = 4;
+  constexpr int U = DEQUANTIZE_UNITS, V = 16 / sizeof(T);
   const uint32_t u0 = blockIdx.x * (256u * U) + threadIdx.x;
   uint32_t row[U], codes[U], s[U];
   int col[U];
@@ -146,8 +157,10 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(uint32_t units, int
   for (int i = 0; i < U; ++i) {
     const uint32_t u = u0 + 256 * i < units ? u0 + 256 * i : units - 1;
     row[i] = divided(u, per_row);
-    col[i] = (int)(u - row[i] * per_row.d) * 8;
-    codes[i] = *(const uint32_t*)((const uint8_t*)X.codes + (int64_t)row[i] * X.ld_codes + (col[i] >> 1));
+    col[i] = (int)(u - row[i] * per_row.d) * V;
+    const uint8_t* c = (const uint8_t*)X.codes + (int64_t)row[i] * X.ld_codes + (col[i] >> 1);
+    if constexpr (V == 8) codes[i] = *(const uint32_t*)c;
+    else codes[i] = *(const uint16_t*)c;
     s[i] = ((const uint8_t*)X.scales)[(int64_t)row[i] * X.ld_scales + (col[i] >> 5)];
   }
 #pragma unroll
@@ -156,24 +169,23 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(uint32_t units, int
     const int n = K - col[i];
     const float f = s[i] == 255u ? __uint_as_float(0x7FC00000u) : mx4_scale_f32(s[i]);
     T* y = Y + (int64_t)row[i] * ldy + col[i];
-    float v[8];
+    float v[V];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = mx4_value(codes[i] >> (4 * j), f);
-    if (n >= 8) {
-      if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<f4_any*>(y) = f4_any{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<f4_any*>(y + 4) = f4_any{v[4], v[5], v[6], v[7]};
+    for (int j = 0; j < V; ++j) v[j] = mx4_value(codes[i] >> (4 * j), f);
+    if (n >= V) {
+      if constexpr (V == 4) {
+        store_as<ONCE>(y, f4_any{v[0], v[1], v[2], v[3]});
       } else {
         u4_any2 o;
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[j] = bf16_pair(v[2 * j], v[2 * j + 1]);
-        *reinterpret_cast<u4_any2*>(y) = o;
+        store_as<ONCE>(y, o);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < V; ++j)
         if (j < n) {
-          if constexpr (sizeof(T) == 4) y[j] = v[j];
+          if constexpr (V == 4) y[j] = v[j];
           else y[j] = f2bf(v[j]);
         }
     }
@@ -194,7 +206,7 @@ struct Mx4Args {
   int64_t ldc;
   const float* bias;
   int relu;
-  bool streamed;   // C past the caches (launch rule below)
+  bool streamed;   // whole lines of a bf16 C past the caches
 };
 
 // 8 bf16 of C
@@ -1016,7 +1028,12 @@ const char* bad_mx4(const llp_mx4* x, int64_t rows, int64_t K) {
   return nullptr;
 }
 
-// rows of a launch: fewer than 2^31 units of 8 values
+// A result that the 256 MB of last-level cache cannot hold passes by the caches, which what is read then keeps
+// (131072 x 1024 x 1024 to bf16: 108 -> 93 us, 347 -> 342 with a kernel after it that reads C; a C of half the size would be
+// read from the cache: 47 -> 49, 166 -> 175; 262144 x 1024 back to bf16: 122 -> 93)
+bool streams(int64_t M, int64_t N, int dtype) { return M * N >= 1ll << (dtype == LLP_F32 ? 26 : 27); }
+
+// rows of a launch: fewer than 2^31 units
 int64_t slice_rows(int64_t per_row) { return std::max<int64_t>(1, ((1ll << 31) - 1) / per_row); }
 
 int quantize(int dtype, int64_t M, int64_t K, llp_operand X, llp_mx4 out, hipStream_t s) {
@@ -1035,7 +1052,7 @@ int quantize(int dtype, int64_t M, int64_t K, llp_operand X, llp_mx4 out, hipStr
     o.codes = (char*)o.codes + r * o.ld_codes, o.scales = (char*)o.scales + r * o.ld_scales;
     const uint32_t units = (uint32_t)(n * per_row);
     auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3((units + 1023u) / 1024u), dim3(256), 0, s, units, (int)K, fast_div((uint32_t)per_row), x, o);
+      hipLaunchKernelGGL(kernel, dim3((units - 1) / (256u * QUANTIZE_UNITS) + 1), dim3(256), 0, s, units, (int)K, fast_div((uint32_t)per_row), x, o);
     };
     if (dtype == LLP_F32) x.ptr2 ? go(mx4_quantize_kernel<float, true>) : go(mx4_quantize_kernel<float, false>);
     else x.ptr2 ? go(mx4_quantize_kernel<bf16_t, true>) : go(mx4_quantize_kernel<bf16_t, false>);
@@ -1066,17 +1083,19 @@ extern "C" int llp_mx4_dequantize(int64_t M, int64_t K, const llp_mx4* X, int dt
   LLP_CHECK_ARG(Y, "llp_mx4_dequantize: null pointer");
   const char* why = bad_mx4(X, M, K);
   LLP_CHECK_ARG(!why, "llp_mx4_dequantize: X: %s", why);
-  const int64_t per_row = (K + 7) / 8, slice = slice_rows(per_row);
+  const int64_t v = dtype == LLP_F32 ? 4 : 8, per_row = (K + v - 1) / v, slice = slice_rows(per_row);
+  const bool once = streams(M, K, dtype);
   for (int64_t r = 0; r < M; r += slice) {
     const int64_t n = std::min(M - r, slice);
     llp_mx4 x = *X;
     x.codes = (char*)x.codes + r * x.ld_codes, x.scales = (char*)x.scales + r * x.ld_scales;
     const uint32_t units = (uint32_t)(n * per_row);
-    const dim3 grid((units + 1023u) / 1024u);
-    if (dtype == LLP_F32)
-      hipLaunchKernelGGL(mx4_dequantize_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, units, (int)K, fast_div((uint32_t)per_row), x, (float*)Y + r * ldy, ldy);
-    else
-      hipLaunchKernelGGL(mx4_dequantize_kernel<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, units, (int)K, fast_div((uint32_t)per_row), x, (bf16_t*)Y + r * ldy, ldy);
+    auto go = [&](auto kernel, auto* y) {
+      hipLaunchKernelGGL(kernel, dim3((units - 1) / (256u * DEQUANTIZE_UNITS) + 1), dim3(256), 0, (hipStream_t)stream, units,
+                         (int)K, fast_div((uint32_t)per_row), x, y + r * ldy, ldy);
+    };
+    if (dtype == LLP_F32) once ? go(mx4_dequantize_kernel<float, true>, (float*)Y) : go(mx4_dequantize_kernel<float, false>, (float*)Y);
+    else once ? go(mx4_dequantize_kernel<bf16_t, true>, (bf16_t*)Y) : go(mx4_dequantize_kernel<bf16_t, false>, (bf16_t*)Y);
     LLP_LAUNCH_CHECK();
   }
   return LLP_OK;
@@ -1117,10 +1136,7 @@ extern "C" int llp_gemm_nt_mx4(int64_t M, int64_t N, int64_t K, int a_dtype, con
     LLP_CHECK_ARG(M == 1 || ldc >= N, "llp_gemm_nt_mx4: C's rows overlap");
     g.C = C, g.ldc = ldc;
     out = c_dtype == LLP_F32 ? 0 : 1;
-    // a bf16 C that the 256 MB of last-level cache cannot hold passes by the caches, which A and W then keep
-    // (131072 x 1024 x 1024: 108 -> 93 us, 347 -> 342 with a kernel after it that reads C; a C of half the size would be
-    // read from the cache: 47 -> 49, 166 -> 175)
-    g.streamed = M * N >= (1ll << 27);
+    g.streamed = streams(M, N, c_dtype);
   }
   const int64_t n_out = C4 ? g.Np : N;
   hipStream_t s = (hipStream_t)stream;
