@@ -206,7 +206,7 @@ struct Mx4Args {
   int64_t ldc;
   const float* bias;
   int relu;
-  bool streamed;   // whole lines of a bf16 C past the caches
+  bool streamed;   // whole lines of C past the caches
 };
 
 // 8 bf16 of C
@@ -215,6 +215,26 @@ __device__ __forceinline__ void store_c8(const Mx4Args& g, int64_t m, int64_t n,
   const u4_any2 c = {v[0], v[1], v[2], v[3]};
   if (g.streamed) __builtin_nontemporal_store(c, at);
   else *at = c;
+}
+
+// 32 rows x 64 columns of an f32 C (two tiles of a wave's result) through 8 KB of LDS that the wave has to itself, so that a
+// store covers 256 bytes of a row.  Chunk c (16 bytes) of row r at place c ^ r.
+__device__ __forceinline__ void store_f32_pair(const Mx4Args& g, uint8_t* part, const float (&y)[2][16], int64_t m0,
+                                               int64_t n0, int lane) {
+  const int h = lane >> 5, li = lane & 31;
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    *reinterpret_cast<float4_t*>(part + li * 256 + (((2 * c + h) ^ (li & 15)) << 4)) =
+        float4_t{y[c >> 2][4 * (c & 3)], y[c >> 2][4 * (c & 3) + 1], y[c >> 2][4 * (c & 3) + 2], y[c >> 2][4 * (c & 3) + 3]};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + (lane >> 4), q = lane & 15;
+    const float4_t v = *reinterpret_cast<const float4_t*>(part + r * 256 + ((q ^ (r & 15)) << 4));
+    f4_any* const at = reinterpret_cast<f4_any*>((float*)g.C + (m0 + r) * g.ldc + n0 + 4 * q);
+    const f4_any c = {v[0], v[1], v[2], v[3]};
+    if (g.streamed) __builtin_nontemporal_store(c, at);
+    else *at = c;
+  }
 }
 
 // bias of a lane's 16 columns n0 + 8 j + 4 h + i (zero past N)
@@ -267,21 +287,20 @@ __device__ __forceinline__ void tile_codes(const float (&y)[16], int h, uint32_t
   c[1] = (x[0] >> 16) | (x[1] & 0xFFFF0000u);
 }
 
-// One 32 x 32 tile of a wave's result stored: bias, ReLU, the output's type.  FULL: the whole tile lies
-// within M and N.
-template <int OUT, bool FULL>
+// One 32 x 32 tile of a wave's result, perhaps past M or N, stored: bias, ReLU, the output's type
+template <int OUT>
 __device__ __forceinline__ void store_tile(const Mx4Args& g, const float16_t& acc, const float (&b)[16], int64_t m,
                                            int64_t nb, int h) {
-  const bool live = FULL || m < g.M;
+  const bool live = m < g.M;
   float y[16];
   tile_act(acc, b, g.relu, y);
   if constexpr (OUT == 2) {
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (!FULL && nb + 8 * (i >> 2) + 4 * h + (i & 3) >= g.N) y[i] = 0.f;
+      if (nb + 8 * (i >> 2) + 4 * h + (i & 3) >= g.N) y[i] = 0.f;
     uint32_t c[2], sc;
     tile_codes(y, h, c, sc);
-    if (live && (FULL || nb < g.Np)) {
+    if (live && nb < g.Np) {
       uint32_t* o = (uint32_t*)((uint8_t*)g.C4.codes + m * g.C4.ld_codes + nb / 2 + 8 * h);
       o[0] = c[0];
       o[1] = c[1];
@@ -298,7 +317,7 @@ __device__ __forceinline__ void store_tile(const Mx4Args& g, const float16_t& ac
       const int64_t n = nb + 16 * j + 8 * h;
       bf16_t* o = (bf16_t*)g.C + m * g.ldc + n;
       const uint32_t d[4] = {x0[0], x1[0], x0[1], x1[1]};
-      if (FULL || (live && n + 8 <= g.N)) {
+      if (live && n + 8 <= g.N) {
         *reinterpret_cast<u4_any2*>(o) = u4_any2{d[0], d[1], d[2], d[3]};
       } else if (live) {
 #pragma unroll
@@ -311,7 +330,7 @@ __device__ __forceinline__ void store_tile(const Mx4Args& g, const float16_t& ac
     for (int j = 0; j < 4; ++j) {
       const int64_t n = nb + 8 * j + 4 * h;
       float* o = (float*)g.C + m * g.ldc + n;
-      if (FULL || (live && n + 4 <= g.N)) {
+      if (live && n + 4 <= g.N) {
         *reinterpret_cast<f4_any*>(o) = f4_any{y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]};
       } else if (live) {
 #pragma unroll
@@ -679,7 +698,25 @@ __global__ __launch_bounds__(256, 2) void gemm_mx4_kernel(Mx4Args g, FastDiv til
   }
 
   const bool full = m0 + S::TM <= g.M && n0 + S::TN <= g.N;
-  if constexpr (OUT != 0) {
+  if constexpr (OUT == 0) {
+    if (full) {
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the last stage was read by all
+#pragma unroll
+      for (int f = 0; f < NI; f += 2) {
+        const int64_t nb = n0 + (wn * NI + f) * 32;
+        float b[2][16], y[2][16];
+        tile_bias(g, nb, h, true, b[0]);
+        tile_bias(g, nb + 32, h, true, b[1]);
+#pragma unroll
+        for (int e = 0; e < MI; ++e) {
+          tile_act(acc[f][e], b[0], g.relu, y[0]);
+          tile_act(acc[f + 1][e], b[1], g.relu, y[1]);
+          store_f32_pair(g, smem + wave * 8192, y, m0 + (wm * MI + e) * 32, nb, lane);
+        }
+      }
+      return;
+    }
+  } else {
     // Through LDS, so that a store covers whole lines of the output's rows (the registers hold runs of 8 bytes,
     // or 2 of codes, in 32 rows).  A wave writes and reads its own part.
     if (full) {
@@ -738,13 +775,9 @@ __global__ __launch_bounds__(256, 2) void gemm_mx4_kernel(Mx4Args g, FastDiv til
   for (int f = 0; f < NI; ++f) {
     const int64_t nb = n0 + (wn * NI + f) * 32;
     float b[16];
-    tile_bias(g, nb, h, full, b);
+    tile_bias(g, nb, h, false, b);
 #pragma unroll
-    for (int e = 0; e < MI; ++e) {
-      const int64_t m = m0 + (wm * MI + e) * 32 + li;
-      if (full) store_tile<OUT, true>(g, acc[f][e], b, m, nb, h);
-      else store_tile<OUT, false>(g, acc[f][e], b, m, nb, h);
-    }
+    for (int e = 0; e < MI; ++e) store_tile<OUT>(g, acc[f][e], b, m0 + (wm * MI + e) * 32 + li, nb, h);
   }
 }
 
@@ -922,6 +955,7 @@ __global__ __launch_bounds__(512, 2) void gemm_mx4_wide_kernel(Mx4Args g, FastDi
     for (int e = 0; e < 2; ++e) {
       const int64_t m = mc + 32 * e + li;
       uint32_t row_scales4 = 0;
+      float y2[2][16];
 #pragma unroll
       for (int f = 0; f < 4; ++f) {
         const int64_t nb = nc + 32 * f;
@@ -933,9 +967,13 @@ __global__ __launch_bounds__(512, 2) void gemm_mx4_wide_kernel(Mx4Args g, FastDi
 #pragma unroll
           for (int i = 0; i < 4; ++i) b[4 * j + i] = v[i];
         }
-        if (OUT == 0 || !full) {
-          if (full) store_tile<OUT, true>(g, acc[f][e], b, m, nb, h);
-          else store_tile<OUT, false>(g, acc[f][e], b, m, nb, h);
+        if (!full) {
+          store_tile<OUT>(g, acc[f][e], b, m, nb, h);
+          continue;
+        }
+        if constexpr (OUT == 0) {
+          tile_act(acc[f][e], b, g.relu, y2[f & 1]);
+          if (f & 1) store_f32_pair(g, out, y2, mc + 32 * e, nb - 32, lane);
           continue;
         }
         float y[16];
