@@ -538,7 +538,8 @@ __global__ __launch_bounds__(512) void gemm_mx4_rows_kernel(Mx4Args g) {
 }
 
 // ---------------------------------------------------------------- the tiled product
-// A workgroup of 4 waves (2 x 2) computes 64 MI rows x 64 NI columns of C, a wave 32 MI x 32 NI.  128 of K
+// A workgroup of 4 waves (2 x 2) computes 64 MI rows x 64 NI columns of C (64 x 128, 128 x 128 or 128 x 256), a wave 32 MI x
+// 32 NI; four, three or two of them share a CU, so that one's loads and stores run under another's products.  128 of K
 // at a time (a step) go through LDS: 64 bytes of codes per row of W and A, by LDS-DMA (global_load_lds)
 // into one of three stages, two of them in flight while one is read, so one barrier a step.  Chunk c (16
 // bytes) of row r lies at place c ^ place(r) of its row, so that the 16 lanes that read LDS together
@@ -573,7 +574,7 @@ __device__ __forceinline__ void wait_vm() {
 }
 
 template <int MI, int NI, int OUT, bool SHORT>
-__global__ __launch_bounds__(256, 2) void gemm_mx4_kernel(Mx4Args g, FastDiv tiles_n, uint32_t tiles) {
+__global__ __launch_bounds__(256, NI == 2 ? 3 : 2) void gemm_mx4_kernel(Mx4Args g, FastDiv tiles_n, uint32_t tiles) {
   using S = Mx4Stage<MI, NI>;
   __shared__ __align__(16) uint8_t smem[S::LDS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -700,6 +701,7 @@ __global__ __launch_bounds__(256, 2) void gemm_mx4_kernel(Mx4Args g, FastDiv til
   const bool full = m0 + S::TM <= g.M && n0 + S::TN <= g.N;
   if constexpr (OUT == 0) {
     if (full) {
+      static_assert(4 * 8192 <= S::LDS, "C tiles in LDS");
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the last stage was read by all
 #pragma unroll
       for (int f = 0; f < NI; f += 2) {
@@ -763,10 +765,11 @@ __global__ __launch_bounds__(256, 2) void gemm_mx4_kernel(Mx4Args g, FastDiv til
           *reinterpret_cast<u4v*>((uint8_t*)g.C4.codes + m * g.C4.ld_codes + (n0 + wn * 32 * NI) / 2 + 16 * q) = v;
       }
       if constexpr (OUT == 2) {
-        static_assert(NI == 4, "a row's scales as one word");
+        using Scales = typename std::conditional<NI == 4, uint32_t, uint16_t>::type;   // a row's NI bytes
+        static_assert(sizeof(Scales) == NI, "a row's scales as one word");
         for (int r = lane; r < 32 * MI; r += 64)
-          *(uint32_t*)((uint8_t*)g.C4.scales + (m0 + wm * 32 * MI + r) * g.C4.ld_scales + n0 / 32 + wn * NI) =
-              *(const uint32_t*)(part + 32 * MI * ROW + r * NI);
+          *(Scales*)((uint8_t*)g.C4.scales + (m0 + wm * 32 * MI + r) * g.C4.ld_scales + n0 / 32 + wn * NI) =
+              *(const Scales*)(part + 32 * MI * ROW + r * NI);
       }
       return;
     }
@@ -789,8 +792,12 @@ int launch_tiled(const Mx4Args& g, int out, int64_t n_out, hipStream_t s) {
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(256), 0, s, g, fast_div((uint32_t)tn), (uint32_t)tiles);
   };
-  if (g.Kp <= 384) out == 0 ? go(gemm_mx4_kernel<MI, NI, 0, true>) : out == 1 ? go(gemm_mx4_kernel<MI, NI, 1, true>) : go(gemm_mx4_kernel<MI, NI, 2, true>);
-  else out == 0 ? go(gemm_mx4_kernel<MI, NI, 0, false>) : out == 1 ? go(gemm_mx4_kernel<MI, NI, 1, false>) : go(gemm_mx4_kernel<MI, NI, 2, false>);
+  if (g.Kp <= 384) {
+    if constexpr (NI == 4) go(gemm_mx4_kernel<MI, NI, 1, true>);   // (128 x 256 on a short K: bf16 only)
+    else out == 0 ? go(gemm_mx4_kernel<MI, NI, 0, true>) : out == 1 ? go(gemm_mx4_kernel<MI, NI, 1, true>) : go(gemm_mx4_kernel<MI, NI, 2, true>);
+  } else {
+    out == 0 ? go(gemm_mx4_kernel<MI, NI, 0, false>) : out == 1 ? go(gemm_mx4_kernel<MI, NI, 1, false>) : go(gemm_mx4_kernel<MI, NI, 2, false>);
+  }
   LLP_LAUNCH_CHECK();
   return LLP_OK;
 }
@@ -1182,16 +1189,24 @@ extern "C" int llp_gemm_nt_mx4(int64_t M, int64_t N, int64_t K, int a_dtype, con
     const int rc = quantize(a_dtype, M, K, *A, *A4, s);
     if (rc != LLP_OK) return rc;
   }
-  // Which kernel, by the tiles there are (us, rows in MXFP4, bf16 out; 32-bit row offsets within a tile):
-  //   few 32 x 32 tiles: the rows kernel, K over a workgroup's waves (1024 x 1024 x 1024: 9.1, tiled 10.2;
-  //     2048 rows: 15.4 / 10.4; 4096 x 1433 -> 257: 12.9 / 15.4; 8192: 19.6 / 15.7), 16 rows at a time while that
-  //     makes no more than two workgroups a CU (256 x 1024 x 1024: 5.7, 64 at a time 6.3; 512 rows: 9.7 / 6.3);
-  //   no more 128 x 256 tiles than CUs: tiled (8192 x 1024 x 1024: 12.3, wide 13.4; 4096 x 2048 x 2048: 17.2 / 19.0);
-  //   more, and K in whole steps of 256: wide (16384 x 1024 x 1024: 15.5, tiled 18.1; 262144 x 2048 x 2048: 651 / 830).
+  // Which kernel, by the tiles there are (GPU time in us, rows in MXFP4, bf16 out; 32-bit row offsets within a tile):
+  //   up to 512 32 x 32 tiles: the rows kernel, K over a workgroup's waves (512 x 1024 x 1024 6.1, tiled 5.8; 768 rows 8.8 / 6.0;
+  //     512 x 8415 -> 256 9.8 / 23.8, 4096 rows 35 / 24; 1024 x 512 x 512 4.3 / 4.6, 2048 rows 5.5 / 4.8), 16 rows at a time
+  //     while that makes no more than two workgroups a CU (256 x 1024 x 1024 5.7, 64 at a time 6.3; 512 rows 9.7 / 6.3);
+  //   more than 256 128 x 256 tiles, and K in whole steps of 256: wide (12288 x 1024 x 1024 15.0, tiled 16.1; 8192 rows 13.5 / 11.8;
+  //     262144 x 2048 x 2048 657 / 845);
+  //   else tiled, 64 x 128 while that makes one workgroup a CU (two for K <= 2048, where latency counts): 1024 x 2048 x 2048
+  //     9.1, 128 x 128 10.2, 4096 rows 21.1 / 18.1; 8192 x 8415 -> 256 26.4 / 29.6, 12288 rows 37.3 / 30.6;
+  //   128 x 128 then, and 128 x 256, where it fits the columns, for long K (262144 x 8415 -> 256 474, 128 x 128 523; 16384 rows
+  //     47.8 / 32.3) and for a bf16 C past the caches (235868 x 128 -> 1024 120 / 137; 235868 x 128 -> 256 27.2 / 23.6).
   const bool near = W->ld_codes < (1 << 23) && (!A4 || A4->ld_codes < (1 << 23));
-  if (A4 && near && (n_out + 31) / 32 * ((M + 31) / 32) > 1024) {
-    if (g.Kp >= 512 && g.Kp % 256 == 0 && (n_out + 255) / 256 * ((M + 127) / 128) > 256) return launch_wide(g, out, n_out, s);
-    return launch_tiled<2, 4>(g, out, n_out, s);
+  auto tiles = [&](int64_t rows, int64_t cols) { return (M + rows - 1) / rows * ((n_out + cols - 1) / cols); };
+  if (A4 && near && tiles(32, 32) > 512) {
+    if (g.Kp >= 512 && g.Kp % 256 == 0 && tiles(128, 256) > 256) return launch_wide(g, out, n_out, s);
+    if (tiles(64, 128) <= (g.Kp <= 2048 ? 512 : 256)) return launch_tiled<1, 2>(g, out, n_out, s);
+    const bool fits = (n_out + 127) / 128 % 2 == 0;
+    if (fits && ((out == 1 && g.streamed) || (g.Kp > 2048 && tiles(128, 256) >= 256))) return launch_tiled<2, 4>(g, out, n_out, s);
+    return launch_tiled<2, 2>(g, out, n_out, s);
   }
-  return (n_out + 31) / 32 * ((M + 15) / 16) <= 512 ? launch_rows<1>(g, src, out, n_out, s) : launch_rows<4>(g, src, out, n_out, s);
+  return tiles(16, 32) <= 512 ? launch_rows<1>(g, src, out, n_out, s) : launch_rows<4>(g, src, out, n_out, s);
 }

@@ -22,12 +22,15 @@ import torch
 import llp_hip as K
 
 
-def _direct(rows, cols):
+def _direct(rows, cols, outs):
     """Whether rows in f32 / bf16 are quantised inside the product (one launch) or first, once, instead of
-    once for each 32 columns of the result.  GPU time in us, inside / first, bf16 rows: 256 x 1024 -> 1024 8.3 / 8.6,
-    512 rows 9.9 / 9.4; 64 x 2048 -> 2048 7.3 / 8.6, 128 rows 12.0 / 11.3; 64 x 4096 -> 64 10.3 / 11.0;
-    1 x 8415 -> 256 10.6 / 10.8, 16 rows 27.7 / 13.3; 512 x 128 -> 1024 5.6 / 6.5, 1024 rows 9.3 / 7.0."""
-    return rows <= 512 and rows * cols <= (1 << 18 if cols <= 4096 else 1 << 15)
+    once for each 32 columns of the result: while the product has one workgroup (16 rows x 32 columns) a CU, and K
+    leaves each of its waves few steps.  GPU time in us, inside / first, bf16 rows: 128 x 1024 -> 1024 5.1 / 6.3, 256 rows
+    8.0 / 7.9; 64 x 2048 -> 2048 7.0 / 7.7, 128 rows 11.7 / 10.5; 512 x 512 -> 512 5.8 / 6.0; 47 x 1433 -> 257 in f32
+    6.0 / 6.5; 8 x 4096 -> 64 8.7 / 9.1, 16 rows 10.0 / 9.9; 8 x 8415 -> 256 18.5 / 11.5.  (A second launch costs its
+    caller about 4 us more.)"""
+    groups = -(-rows // 16) * -(-outs // 32)
+    return (cols <= 2048 and groups <= (512 if cols <= 512 else 256)) or (rows <= 8 and cols <= 4096 and groups <= 256)
 
 
 _FLOATS = (torch.float32, torch.bfloat16)
@@ -223,7 +226,7 @@ def linear(x, w, bias=None, relu=False, out_dtype=None, out=None):
     code, x4 = 0, x if four_in else None
     if not four_in:
         op, code = C.byref(K.Operand(x.data_ptr(), None, None, None, x.stride(0), 0, None)), K.dtype_code(x.dtype)
-        if not _direct(rows, width):
+        if not _direct(rows, width, N):
             x4 = MX4.empty(rows, width, dev)      # scratch: the call quantises x into it first
     c4 = None if x4 is None else C.byref(x4.c)
     act = K.ACT_RELU if relu else K.ACT_NONE

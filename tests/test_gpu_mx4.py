@@ -150,7 +150,8 @@ SHAPES = [(1, 16, 8), (1, 1024, 1024), (1, 1433, 257), (2, 33, 1), (3, 128, 33),
           (33, 256, 128), (47, 1433, 257), (64, 8415, 40), (65, 128, 96), (129, 1000, 129), (255, 512, 256), (257, 384, 300),
           (300, 2048, 64), (513, 128, 513), (1030, 257, 1024), (4099, 64, 72), (2050, 129, 513),
           (33000, 128, 40), (1500, 1433, 700), (5000, 600, 257), (3000, 384, 384), (8200, 100, 300),
-          (8200, 512, 257), (8231, 1024, 129), (8500, 300, 130), (8192, 1500, 96), (8225, 2048, 160)]
+          (600, 300, 1000), (600, 2300, 2050), (2050, 640, 520), (5000, 256, 1030), (9000, 384, 260), (8200, 2200, 300),
+          (8200, 2200, 1024), (8200, 512, 257), (8231, 1024, 129), (8500, 300, 130), (8192, 1500, 96), (8225, 2048, 160)]
 
 
 @pytest.mark.parametrize("M,K,N", SHAPES)
