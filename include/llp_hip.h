@@ -630,7 +630,8 @@ int llp_refresh_shadows(const llp_tensor_desc* descs, int n_tensors, int64_t max
  * input (in place) or a buffer that overlaps no input: the state before the step then stays whole.
  * state_bits 32: exp_avg / exp_avg_sq are f32[numel].
  * state_bits 8: uint8[numel] codes and one scale byte s per 32 consecutive elements
- *   (uint8[ceil(numel / 32)], the value 2^(s - 127); 255: the block holds a NaN): exp_avg as E4M3
+ *   (uint8[ceil(numel / 32)], the value 2^(s - 127); 255: the block holds a NaN or an infinity and reads
+ *   as NaN, all 32 of it): exp_avg as E4M3
  *   codes, exp_avg_sq as codes of sqrt(v) with 4 exponent and 4 mantissa bits, bias 7, no sign (largest
  *   496, 2^-10 apart below 2^-6).  Rounding is stochastic and keeps the means of m and v: one 16-bit
  *   draw per element, half (e mod 2) of word (e mod 8) / 2 of the Philox block e / 8 in stream

@@ -5,7 +5,7 @@
 //   p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
 //
 // 8-bit moments.  Each 32 consecutive elements of a tensor share a power of two 2^k (one byte,
-// k + 127; 255 = the block holds a NaN): m is kept as E4M3 codes, r = sqrt(v) as unsigned codes of
+// k + 127; 255 = the block holds a NaN or an infinity): m is kept as E4M3 codes, r = sqrt(v) as unsigned codes of
 // 4 exponent and 4 mantissa bits (bias 7, largest 496, no NaN code).  k is the least power that
 // holds the block's largest value (448 / 496 times 2^k), so nothing saturates.  The root is what is kept because
 // its range is half of v's in exponents: 2^-10 .. 496 beside the block's largest covers 2^38 of v.
@@ -15,7 +15,7 @@
 // a code is 3 to 6 % wide, and v would never move down.
 // The update of p uses m' and v' before they are rounded.
 //
-// Bound by memory: per element 8 B of p, 4 (2) of g, and 16 B of f32 moments or 4.1 B of 8-bit ones.  36 M f32
+// Bound by memory: per element 8 B of p, 4 (2) of g, and 16 B of f32 moments or 4.1 B of 8-bit ones.  34 M f32
 // elements with a bf16 copy: 200 us at 5.1 TB/s with f32 moments, 1e8 with 8-bit ones 342 us at 5.3 TB/s (a large copy
 // reaches 4.8); 500,000 elements 5.0 and 5.6 us, where the launch is what counts.
 #include <hip/hip_runtime.h>
@@ -332,6 +332,7 @@ __global__ __launch_bounds__(256) void adamw_copy_t_kernel(const llp_adamw_desc*
                                                            const int32_t* __restrict__ work) {
   __shared__ float tile[64][65];
   const llp_adamw_desc d = descs[work[2 * (int64_t)blockIdx.x]];
+  if (!d.copy_t) return;
   const int64_t ti = work[2 * (int64_t)blockIdx.x + 1], tc = (d.cols + 63) / 64;
   const int64_t r0 = (ti / tc) * 64, c0 = (ti % tc) * 64;
   const int64_t ldt = d.copy_t_ld ? d.copy_t_ld : d.rows;

@@ -248,8 +248,8 @@ class AdamW(torch.optim.Optimizer):
     no maximize); ``state_bits`` 32 or 8; ``seed`` of the 8-bit moments' rounding.
 
     Params in f32 or bf16 on the GPU, dense gradients of one dtype in a group.  ``state[p]`` holds
-    ``step`` and exp_avg / exp_avg_sq (f32, or uint8 codes with exp_avg_scale / exp_avg_sq_scale).  A
-    param without a gradient is left as it is; the update number is the group's, so params that step
+    ``step`` and exp_avg / exp_avg_sq (f32, or uint8 codes with exp_avg_scale / exp_avg_sq_scale; a NaN or an
+    infinity takes its 32 neighbours' moments with it).  A param without a gradient is left as it is; the update number is the group's, so params that step
     together must always have done so (refused else).  After a first eager step on the same gradients'
     storage ``step()`` can be captured into a graph (``zero_grad(set_to_none=False)``); a graph keeps the
     hyper-parameters and the state that were there, so ``load_state_dict`` asks for a new capture."""

@@ -433,3 +433,101 @@ def test_adamw_step_as_the_tables_grow():
             tab.step(torch.full((1,), t, dtype=torch.int64, device=DEV), seed=9, **HYPER)
         got.append([ps[0], *st[0], *st[1]])
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def _eager_and_torch(ps):
+    o = _opt()
+    mine, ref = [torch.nn.Parameter(p.to(DEV)) for p in ps], [torch.nn.Parameter(p.double()) for p in ps]
+    return mine, ref, o.AdamW(mine, lr=0.02, weight_decay=0.1), torch.optim.AdamW(ref, lr=0.02, weight_decay=0.1)
+
+
+def _close_after(mine, ref, T):
+    # as in test_optimizer_matches_torch_adamw
+    for x, y in zip(mine, ref):
+        tol = T * (4 * U * (y.detach().abs() + 0.02 * T * 4) + 200 * U * 0.02 * 7)
+        assert ((x.detach().cpu().double() - y.detach()).abs() <= tol).all()
+
+
+def test_optimizer_graph_outlives_other_gradients():
+    """A captured step goes on with its own gradients' storage while eager steps use another, on one count."""
+    gen = torch.Generator().manual_seed(31)
+    mine, ref, a, b = _eager_and_torch([torch.randn(50, 20, generator=gen), torch.randn(77, generator=gen)])
+
+    def grads():
+        return [torch.randn(p.shape, generator=gen) for p in ref]
+
+    def torch_step(gs):
+        for y, g in zip(ref, gs):
+            y.grad = g.double()
+        b.step()
+
+    gs = grads()
+    for x, g in zip(mine, gs):
+        x.grad = g.to(DEV)
+    a.step()
+    torch_step(gs)
+    held = [x.grad for x in mine]
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        a.step()
+    T = 1
+    for t in range(4):
+        gs = grads()
+        for h, g in zip(held, gs):
+            h.copy_(g)
+        graph.replay()
+        torch_step(gs)
+        gs = grads()
+        for x, g in zip(mine, gs):
+            x.grad = g.to(DEV)
+        a.step()
+        torch_step(gs)
+        T += 2
+    torch.cuda.synchronize()
+    _close_after(mine, ref, T)
+    assert float(a.state_dict()["state"][0]["step"]) == T
+
+
+def test_optimizer_refuses_params_of_different_age():
+    gen = torch.Generator().manual_seed(32)
+    mine, _, a, _ = _eager_and_torch([torch.randn(5, generator=gen), torch.randn(6, generator=gen)])
+    for x in mine:
+        x.grad = torch.ones_like(x)
+    a.step()
+    g1 = mine[1].grad
+    mine[1].grad = None
+    a.step()
+    before = [x.detach().clone() for x in mine]
+    mine[1].grad = g1
+    with pytest.raises(RuntimeError, match="same number of steps"):
+        a.step()
+    assert all(torch.equal(x, y) for x, y in zip(mine, before))
+    sd = a.state_dict()["state"]
+    assert float(sd[0]["step"]) == 2 and float(sd[1]["step"]) == 1
+
+
+def test_two_tables_on_two_streams():
+    """Steps of two tables at once give what they give alone."""
+    o = _opt()
+    sizes = [(1000, 300), (300,), (257,)]
+
+    def tables():
+        out = []
+        for seed, bits in ((1, 32), (2, 8)):
+            P, G, M, V, MS, VS = _problem(sizes, seed, bits=bits)
+            out.append((o.AdamWTable(P, G, M, V, **({} if bits == 32 else dict(exp_avg_scale=MS, exp_avg_sq_scale=VS))), P + M + V))
+        return out
+
+    got = []
+    for streams in ([torch.cuda.current_stream()] * 2, [torch.cuda.Stream(), torch.cuda.Stream()]):
+        tabs = tables()
+        ctr = torch.zeros(1, dtype=torch.int64, device=DEV)
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for s, (tab, _) in zip(streams, tabs):
+                with torch.cuda.stream(s):
+                    tab.step(ctr, seed=3, **HYPER)
+        torch.cuda.synchronize()
+        got.append([t for _, ts in tabs for t in ts])
+    assert all(torch.equal(x, y) for x, y in zip(*got))

@@ -361,3 +361,50 @@ def test_given_outputs_that_overlap_are_refused():
     before = m.dequantize(q)
     y = m.linear(q, w, out_dtype="mx4")
     assert torch.equal(m.dequantize(q), before) and m.linear(q, w, out=m.MX4.empty(64, 128, DEV)).shape == y.shape
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("K", [1, 7, 33, 130, 1433])
+def test_dequantize_into_a_strided_view(dt, K):
+    m = mx()
+    x = torch.randn(37, K, generator=torch.Generator().manual_seed(K)).to(DEV)
+    q = m.quantize(x)
+    wide = torch.full((39, K + 5), 7.0, dtype=TYPES[dt], device=DEV)
+    out = wide[1:38, 3:3 + K]
+    assert m.dequantize(q, out=out) is out
+    assert np.array_equal(_f64(out), Q.mx4_round(_f64(x)))
+    wide[1:38, 3:3 + K] = 7.0
+    assert (wide == 7.0).all()
+
+
+def test_quantize_repeated_rows():
+    """Rows that are one row in memory, and the same index many times."""
+    m = mx()
+    row = torch.randn(1, 300, device=DEV)
+    _same(m.quantize(row.expand(50, 300)), np.repeat(_f64(row), 50, 0))
+    h = torch.randn(3, 300, device=DEV)
+    _same(m.quantize(h, torch.full((500,), 2, dtype=torch.int32, device=DEV)), np.repeat(_f64(h[2:]), 500, 0))
+    with pytest.raises(RuntimeError, match="overlap"):
+        m.linear(row.expand(50, 300), m.quantize(torch.randn(8, 300, device=DEV)))
+
+
+@pytest.mark.parametrize("M,K,N", [(600, 300, 1000), (2050, 640, 520), (9000, 384, 260), (8200, 512, 512), (40, 1024, 2048)])
+def test_replays_of_one_graph_beside_eager_calls(M, K, N):
+    """Each kernel captured, replayed three times on new rows, with eager calls of another shape between."""
+    m = mx()
+    g = torch.Generator(device=DEV).manual_seed(M)
+    w, b = m.quantize(torch.randn(N, K, generator=g, device=DEV)), torch.randn(N, generator=g, device=DEV)
+    x = torch.randn(M, K, generator=g, device=DEV).bfloat16()
+    m.linear(x, w, b, relu=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = m.linear(x, w, b, relu=True)
+        q = m.linear(m.quantize(x), w, b, relu=True, out_dtype="mx4")
+    for _ in range(3):
+        x.copy_(torch.randn(M, K, generator=g, device=DEV))
+        graph.replay()
+        m.linear(torch.randn(100, K, generator=g, device=DEV), w)
+        torch.cuda.synchronize()
+        assert torch.equal(y, m.linear(x, w, b, relu=True))
+        assert torch.equal(q.codes, m.linear(m.quantize(x), w, b, relu=True, out_dtype="mx4").codes)
