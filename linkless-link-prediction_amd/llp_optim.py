@@ -8,8 +8,7 @@ place or into other buffers.
 """
 from __future__ import annotations
 
-import ctypes as C
-
+import numpy as np
 import torch
 
 import llp_hip as K
@@ -28,6 +27,15 @@ def _check(name, ts, ref, dtypes, dev):
 
 
 _FLOATS = (torch.float32, torch.bfloat16)
+
+
+def _pairs(counts):
+    """(tensor, 0), (tensor, 1) .. up to each tensor's count as int32 pairs; counts: two runs over the tensors."""
+    c = np.asarray(counts, dtype=np.int64)
+    out = np.empty((int(c.sum()), 2), dtype=np.int32)
+    out[:, 0] = np.repeat(np.arange(c.size) % (c.size // 2), c)
+    out[:, 1] = np.arange(out.shape[0]) - np.repeat(np.cumsum(c) - c, c)
+    return torch.from_numpy(out)
 
 
 class AdamWTable:
@@ -104,7 +112,7 @@ class AdamWTable:
             raise RuntimeError("AdamWTable runs only on the MI355X HIP device (got CPU tensors; no CPU fallback)")
         self._apart(ins, outs, grads, copies, copies_t, values)
         L = K.load()
-        descs, work, work_t = [], [], []
+        descs, items, tiles = [], [], []
 
         def at(ts, i):
             return None if ts is None else ts[i].data_ptr()
@@ -120,19 +128,15 @@ class AdamWTable:
                 at(outs.get("exp_avg_sq_scale"), i), K.ptr(c[0]), K.ptr(ct[0]),
                 at(values.get("exp_avg"), i), at(values.get("exp_avg_sq"), i), p.numel(), rows, cols,
                 c[1], ct[1], groups[i], K.dtype_code(kinds.pop()) if kinds else K.LLP_F32))
-            items = L.llp_adamw_work_items(p.numel())
-            work.append(torch.stack([torch.full((items,), i, dtype=torch.int32), torch.arange(items, dtype=torch.int32)], 1))
-            if ct[0] is not None:
-                tiles = L.llp_adamw_copy_t_items(rows, cols)
-                work_t.append(torch.stack([torch.full((tiles,), i, dtype=torch.int32),
-                                           torch.arange(tiles, dtype=torch.int32)], 1))
+            items.append(L.llp_adamw_work_items(p.numel()))
+            tiles.append(L.llp_adamw_copy_t_items(rows, cols) if ct[0] is not None else 0)
         self.device = dev
         self.n = len(params)
         self.param_code, self.grad_code = K.dtype_code(params[0].dtype), K.dtype_code(grads[0].dtype)
-        self._descs = K.descs_to_device(descs, dev)
-        self._work = torch.cat(work).to(dev)
-        self._work_t = torch.cat(work_t).to(dev) if work_t else None
-        self._args = (self._descs.data_ptr(), self.n, self._work.data_ptr(), self._work.shape[0])
+        self._descs, self._work = K.descs_to_device(descs, dev), _pairs(items + tiles).to(dev)
+        self.n_work, self.n_tiles = sum(items), sum(tiles)
+        self._args = (self._descs.data_ptr(), self.n, self._work.data_ptr(), self.n_work)
+        self._args_t = (self._descs.data_ptr(), self._work.data_ptr() + 8 * self.n_work, self.n_tiles, self.param_code)
         self._keep = (ins, outs, grads, copies, copies_t, values)
 
     @staticmethod
@@ -214,9 +218,8 @@ class AdamWTable:
             raise TypeError(f"AdamWTable.step: sumsq as f32[{self.n_groups}] on {self.device}")
         K.launch("llp_adamw_step", self.device, *self._args, self.bits, self.param_code, self.grad_code, K.ptr(sumsq),
                  max_norm, lr, betas[0], betas[1], eps, weight_decay, step.data_ptr(), int(seed) & 0xFFFFFFFFFFFFFFFF)
-        if self._work_t is not None:
-            K.launch("llp_adamw_copy_t", self.device, self._descs.data_ptr(), self._work_t.data_ptr(),
-                     self._work_t.shape[0], self.param_code)
+        if self.n_tiles:
+            K.launch("llp_adamw_copy_t", self.device, *self._args_t)
 
     def values(self):
         """Fill the ``values`` lists with the values of the 8-bit moments that the last step wrote."""
@@ -248,11 +251,12 @@ class AdamW(torch.optim.Optimizer):
     no maximize); ``state_bits`` 32 or 8; ``seed`` of the 8-bit moments' rounding.
 
     Params in f32 or bf16 on the GPU, dense gradients of one dtype in a group.  ``state[p]`` holds
-    ``step`` and exp_avg / exp_avg_sq (f32, or uint8 codes with exp_avg_scale / exp_avg_sq_scale; a NaN or an
-    infinity takes its 32 neighbours' moments with it).  A param without a gradient is left as it is; the update number is the group's, so params that step
-    together must always have done so (refused else).  After a first eager step on the same gradients'
-    storage ``step()`` can be captured into a graph (``zero_grad(set_to_none=False)``); a graph keeps the
-    hyper-parameters and the state that were there, so ``load_state_dict`` asks for a new capture."""
+    ``step`` and exp_avg / exp_avg_sq (f32, or uint8 codes with exp_avg_scale / exp_avg_sq_scale; a NaN or
+    an infinity takes the moments of its block of 32 with it).  A param without a gradient is left as it
+    is; the update number is the group's, so params that step together must always have done so (refused
+    else).  After a first eager step on the same gradients' storage ``step()`` can be captured into a
+    graph (``zero_grad(set_to_none=False)``); a graph keeps the hyper-parameters and the state that were
+    there, so ``load_state_dict`` asks for a new capture."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
         if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and 0 <= betas[0] < 1 and 0 <= betas[1] < 1):

@@ -260,3 +260,8 @@ def test_rows_of_a_given_output_do_not_overlap():
     for bad in (torch.zeros(1, 10).expand(4, 10), torch.zeros(100).as_strided((4, 10), (9, 1))):
         with pytest.raises(ValueError, match="overlap"):
             llp_mx._row_stride(bad, "x")
+
+
+def test_adamw_work_pairs():
+    assert llp_optim._pairs([2, 0, 3, 0, 1, 2]).tolist() == [[0, 0], [0, 1], [2, 0], [2, 1], [2, 2], [1, 0], [2, 0], [2, 1]]
+    assert llp_optim._pairs([0, 0]).shape == (0, 2)
