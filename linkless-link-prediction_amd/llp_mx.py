@@ -129,7 +129,8 @@ def _rows2d(x, what):
         raise ValueError(f"{what}: a 2-D tensor with contiguous rows")
     if x.dtype not in _FLOATS:
         raise TypeError(f"{what}: f32 or bf16, not {x.dtype}")
-    _on_gpu(x.device)
+    if not x.is_cuda:
+        _on_gpu(x.device)
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{what}: MXFP4 has no gradient; call it under torch.no_grad()")
 
@@ -200,7 +201,8 @@ def linear(x, w, bias=None, relu=False, out_dtype=None, out=None):
             lead = x.shape[:-1]
             x = x.reshape(-1, x.shape[-1])
         _rows2d(x, "linear")
-    _on_gpu(x.device)
+    else:
+        _on_gpu(x.device)
     rows, width = x.shape
     N, dev = w.rows, x.device
     if width != w.cols or dev != w.device:
@@ -215,13 +217,18 @@ def linear(x, w, bias=None, relu=False, out_dtype=None, out=None):
     if out is None:
         if out_dtype is None:
             out_dtype = torch.bfloat16 if four_in else x.dtype
-        out = MX4.empty(rows, N, dev) if out_dtype == "mx4" else torch.empty((rows, N), dtype=out_dtype, device=dev)
+        four_out, ldc = out_dtype == "mx4", N
+        out = MX4.empty(rows, N, dev) if four_out else torch.empty((rows, N), dtype=out_dtype, device=dev)
     elif tuple(out.shape) != (rows, N) or out.device != dev or lead is not None:
         raise ValueError(f"linear: out is {tuple(out.shape)} on {out.device}, the result is {(rows, N)} on {dev}")
     else:
         _apart("linear", out, x, w, *([] if bias is None else [bias.view(1, N)]))
-    four_out = isinstance(out, MX4)
-    if not four_out and (out.dtype not in _FLOATS or (N > 1 and out.stride(1) != 1)):
+        four_out = isinstance(out, MX4)
+        if not four_out:
+            if N > 1 and out.stride(1) != 1:
+                raise TypeError("linear: out in f32 or bf16 with contiguous rows")
+            ldc = _row_stride(out, "linear")
+    if not four_out and out.dtype not in _FLOATS:
         raise TypeError("linear: out in f32 or bf16 with contiguous rows")
     code, x4 = 0, x if four_in else None
     if not four_in:
@@ -236,5 +243,5 @@ def linear(x, w, bias=None, relu=False, out_dtype=None, out=None):
                  C.byref(out.c), b, act)
         return out
     K.launch("llp_gemm_nt_mx4", dev, rows, N, width, code, op, c4, C.byref(w.c),
-             out.data_ptr(), _row_stride(out, "linear"), K.dtype_code(out.dtype), None, b, act)
+             out.data_ptr(), ldc, K.dtype_code(out.dtype), None, b, act)
     return out if lead is None else out.reshape(*lead, N)
