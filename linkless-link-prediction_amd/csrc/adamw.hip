@@ -195,13 +195,15 @@ __device__ __forceinline__ void store_copy(const llp_adamw_desc& d, int64_t e, i
     else store8<ONCE>((float*)d.copy, e, n, p);
     return;
   }
+  int64_t c = e % d.cols, at = e / d.cols * d.copy_ld + c;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     if (i < n) {
-      const int64_t at = (e + i) / d.cols * d.copy_ld + (e + i) % d.cols;
       if (d.copy_dtype == LLP_BF16) ((bf16_t*)d.copy)[at] = f2bf(p[i]);
       else ((float*)d.copy)[at] = p[i];
     }
+    ++at;
+    if (++c == d.cols) c = 0, at += d.copy_ld - d.cols;
   }
 }
 
