@@ -16,10 +16,11 @@
 // The update of p uses m' and v' before they are rounded.
 //
 // Bound by memory: per element 8 B of p, 4 (2) of g, and 16 B of f32 moments or 4.1 B of 8-bit ones.  34 M f32
-// elements with a bf16 copy: 200 us at 5.1 TB/s with f32 moments, 1e8 with 8-bit ones 342 us at 5.3 TB/s (a large copy
-// reaches 4.8); 500,000 elements 5.0 and 5.6 us, where the launch is what counts.
+// elements with a bf16 copy, into other buffers: 190 us at 5.4 TB/s with f32 moments; 1e8 in place 548 us (5.5 TB/s), with
+// 8-bit moments 340 us (5.3 TB/s; a large copy reaches 4.8); 500,000 elements 5.0 and 5.6 us, where the launch is what counts.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "llp_common.h"
@@ -110,10 +111,9 @@ __device__ __forceinline__ void load_codes(const uint8_t* p, int64_t e, int n, u
       if (i < n) w[i >> 2] |= (uint32_t)p[e + i] << (8 * (i & 3));
   }
 }
-template <bool ONCE>
 __device__ __forceinline__ void store_codes(uint8_t* p, int64_t e, int n, const uint32_t (&w)[2]) {
   if (n == 8) {
-    store_as<ONCE>(p + e, u2_any1{w[0], w[1]});
+    *reinterpret_cast<u2_any1*>(p + e) = u2_any1{w[0], w[1]};
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -296,8 +296,8 @@ __global__ __launch_bounds__(256) void adamw_kernel(const llp_adamw_desc* __rest
       }
       if (sm == 255u) cm[0] = cm[1] = 0;
       if (sr == 255u) cr[0] = cr[1] = 0;
-      store_codes<ONCE>((uint8_t*)d.exp_avg_out, e, n, cm);
-      store_codes<ONCE>((uint8_t*)d.exp_avg_sq_out, e, n, cr);
+      store_codes((uint8_t*)d.exp_avg_out, e, n, cm);
+      store_codes((uint8_t*)d.exp_avg_sq_out, e, n, cr);
       if (n && (threadIdx.x & 3) == 0) {
         d.exp_avg_scale_out[e >> 5] = (uint8_t)sm;
         d.exp_avg_sq_scale_out[e >> 5] = (uint8_t)sr;
@@ -382,9 +382,13 @@ extern "C" int llp_adamw_step(const llp_adamw_desc* descs, int n_tensors, const 
   if (n_work == 0) return LLP_OK;
   LLP_CHECK_ARG(descs && work && step, "llp_adamw_step: null pointer");
   const AdamWArgs a{lr, beta1, beta2, eps, weight_decay, max_norm, seed};
+  // Large steps: params, gradients and copies pass by the caches, which the moments then keep to themselves.  f32 moments
+  // of more than 16 M elements, with a workgroup for every item: 2e7 elements 107 -> 94 us, 4e7 236 -> 214, 1e8 589 -> 548 (1e7
+  // would go from 46 to 50).  8-bit ones of more than 32 M, in 4,096 workgroups as always, for the step's constants and the
+  // rounding take longer (1e8 340, one an item 347): 4e7 148 -> 138, 1e8 367 -> 340 (2e7 would go from 64 to 70).
+  const unsigned grid = state_bits == 32 && n_work > 8192 ? (unsigned)std::min<int64_t>(n_work, 1 << 20) : aw_grid(n_work);
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(aw_grid(n_work)), dim3(256), 0, (hipStream_t)stream, descs, work, n_work, sumsq, a,
-                       step);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, descs, work, n_work, sumsq, a, step);
   };
   auto types = [&](auto bits, auto once) {
     constexpr int B = bits;
@@ -394,9 +398,7 @@ extern "C" int llp_adamw_step(const llp_adamw_desc* descs, int n_tensors, const 
   };
   constexpr std::integral_constant<int, 32> b32{};
   constexpr std::integral_constant<int, 8> b8{};
-  // 8-bit steps of more than 32 M elements (580 MB, twice the last-level cache) pass by the caches: 4e7 elements 148 -> 138 us,
-  // 1e8 367 -> 342; 2e7 would go from 64 to 69.  With f32 moments it only costs (1e8 / 2.8: 200 -> 210).
-  if (state_bits == 32) types(b32, std::false_type{});
+  if (state_bits == 32) n_work > 8192 ? types(b32, std::true_type{}) : types(b32, std::false_type{});
   else if (n_work >= 16384) types(b8, std::true_type{});
   else types(b8, std::false_type{});
   LLP_LAUNCH_CHECK();

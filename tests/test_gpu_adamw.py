@@ -531,3 +531,24 @@ def test_two_tables_on_two_streams():
         torch.cuda.synchronize()
         got.append([t for _, ts in tabs for t in ts])
     assert all(torch.equal(x, y) for x, y in zip(*got))
+
+
+def test_adamw_f32_large_tensor():
+    """Past 16 M elements: slices of one tensor, its ends among them."""
+    o = _opt()
+    n = (1 << 24) + 2053
+    gen = torch.Generator(device=DEV).manual_seed(13)
+    p, m = (torch.randn(n, device=DEV, generator=gen) for _ in "pm")
+    g, v = 1e-3 * torch.randn(n, device=DEV, generator=gen), torch.rand(n, device=DEV, generator=gen) * 1e-6
+    copy = torch.empty(n, dtype=torch.bfloat16, device=DEV)
+    tab = o.AdamWTable([p], [g], [m], [v], copies=[copy])
+    at = [slice(0, 4096), slice(n // 2, n // 2 + 4096), slice(n - 4096, n)]
+    before = [[_f64(t[s]) for t in (p, g, m, v)] for s in at]
+    tab.step(torch.full((1,), 6, dtype=torch.int64, device=DEV), **HYPER)
+    for s, (p0, g0, m0, v0) in zip(at, before):
+        rp, rm, rv = Q.adamw(p0, g0, m0, v0, 7, HYPER["lr"], HYPER["betas"], HYPER["eps"], HYPER["weight_decay"])
+        terms = 0.9 * np.abs(m0) + 0.1 * np.abs(g0)
+        upd = HYPER["lr"] / (1 - 0.9 ** 7) * terms / (np.sqrt(rv) / np.sqrt(1 - 0.999 ** 7) + 1e-8)
+        assert (np.abs(_f64(p[s]) - rp) <= 3 * U * np.abs(p0) + 24 * U * upd).all()
+        assert (np.abs(_f64(m[s]) - rm) <= 8 * U * terms).all() and (np.abs(_f64(v[s]) - rv) <= 13 * U * rv).all()
+    assert torch.equal(copy, p.bfloat16())
