@@ -636,6 +636,8 @@ int llp_refresh_shadows(const llp_tensor_desc* descs, int n_tensors, int64_t max
  *   496, 2^-10 apart below 2^-6).  Rounding is stochastic and keeps the means of m and v: one 16-bit
  *   draw per element, half (e mod 2) of word (e mod 8) / 2 of the Philox block e / 8 in stream
  *   65536 t + (the tensor's index in the table) with key `seed`; byte-swapped for exp_avg_sq.
+ *   Where v > 0 its code is at least 1 (v read back as 0 beside an m that is not would make the next
+ *   update m / eps); below the least code's square the mean of v grows by less than that square.
  *   The same seed, step and inputs give the same bits.
  * work: n_work (tensor, item) int32 pairs, each tensor's items 0 .. llp_adamw_work_items(numel) - 1.
  * llp_adamw_values: 8-bit moments (of the *_out buffers) as the values m and v they stand for, f32 or

@@ -8,11 +8,14 @@
 // k + 127; 255 = the block holds a NaN or an infinity): m is kept as E4M3 codes, r = sqrt(v) as unsigned codes of
 // 4 exponent and 4 mantissa bits (bias 7, largest 496, no NaN code).  k is the least power that
 // holds the block's largest value (448 / 496 times 2^k), so nothing saturates.  The root is what is kept because
-// its range is half of v's in exponents: 2^-10 .. 496 beside the block's largest covers 2^38 of v.
+// its range is half of v's in exponents: codes of 2^-10 .. 496 are v over 2^38 within a block.
 // Rounding is stochastic, from one 16-bit Philox draw per element, and keeps the MEAN of m and of
-// v = r^2 (not of r, whose square would grow by the rounding's variance, up to 0.4 % a step, against
-// a decay of 1 - b2 = 0.1 %).  Rounding to nearest would do worse still: a step changes v by 0.1 %,
+// v = r^2 (not of r, whose square would grow by the rounding's variance, up to 0.1 % a step, as much as
+// its decay of 1 - b2 = 0.1 %).  Rounding to nearest would do worse still: a step changes v by 0.1 %,
 // a code is 3 to 6 % wide, and v would never move down.
+// One exception: where v' > 0 the code of r is at least 1.  A root rounded to 0 beside a first moment that is not would make the
+// next update m' / eps (with gradient sizes log-normal of sigma 2 within a block, 5 % of them at a time, single updates of 230 lr;
+// 1.7 lr with the least code, 1.2 lr in f32).  The mean of v below the least code's square grows by less than that square.
 // The update of p uses m' and v' before they are rounded.
 //
 // Bound by memory: per element 8 B of p, 4 (2) of g, and 16 B of f32 moments or 4.1 B of 8-bit ones.  34 M f32
@@ -174,8 +177,8 @@ __device__ __forceinline__ uint32_t round_m(float y, uint32_t w) {
   const uint32_t c = ((t + (((w ^ 0xFFFFu) << 4) | 7u)) >> 20) - (sub ? 968u : 960u);
   return c | ((__float_as_uint(y) >> 24) & 0x80u);
 }
-// r (y = r 2^-k <= 496, x = v 2^-2k) to a code, up where u < (x - lo^2) / (hi^2 - lo^2)
-__device__ __forceinline__ uint32_t round_r(float y, float x, uint32_t w) {
+// r (y = r 2^-k <= 496, x = v 2^-2k) to a code, up where u < (x - lo^2) / (hi^2 - lo^2), at least `least`
+__device__ __forceinline__ uint32_t round_r(float y, float x, uint32_t w, uint32_t least) {
   const bool sub = y < 0x1p-6f;
   const float off = sub ? 0x1p-6f : 0.f;
   const uint32_t t = __float_as_uint(y + off) & 0xFFF80000u;
@@ -184,6 +187,7 @@ __device__ __forceinline__ uint32_t round_r(float y, float x, uint32_t w) {
   const float u = fmaf((float)w, 0x1p-16f, 0x1p-17f);
   uint32_t c = (t >> 19) - (sub ? 1936u : 1920u);
   c += u * den < num ? 1u : 0u;
+  c = c < least ? least : c;
   return c > 255u ? 255u : c;
 }
 
@@ -292,7 +296,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(const llp_adamw_desc* __rest
         const uint32_t x = u4_word(draw, i >> 1) >> (16 * (i & 1)) & 0xFFFFu;
         const uint32_t y = (x >> 8) | ((x & 0xFFu) << 8);
         cm[i >> 2] |= round_m(m[i] * im, x) << (8 * (i & 3));
-        cr[i >> 2] |= round_r(r[i] * ir, (v[i] * ir) * ir, y) << (8 * (i & 3));
+        cr[i >> 2] |= round_r(r[i] * ir, (v[i] * ir) * ir, y, v[i] > 0.f ? 1u : 0u) << (8 * (i & 3));
       }
       if (sm == 255u) cm[0] = cm[1] = 0;
       if (sr == 255u) cr[0] = cr[1] = 0;

@@ -2,7 +2,8 @@
 
 ``AdamW`` is a torch.optim.Optimizer: torch.optim.AdamW's update (decoupled weight decay) in one launch
 for each parameter group, ``state_bits=8`` with block-scaled moments of 8.25 bits a value, rounded
-stochastically so that their means are kept.  The training engines take it in place of
+stochastically so that their means are kept (the second moment's down to its block's least code, which a
+positive one never falls below).  The training engines take it in place of
 torch.optim.Adam (src/main.py:400-402).  ``AdamWTable`` is the step itself over lists of tensors, in
 place or into other buffers.
 """

@@ -110,8 +110,8 @@ def scales8(size, signed):
 
 
 def round8(x, w, scales, signed):
-    """Stochastic rounding of m, or of v held by its root: (codes, how far each draw was from turning the
-    other way, as a share of the distance between the codes)."""
+    """Stochastic rounding of m, or of v held by its root and where positive at least code 1: (codes, how far
+    each draw was from turning the other way, as a share of the distance between the codes)."""
     n = x.size
     f = np.repeat(np.exp2(scales.astype(np.float64) - 127), 32)[:n]
     lv = levels8(signed) if signed else levels8(False) ** 2
@@ -124,6 +124,8 @@ def round8(x, w, scales, signed):
     code = np.where(u < share, i + 1, i)
     if signed:
         code = code + 128 * (np.signbit(x) & (code > 0))
+    else:
+        code = np.where(x > 0, np.maximum(code, 1), code)
     return code.astype(np.uint8), np.abs(u - share)
 
 
