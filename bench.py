@@ -553,7 +553,7 @@ def main():
     torch.cuda.synchronize()
     dt = time.perf_counter() - t0
     if world > 1:
-        t = torch.tensor([dt], device=dev, dtype=torch.float64)
+        t = torch.tensor([dt], device=dev if backend == "nccl" else "cpu", dtype=torch.float64)
         dist.all_reduce(t, op=dist.ReduceOp.MAX)
         dt = float(t.item())
     if opt.profile_kernels:
@@ -570,7 +570,7 @@ def main():
     # dominant kernel: student layer-2 forward GEMM (rows_exec x 1024 x 1024, bf16 MFMA);
     # rows_exec = unique nodes of this rank's student rows
     rows_exec = eng.last_student_rows
-    rows_all = torch.tensor([float(rows_exec)], dtype=torch.float64, device=dev)
+    rows_all = torch.tensor([float(rows_exec)], dtype=torch.float64, device=dev if backend == "nccl" else "cpu")
     if world > 1:
         dist.all_reduce(rows_all)
     if not kern_ev:   # graph mode: time the dominant kernel in a few eager steps after the timed region

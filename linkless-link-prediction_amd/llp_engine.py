@@ -141,6 +141,18 @@ def _acc_dtype(t):
     return t.dtype if t.dtype in (torch.float32, torch.float64) else torch.float32
 
 
+def _all_reduce(t, group=None, async_op=False):
+    """SUM all-reduce of ``t`` in place; the work handle with ``async_op``, where there is one.  gloo is given host
+    memory only (its collectives on device tensors can hang when ranks share a GPU): a device tensor goes there and
+    back by synchronous copies, and nothing is left to wait for."""
+    if t.is_cuda and dist.get_backend(group) == "gloo":
+        host = t.cpu()
+        dist.all_reduce(host, op=dist.ReduceOp.SUM, group=group)
+        t.copy_(host)
+        return None
+    return dist.all_reduce(t, op=dist.ReduceOp.SUM, group=group, async_op=async_op)
+
+
 def _resets_on_error(step):
     """Engine step decorator: a step that raises resets the persistent device state
     (EngineBase.reset_device_state) before the exception propagates."""
@@ -452,7 +464,7 @@ class EngineBase:
                 # the true total over the ranks' shards (BCE normaliser, BatchNorm row count),
                 # not a proportional estimate; injected negatives are host-known (no capture)
                 t = torch.tensor([n_neg], dtype=torch.int64, device=self.device)
-                dist.all_reduce(t, op=dist.ReduceOp.SUM, group=self.group)
+                _all_reduce(t, self.group)
                 n_neg_total = int(t.item())
             else:   # one rank, or an emulated shard (timing): proportional to the link slice
                 n_neg_total = n_neg if P_total == P else int(round(n_neg * P_total / max(P, 1)))
@@ -657,7 +669,7 @@ class EngineBase:
             sums = self._buf(f"nsum_{tag}", (2, H), torch.float64)
             K.norm_colsums(y, sums, self._ws("ws_norm", K.norm_ws_bytes(M, H)))
             if sync and self.world > 1:
-                self._collective(lambda: dist.all_reduce(sums, op=dist.ReduceOp.SUM, group=self.group))
+                self._collective(lambda: _all_reduce(sums, self.group))
         m = nm.m
         K.norm_fwd(nm.kind, y, out, stats, nm.gamma(), nm.beta(), nm.eps, training, sums, count, nm.momentum,
                    getattr(m, "running_mean", None), getattr(m, "running_var", None),
@@ -676,7 +688,7 @@ class EngineBase:
                         dgamma=None if m.weight is None else m.weight.grad,
                         dbeta=None if m.bias is None else m.bias.grad, rows=rows)
         if nm.batch and sync and self.world > 1:
-            self._collective(lambda: dist.all_reduce(sums, op=dist.ReduceOp.SUM, group=self.group))
+            self._collective(lambda: _all_reduce(sums, self.group))
         K.norm_bwd(nm.kind, gout, out, alpha, y, stats, gy, nm.gamma(), sums, count, rows=rows)
 
     def _allreduce_tail_begin(self):
@@ -690,8 +702,7 @@ class EngineBase:
         are final (stream order); the rest of flat_grad goes in _finish_allreduce."""
         if self.world > 1 and hi > lo and all(hi <= a or lo >= b for a, b in self._issued):
             self._issued.append((lo, hi))
-            self._collective(lambda: self._works.append(
-                dist.all_reduce(self.flat_grad[lo:hi], op=dist.ReduceOp.SUM, group=self.group, async_op=True)))
+            self._collective(lambda: self._works.append(_all_reduce(self.flat_grad[lo:hi], self.group, async_op=True)))
 
     def _grad_slice(self, *params):
         """[lo, hi) of the given parameters' gradients in flat_grad (contiguous)."""
@@ -705,9 +716,10 @@ class EngineBase:
         """All-reduce the ranges not yet issued (``rest``), then make the stream
         wait for every bucket (stream-ordered: no host block on RCCL)."""
         for lo, hi in rest:
-            dist.all_reduce(self.flat_grad[lo:hi], op=dist.ReduceOp.SUM, group=self.group)
+            _all_reduce(self.flat_grad[lo:hi], self.group)
         for w in self._works:
-            w.wait()
+            if w is not None:
+                w.wait()
         self._works = []
 
     def _collective(self, fn):
@@ -867,7 +879,7 @@ class EngineBase:
         # instead of leaving the others to hang in the next epoch's collectives
         tot = torch.stack([self.loss_sum.view(()), self._device_error_flag()])
         if self.world > 1:
-            dist.all_reduce(tot, group=self.group)
+            _all_reduce(tot, self.group)
         self.check_device_errors(flag=tot[1])
         steps = int(self.adam_step.item())
         for p in self.all_params:
@@ -1631,10 +1643,10 @@ class DistillEngine(EngineBase):
             full.view(world, *part.shape).copy_(part.unsqueeze(0).expand(world, *part.shape))
         elif dist.get_backend(self.group) == "nccl":
             dist.all_gather_into_tensor(full, part, group=self.group)
-        else:   # gloo (CPU rehearsal / tests): all_reduce is its one CUDA collective; exact in f32
+        else:   # gloo (rehearsal, tests): through _all_reduce, which stages device tensors on the host; exact in f32
             t = torch.zeros(full.shape, dtype=_acc_dtype(full), device=full.device)
             t.view(self.world, *part.shape)[self.rank].copy_(part)
-            dist.all_reduce(t, op=dist.ReduceOp.SUM, group=self.group)
+            _all_reduce(t, self.group)
             full.copy_(t)
 
     def _reduce_scatter_rows(self, part, full, world, rank):
@@ -1645,7 +1657,7 @@ class DistillEngine(EngineBase):
             dist.reduce_scatter_tensor(part, full, op=dist.ReduceOp.SUM, group=self.group)
         else:
             t = full.to(_acc_dtype(full))
-            dist.all_reduce(t, op=dist.ReduceOp.SUM, group=self.group)
+            _all_reduce(t, self.group)
             part.copy_(t.view(self.world, *part.shape)[self.rank])
 
     def capture_minibatch(self, anchors, link_ids, pairs, segmented=None, debug_cuts=False, mode="thread_local",
