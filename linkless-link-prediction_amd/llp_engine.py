@@ -463,7 +463,7 @@ class EngineBase:
             if self.world > 1:
                 # the true total over the ranks' shards (BCE normaliser, BatchNorm row count),
                 # not a proportional estimate; injected negatives are host-known (no capture)
-                t = torch.tensor([n_neg], dtype=torch.int64, device=self.device)
+                t = torch.tensor([n_neg], dtype=torch.int64, device=self.dev)
                 _all_reduce(t, self.group)
                 n_neg_total = int(t.item())
             else:   # one rank, or an emulated shard (timing): proportional to the link slice
