@@ -927,6 +927,23 @@ def descs_to_device(descs, device):
     return host.to(device)
 
 
+def rows_meet(a, b):
+    """Whether two sets of rows share a byte; each is (first byte, rows, bytes from row to row, bytes of a row), the
+    rows of a set apart from one another."""
+    if min(a[1], a[3], b[1], b[3]) <= 0:
+        return False
+    # one piece where the rows follow each other
+    a, b = ((p, 1, n * w, n * w) if n == 1 or s == w else (p, n, s, w) for p, n, s, w in (a, b))
+    (pa, na, sa, wa), (pb, nb, sb, wb) = (a, b) if a[1] <= b[1] else (b, a)
+
+    def between(at, most, least):
+        """A row j of b in least..most that meets [at, at + wa): pb + j sb < at + wa and at < pb + j sb + wb."""
+        return max((at - wb - pb) // sb + 1, least) <= min(-(-(at + wa - pb) // sb) - 1, most)
+    if na > 1 and sa == sb:        # (row i of a meets row j of b as row 0 would meet row j - i)
+        return between(pa, nb - 1, 1 - na)
+    return any(between(pa + i * sa, nb - 1, 0) for i in range(na))
+
+
 def launch(what, dev, *args):
     """Entry point ``what`` with ``args`` and the current stream of ``dev``, with ``dev`` the current device (a
     kernel launches on the current device; the tensors may live on another)."""

@@ -9,6 +9,8 @@ place or into other buffers.
 """
 from __future__ import annotations
 
+import bisect
+
 import numpy as np
 import torch
 
@@ -178,35 +180,58 @@ class AdamWTable:
     @staticmethod
     def _apart(ins, outs, grads, copies, copies_t, values):
         """What a step writes overlaps nothing else that it reads or writes but its own input in place."""
-        spans = []
+        spans, strided = [], []      # (first byte, byte past the last, written); rows of copies with a stride, likewise
 
-        def add(t, write, own):
-            if t is not None and t.numel():
+        def add(t, write):
+            if t.numel():
                 lo = t.data_ptr()
-                spans.append((lo, lo + t.numel() * t.element_size(), write, own))
+                spans.append((lo, lo + t.numel() * t.element_size(), write))
 
         for k in ins:
-            for i, (a, b) in enumerate(zip(ins[k], outs[k])):
+            for a, b in zip(ins[k], outs[k]):
                 if a.data_ptr() == b.data_ptr():
-                    add(a, True, None)
+                    add(a, True)
                 else:
-                    add(a, False, None)
-                    add(b, True, None)
+                    add(a, False)
+                    add(b, True)
         for t in grads:
-            add(t, False, None)
-        for t, ld in copies + copies_t:
-            if not ld:
-                add(t, True, None)
+            add(t, False)
+        for ts, turned in ((copies, False), (copies_t, True)):
+            for p, (t, ld) in zip(ins["params"], ts):
+                if t is None:
+                    continue
+                rows, cols = (p.shape[0], p.shape[1]) if p.dim() == 2 else (1, p.numel())
+                rows, cols = (cols, rows) if turned else (rows, cols)
+                if not ld:
+                    add(t, True)
+                elif rows and cols:
+                    strided.append((t.data_ptr(), rows, ld * t.element_size(), cols * t.element_size()))
         for ts in (values or {}).values():
             for t in ts:
-                add(t, True, None)
+                add(t, True)
         spans.sort()
-        end, wrote = 0, 0       # the furthest ends of what was seen, read or written
-        for lo, hi, write, _ in spans:
+        clash = ValueError("AdamWTable: a buffer that the step writes overlaps another one")
+        end, wrote, ends = 0, 0, []       # the furthest ends of what was seen, read or written
+        for lo, hi, write in spans:
             if lo < wrote or (write and lo < end):
-                raise ValueError("AdamWTable: a buffer that the step writes overlaps another one")
+                raise clash
             end = max(end, hi)
             wrote = max(wrote, hi) if write else wrote
+            ends.append(end)
+        # the rows of each strided copy against the pieces within its span, and against the copies before it
+        strided.sort()
+        before = []
+        for rows in strided:
+            lo, hi = rows[0], rows[0] + (rows[1] - 1) * rows[2] + rows[3]
+            i = bisect.bisect_left(spans, (hi,)) - 1
+            while i >= 0 and ends[i] > lo:
+                if K.rows_meet(rows, (spans[i][0], 1, 1, spans[i][1] - spans[i][0])):
+                    raise clash
+                i -= 1
+            before = [(h, r) for h, r in before if h > lo]
+            if any(K.rows_meet(rows, r) for _, r in before):
+                raise clash
+            before.append((hi, rows))
 
     def step(self, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, sumsq=None, max_norm=1.0, seed=0):
         """One update, number *step + 1 (``step``: int64 device scalar, read and not advanced).  sumsq (f32,
