@@ -98,25 +98,28 @@ def _row_stride(out, what):
 
 
 def _spans(t):
-    """Where the rows of a matrix lie: [(first byte, byte past the last)]."""
+    """Where the rows of a matrix lie: [(first byte, rows, bytes from row to row, bytes of a row)]."""
     rows, cols = t.shape
     if not rows:
         return []
     if isinstance(t, MX4):
         p = _pad(cols)
-        return [(t.c.codes, t.c.codes + (rows - 1) * t.c.ld_codes + p // 2),
-                (t.c.scales, t.c.scales + (rows - 1) * t.c.ld_scales + p // 32)]
-    at, size = t.data_ptr(), t.element_size()
-    return [(at, at + ((rows - 1) * t.stride(0) + cols) * size)]
+        at = [(t.c.codes, rows, t.c.ld_codes, p // 2), (t.c.scales, rows, t.c.ld_scales, p // 32)]
+    else:
+        size = t.element_size()
+        at = [(t.data_ptr(), rows, (t.stride(0) if rows > 1 else cols) * size, cols * size)]
+    # rows that overlap one another, as an expanded tensor's: one piece
+    return [(a, n, s, w) if s >= w else (a, 1, 1, (n - 1) * s + w) for a, n, s, w in at]
 
 
 def _apart(what, out, *inputs):
     """A given output shares no memory with what the call reads."""
     mine = _spans(out)
+    if len(mine) == 2 and K.rows_meet(*mine):
+        raise ValueError(f"{what}: out's codes and scales overlap")
     for t in inputs:
-        for a, b in _spans(t):
-            if any(a < hi and lo < b for lo, hi in mine):
-                raise ValueError(f"{what}: out overlaps an input")
+        if any(K.rows_meet(a, b) for a in _spans(t) for b in mine):
+            raise ValueError(f"{what}: out overlaps an input")
 
 
 def _on_gpu(dev):
@@ -171,7 +174,7 @@ def quantize(x, idx=None, x2=None, idx2=None, out=None):
     elif out.shape != (rows, x.shape[1]) or out.device != x.device:
         raise ValueError(f"quantize: out is {out.shape} on {out.device}, the rows are {(rows, x.shape[1])} on {x.device}")
     else:
-        _apart("quantize", out, x, *([] if x2 is None else [x2]))
+        _apart("quantize", out, x, *(t if t.dim() == 2 else t.view(1, -1) for t in (idx, x2, idx2) if t is not None))
     K.launch("llp_mx4_quantize", x.device, K.dtype_code(x.dtype), rows, x.shape[1], C.byref(op), C.byref(out.c))
     return out
 

@@ -68,6 +68,50 @@ def test_strided_copies_that_overlap_are_refused():
         _apart([torch.zeros(2, 8), wide[0, 7:19]], [(wide, 20), none])
 
 
+def _mx4(flat, at, rows=10, cols=100, ld_codes=64, ld_scales=4, scales_at=None):
+    p = -(-cols // 128) * 128
+    scales_at = at + rows * ld_codes if scales_at is None else scales_at
+    return llp_mx.MX4(torch.as_strided(flat, (rows, p // 2), (ld_codes, 1), at),
+                      torch.as_strided(flat, (rows, p // 32), (ld_scales, 1), scales_at), cols)
+
+
+def test_mx4_outputs_overlap_no_index():
+    flat = torch.zeros(8192, dtype=torch.uint8)
+    out, x = _mx4(flat, 0), torch.zeros(20, 100)
+    words = flat.view(torch.int32)
+    llp_mx._apart("x", out, x, words[170:180].view(1, -1), words[0:0].view(1, -1))
+    for idx in (words[0:10], words[155:165], words[165:175]):      # codes, codes and scales, scales
+        with pytest.raises(ValueError, match="overlaps"):
+            llp_mx._apart("x", out, x, idx.view(1, -1))
+
+
+def test_quantize_checks_its_indices(monkeypatch):
+    """quantize looks at both index tensors (the checks alone: nothing is launched)."""
+    monkeypatch.setattr(llp_mx, "_rows2d", lambda x, what: None)
+    monkeypatch.setattr(K, "launch", lambda *a: None)
+    flat = torch.zeros(8192, dtype=torch.uint8)
+    out, x, words = _mx4(flat, 0), torch.zeros(20, 100), flat.view(torch.int32)
+    free, bad = words[1000:1010], words[20:30]
+    assert llp_mx.quantize(x, free, x, free, out=out) is out
+    for i, j in ((bad, free), (free, bad)):
+        with pytest.raises(ValueError, match="overlaps"):
+            llp_mx.quantize(x, i, x, j, out=out)
+    with pytest.raises(ValueError, match="overlaps"):
+        llp_mx.quantize(x, bad, out=out)
+
+
+def test_mx4_codes_and_scales_of_an_output_are_apart():
+    flat = torch.zeros(8192, dtype=torch.uint8)
+    x = torch.zeros(20, 100)
+    llp_mx._apart("x", _mx4(flat, 0, ld_codes=80, ld_scales=80, scales_at=64), x)      # side by side in rows of 80 bytes
+    for at in (60, 636):
+        with pytest.raises(ValueError, match="codes and scales overlap"):
+            llp_mx._apart("x", _mx4(flat, 0, scales_at=at), x)
+    row = torch.zeros(1, 100).expand(20, 100)                                          # an input that is one row in memory
+    llp_mx._apart("x", _mx4(flat, 0), row)
+    llp_mx._apart("x", row, _mx4(flat, 0))                                             # (its own rows: _row_stride)
+
+
 def test_many_tensors():
     ps = [torch.zeros(2, 4) for _ in range(2000)]
     wide, own = torch.zeros(2, 4 * 100), [torch.zeros(2, 6) for _ in range(1900)]
