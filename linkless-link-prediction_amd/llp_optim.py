@@ -339,8 +339,10 @@ class AdamW(torch.optim.Optimizer):
             grads = [p.grad for p in params]
             if any(g.is_sparse for g in grads):
                 raise RuntimeError("AdamW: dense gradients only")
-            where = tuple((p.data_ptr(), g.data_ptr(), p.numel(), p.dtype, g.dtype,
-                           self.init_state(p)["exp_avg"].data_ptr()) for p, g in zip(params, grads))
+            # all that the table took from these tensors: where they and the moments lie, types and layouts
+            where = tuple((p.data_ptr(), g.data_ptr(), p.numel(), p.dtype, g.dtype, p.is_contiguous(), g.is_contiguous(),
+                           *(t.data_ptr() for k, t in self.init_state(p).items() if k != "step"))
+                          for p, g in zip(params, grads))
             at = self._tables.get(i)
             capturing = params[0].is_cuda and torch.cuda.is_current_stream_capturing()
             if at is None or at[0] != where:
