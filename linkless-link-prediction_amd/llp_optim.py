@@ -274,7 +274,8 @@ def from_args(args, params):
 
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW on the HIP step: ``lr``, ``betas``, ``eps``, ``weight_decay`` as there (no amsgrad,
-    no maximize); ``state_bits`` 32 or 8; ``seed`` of the 8-bit moments' rounding.
+    no maximize: groups and checkpoints that ask for them are refused); ``state_bits`` 32 or 8; ``seed`` of the
+    8-bit moments' rounding.
 
     Params in f32 or bf16 on the GPU, dense gradients of one dtype in a group.  ``state[p]`` holds
     ``step`` and exp_avg / exp_avg_sq (f32, or uint8 codes with exp_avg_scale / exp_avg_sq_scale; a NaN or
@@ -293,6 +294,19 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.seed = int(state_bits), int(seed)
         self._tables = {}      # per group: (addresses, table, device step counter, params)
         self._counters, self._captured = {}, []
+
+    @staticmethod
+    def _known(group):
+        """A group asks for nothing that the step does not do."""
+        for name in ("amsgrad", "maximize"):
+            if group.get(name):
+                raise ValueError(f"AdamW: no {name}")
+        if group.get("weight_decay") and not group.get("decoupled_weight_decay", True):
+            raise ValueError("AdamW: the decay is decoupled (the group's is Adam's)")
+
+    def add_param_group(self, param_group):
+        self._known(param_group)
+        super().add_param_group(param_group)
 
     def __getstate__(self):
         self._sync_steps()
@@ -382,6 +396,12 @@ class AdamW(torch.optim.Optimizer):
         return super().state_dict()
 
     def load_state_dict(self, state_dict):
+        # (all looked at before anything is taken over)
+        for group in state_dict["param_groups"]:
+            self._known(group)
+        for st in state_dict["state"].values():
+            if "exp_avg" in st and ("exp_avg_scale" in st) != (self.state_bits == 8):
+                raise ValueError(f"AdamW: the loaded moments are not in {self.state_bits} bits")
         super().load_state_dict(state_dict)
         self._tables = {}
         # the base class casts state to the param's dtype: the moments are taken over as they are
@@ -391,5 +411,3 @@ class AdamW(torch.optim.Optimizer):
             if k in state_dict["state"]:
                 for name, v in state_dict["state"][k].items():
                     self.state[p][name] = v.detach().clone() if name == "step" else v.detach().clone().to(p.device)
-                if ("exp_avg_scale" in self.state[p]) != (self.state_bits == 8):
-                    raise ValueError(f"AdamW: the loaded moments are not in {self.state_bits} bits")

@@ -63,3 +63,41 @@ def test_replaced_state_is_another_table(tables, bits):
         opt.step()
         assert len(tables) == 2 + n, name
     assert float(opt.state_dict()["state"][0]["step"]) == 1 + 2 * (len(opt.state[p]) - 1)
+
+
+def _stepped(cls, **kw):
+    p = torch.nn.Parameter(torch.randn(4, 3))
+    p.grad = torch.randn(4, 3)
+    opt = cls([p], **kw)
+    opt.step()
+    return opt.state_dict()
+
+
+def test_checkpoints_that_ask_for_more_are_refused():
+    p = torch.nn.Parameter(torch.randn(4, 3))
+    opt = llp_optim.AdamW([p], lr=0.5)
+    for sd, why in ((_stepped(torch.optim.AdamW, amsgrad=True), "amsgrad"), (_stepped(torch.optim.AdamW, maximize=True), "maximize"),
+                    (_stepped(torch.optim.Adam, weight_decay=0.1), "decoupled")):
+        with pytest.raises(ValueError, match=why):
+            opt.load_state_dict(sd)
+    eight = llp_optim.AdamW([p], state_bits=8, lr=0.5)
+    with pytest.raises(ValueError, match="8 bits"):
+        eight.load_state_dict(_stepped(torch.optim.AdamW))
+    for o in (opt, eight):               # nothing was taken over
+        assert not o.state and o.param_groups[0]["lr"] == 0.5 and "amsgrad" not in o.param_groups[0]
+    opt.load_state_dict(_stepped(torch.optim.AdamW, lr=0.25))
+    assert opt.param_groups[0]["lr"] == 0.25 and float(opt.state[p]["step"]) == 1
+    opt.load_state_dict(_stepped(torch.optim.Adam))      # (no decay: the same update)
+    empty = torch.optim.AdamW([p]).state_dict()
+    opt.load_state_dict(empty), eight.load_state_dict(empty)
+
+
+@pytest.mark.parametrize("name", ["amsgrad", "maximize"])
+def test_groups_that_ask_for_more_are_refused(name):
+    a, b = (torch.nn.Parameter(torch.zeros(3)) for _ in "ab")
+    with pytest.raises(ValueError, match=name):
+        llp_optim.AdamW([{"params": [a], name: True}])
+    opt = llp_optim.AdamW([{"params": [a], name: False}])
+    with pytest.raises(ValueError, match=name):
+        opt.add_param_group({"params": [b], name: True})
+    assert len(opt.param_groups) == 1
