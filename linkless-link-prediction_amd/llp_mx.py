@@ -10,7 +10,7 @@ inverse and the product, on the hand-written kernels of csrc/mx4.hip.
 Each 32 consecutive values of a row share a power of two; a value is a 4-bit code (0, 0.5, 1, 1.5, 2, 3,
 4, 6 and a sign) to nearest, ties to even, saturated at 6.  A block with a NaN or an infinity reads as
 NaN.  Products are exact and summed in f32.  There is no gradient: under autograd, with an input that
-requires one, the calls raise.  Replaces nn.Linear + ReLU of MLP / LinkPredictor in evaluation
+requires one, the calls raise, and with a dual tensor of forward mode.  Replaces nn.Linear + ReLU of MLP / LinkPredictor in evaluation
 (src/models.py:45-54,139-150); used by llp_eval with dtype "mxfp4".
 """
 from __future__ import annotations
@@ -18,6 +18,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 import llp_hip as K
 
@@ -127,6 +128,14 @@ def _on_gpu(dev):
         raise RuntimeError("LLP ops run only on the MI355X HIP device (got a CPU tensor; no CPU fallback)")
 
 
+def _no_gradient(t, what):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{what}: MXFP4 has no gradient; call it under torch.no_grad()")
+    # (the tangent of a dual tensor, which torch.no_grad() leaves on; outside of every dual level there is none)
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"{what}: MXFP4 has no gradient, forward mode neither; unpack the dual tensor")
+
+
 def _rows2d(x, what):
     if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
         raise ValueError(f"{what}: a 2-D tensor with contiguous rows")
@@ -134,8 +143,7 @@ def _rows2d(x, what):
         raise TypeError(f"{what}: f32 or bf16, not {x.dtype}")
     if not x.is_cuda:
         _on_gpu(x.device)
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{what}: MXFP4 has no gradient; call it under torch.no_grad()")
+    _no_gradient(x, what)
 
 
 def _index(i, x, what):
@@ -211,8 +219,7 @@ def linear(x, w, bias=None, relu=False, out_dtype=None, out=None):
     if width != w.cols or dev != w.device:
         raise ValueError(f"linear: x has {width} columns on {dev}, w has {w.cols} on {w.device}")
     if bias is not None:
-        if bias.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("linear: MXFP4 has no gradient; call it under torch.no_grad()")
+        _no_gradient(bias, "linear")
         if bias.shape != (N,) or bias.device != dev:
             raise ValueError(f"linear: bias of {N} values on {dev}")
         if bias.dtype != torch.float32 or not bias.is_contiguous():
