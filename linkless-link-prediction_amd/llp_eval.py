@@ -34,6 +34,12 @@ def _as_pairs(edges: torch.Tensor) -> torch.Tensor:
     return edges.to(torch.int32).contiguous()
 
 
+def _mx_weight(lin):
+    """A layer's weight in MXFP4 (through f32 where it is in another type than f32 / bf16)."""
+    w = lin.weight.detach()
+    return llp_mx.quantize((w if w.dtype in (torch.float32, torch.bfloat16) else w.float()).contiguous())
+
+
 class EdgeScorer:
     """predictor(h[e0], h[e1]) (src/models.py:139-150) in eval mode."""
 
@@ -46,7 +52,7 @@ class EdgeScorer:
 
     def _weights(self):
         lins = list(self.predictor.lins)
-        hid = [(llp_mx.quantize(l.weight.detach()) if self.mx else l.weight.detach().to(self.dtype).contiguous(),
+        hid = [(_mx_weight(l) if self.mx else l.weight.detach().to(self.dtype).contiguous(),
                 l.bias.detach().float().contiguous()) for l in lins[:-1]]
         head = (lins[-1].weight.detach().float().reshape(-1).contiguous(), lins[-1].bias.detach().float().contiguous())
         return hid, head
@@ -102,7 +108,7 @@ def _embed_mlp_mx(layers, norms, x):
     h = x if x.dtype in (torch.float32, torch.bfloat16) else x.float()
     h = h.contiguous()
     for l, lin in enumerate(layers):
-        W, b = llp_mx.quantize(lin.weight.detach()), lin.bias.detach().float()
+        W, b = _mx_weight(lin), lin.bias.detach().float()
         last = l == len(layers) - 1
         if norms and not last:
             h = llp_mx.linear(h, W, b, out_dtype=torch.bfloat16)
