@@ -41,7 +41,7 @@ DENSE_NEG_STREAM = STREAMS_PER_STEP - 2
 MAX_RW_STEP = STREAMS_PER_STEP - 3          # walks + negatives below DENSE_NEG_STREAM
 # dropout Philox keys (EngineBase._dropout): one per module, one stream per layer and step
 DROP_ENCODER, DROP_PREDICTOR, DROP_TEACHER_PRED = 0, 1, 2
-_ADAMW_KEY = 0xADA << 44      # Philox key of the 8-bit moments' rounding, beside self.seed
+_ADAMW_KEY = 0xADA << 44      # Philox key of the 8-bit moments' rounding, beside self.seed and the optimizer's
 # x at most this dense runs the full-batch student's first layer sparse (llp_spmm_rows): a
 # gathered 512-B weight row per nonzero against a dense 256-wide MFMA pass over every column
 SPARSE_X_MAX_DENSITY = 0.05
@@ -768,7 +768,7 @@ class EngineBase:
         if self.adamw is not None:   # (the gradients stay unclipped: the coefficient is applied as they are read)
             self.adamw.step(self.adam_step, lr=float(g["lr"]), betas=(float(b1), float(b2)), eps=float(g["eps"]),
                             weight_decay=float(g["weight_decay"]), sumsq=self.sumsq, max_norm=1.0,
-                            seed=self.seed ^ _ADAMW_KEY)
+                            seed=self.seed ^ _ADAMW_KEY ^ getattr(self.optimizer, "seed", 0))
             return
         # the one-launch Adam reads the step counter; the step-end launch advances it
         K.adam_step(self.descs_dev, self.n_desc, self.max_numel, self.sumsq, 1.0, float(g["lr"]), float(b1),

@@ -275,7 +275,7 @@ def from_args(args, params):
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW on the HIP step: ``lr``, ``betas``, ``eps``, ``weight_decay`` as there (no amsgrad,
     no maximize: groups and checkpoints that ask for them are refused); ``state_bits`` 32 or 8; ``seed`` of the
-    8-bit moments' rounding.
+    8-bit moments' rounding (the engines mix it into their own; the same on every rank).
 
     Params in f32 or bf16 on the GPU, dense gradients of one dtype in a group.  ``state[p]`` holds
     ``step`` and exp_avg / exp_avg_sq (f32, or uint8 codes with exp_avg_scale / exp_avg_sq_scale; a NaN or
