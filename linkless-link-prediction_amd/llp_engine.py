@@ -325,6 +325,8 @@ class EngineBase:
                 st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
                 st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
             step0 = int(float(st["step"]))
+        if isinstance(opt, llp_optim.AdamW) and any(int(float(opt.state[p]["step"])) != step0 for p in self.all_params):
+            raise ValueError("AdamW: the engine's params must have taken the same number of steps")
         self.adam_step = torch.full((1,), step0, dtype=torch.int64, device=self.dev)
 
     def _build_descs(self):

@@ -25,3 +25,16 @@ def test_the_optimizers_seed_counts(monkeypatch):
         e.adamw = types.SimpleNamespace(step=lambda ctr, seed, **kw: seeds.append(seed))
         e._allreduce_and_update()
     assert len(set(seeds)) == 4 and seeds[0] == 5 ^ llp_engine._ADAMW_KEY
+
+
+def test_params_of_different_age_are_refused():
+    ps = [torch.nn.Parameter(torch.zeros(4)) for _ in range(3)]
+    opt = llp_optim.AdamW(ps)
+    for p in ps:
+        opt.init_state(p)["step"] = torch.tensor(4.0)
+    e = _engine(opt, ps)
+    e._init_optimizer_state()
+    assert int(e.adam_step) == 4
+    opt.state[ps[0]]["step"] = torch.tensor(3.0)
+    with pytest.raises(ValueError, match="same number of steps"):
+        e._init_optimizer_state()
