@@ -377,6 +377,8 @@ class AdamW(torch.optim.Optimizer):
             table.step(ctr, lr=float(group["lr"]), betas=group["betas"], eps=float(group["eps"]),
                        weight_decay=float(group["weight_decay"]), seed=self.seed + (i << 48))
             K.launch("llp_increment", ctr.device, ctr.data_ptr())
+            # written in place, as autograd has to know: a backward through what was saved of them raises
+            torch.autograd.graph.increment_version(params)
         return loss
 
     def hand_over(self):

@@ -101,3 +101,13 @@ def test_groups_that_ask_for_more_are_refused(name):
     with pytest.raises(ValueError, match=name):
         opt.add_param_group({"params": [b], name: True})
     assert len(opt.param_groups) == 1
+
+
+def test_a_step_counts_as_a_write_in_place(tables):
+    """What a forward saved of a param is out of date after the step: backward raises, as after torch's."""
+    w, x = torch.nn.Parameter(torch.randn(3, 3)), torch.randn(3, 3, requires_grad=True)
+    loss = (x @ w).sum()
+    w.grad = torch.randn(3, 3)
+    llp_optim.AdamW([w]).step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
