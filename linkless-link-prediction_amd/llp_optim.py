@@ -140,7 +140,7 @@ class AdamWTable:
         self.n_work, self.n_tiles = sum(items), sum(tiles)
         self._args = (self._descs.data_ptr(), self.n, self._work.data_ptr(), self.n_work)
         self._args_t = (self._descs.data_ptr(), self._work.data_ptr() + 8 * self.n_work, self.n_tiles, self.param_code)
-        self._keep = (ins, outs, grads, copies, copies_t, values)
+        self._keep, self._grads = (ins, outs, copies, copies_t, values), grads
 
     @staticmethod
     def state8(numel, device):
@@ -368,11 +368,12 @@ class AdamW(torch.optim.Optimizer):
                 if len(steps) != 1:
                     raise RuntimeError("AdamW: a group's params must have taken the same number of steps")
                 table = self.table(params, grads)
+                table._grads = None            # p.grad's: zero_grad() frees them
                 ctr = self._counters.setdefault(i, torch.zeros(1, dtype=torch.int64, device=params[0].device))
                 ctr.fill_(int(steps.pop()))
                 at = self._tables[i] = (where, table, ctr, params)
             if capturing:
-                self._captured.append(at)      # a replay reads the table
+                self._captured.append((at, grads))      # a replay reads the table and these gradients
             _, table, ctr, _ = at
             table.step(ctr, lr=float(group["lr"]), betas=group["betas"], eps=float(group["eps"]),
                        weight_decay=float(group["weight_decay"]), seed=self.seed + (i << 48))

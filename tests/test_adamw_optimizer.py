@@ -111,3 +111,28 @@ def test_a_step_counts_as_a_write_in_place(tables):
     llp_optim.AdamW([w]).step()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def test_gradients_are_not_kept(monkeypatch):
+    """zero_grad() lets go of the gradients: the optimizer holds none of them (a captured step's are another matter)."""
+    import weakref
+
+    class Grads(list):
+        pass
+    made = []
+
+    class Table:
+        def __init__(self, params, grads, *a, **kw):
+            self._grads = Grads(grads)
+            made.append(weakref.ref(self._grads))
+
+        def step(self, ctr, **kw):
+            pass
+    Table.state8 = staticmethod(llp_optim.AdamWTable.state8)
+    monkeypatch.setattr(llp_optim, "AdamWTable", Table)
+    monkeypatch.setattr(K, "launch", lambda *a: None)
+    p = torch.nn.Parameter(torch.zeros(4))
+    p.grad = torch.ones(4)
+    opt = llp_optim.AdamW([p])
+    opt.step()
+    assert len(made) == 1 and made[0]() is None
