@@ -19,8 +19,10 @@
 // The update of p uses m' and v' before they are rounded.
 //
 // Bound by memory: per element 8 B of p, 4 (2) of g, and 16 B of f32 moments or 4.1 B of 8-bit ones.  34 M f32
-// elements with a bf16 copy, into other buffers: 190 us at 5.4 TB/s with f32 moments; 1e8 in place 548 us (5.5 TB/s), with
-// 8-bit moments 340 us (5.3 TB/s; a large copy reaches 4.8); 500,000 elements 5.0 and 5.6 us, where the launch is what counts.
+// elements with a bf16 copy, into other buffers: 189 us at 5.4 TB/s with f32 moments; 1e8 in place 548 us (5.5 TB/s), with
+// 8-bit moments 338 us (5.3 TB/s; a large copy reaches 4.8).  500,000 elements: a kernel of 5.7 and 6.7 us (rocprofv3; 5.0 and 5.6
+// apart in a graph), of which memory would take 2.9 and 1.5: latency, of the chain work item -> descriptor -> data and of the
+// step's constants, which every thread computes in f64.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -387,9 +389,12 @@ extern "C" int llp_adamw_step(const llp_adamw_desc* descs, int n_tensors, const 
   LLP_CHECK_ARG(descs && work && step, "llp_adamw_step: null pointer");
   const AdamWArgs a{lr, beta1, beta2, eps, weight_decay, max_norm, seed};
   // Large steps: params, gradients and copies pass by the caches, which the moments then keep to themselves.  f32 moments
-  // of more than 16 M elements, with a workgroup for every item: 2e7 elements 107 -> 94 us, 4e7 236 -> 214, 1e8 589 -> 548 (1e7
-  // would go from 46 to 50).  8-bit ones of more than 32 M, in 4,096 workgroups as always, for the step's constants and the
-  // rounding take longer (1e8 340, one an item 347): 4e7 148 -> 138, 1e8 367 -> 340 (2e7 would go from 64 to 70).
+  // of more than 16 M elements, with a workgroup for every item: 2e7 elements 107 -> 96 us, 4e7 229 -> 222, 1e8 in place 589 -> 548
+  // (1e7 would go from 46 to 50).  8-bit ones of more than 32 M, in 4,096 workgroups as always, for the step's constants and the
+  // rounding take longer (1e8 340, one an item 347): 4e7 151 -> 140, 1e8 369 -> 340 (2e7 would go from 64 to 70).  With what reads
+  // the params or the copies next the gain stays: the transposed copies' launch, f32 moments 2e7 136 -> 134, 4e7 296 -> 294, 1e8 826 ->
+  // 769, 8-bit 4e7 215 -> 203, 1e8 620 -> 560; a read of the bf16 copy, f32 2e7 132 -> 110, 4e7 260 -> 260, 1e8 621 -> 625, 8-bit 4e7
+  // 182 -> 171, 1e8 444 -> 446.
   const unsigned grid = state_bits == 32 && n_work > 8192 ? (unsigned)std::min<int64_t>(n_work, 1 << 20) : aw_grid(n_work);
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, descs, work, n_work, sumsq, a, step);

@@ -1197,8 +1197,9 @@ extern "C" int llp_gemm_nt_mx4(int64_t M, int64_t N, int64_t K, int a_dtype, con
   //     262144 x 2048 x 2048 657 / 845);
   //   else tiled, 64 x 128 while that makes one workgroup a CU (two for K <= 2048, where latency counts): 1024 x 2048 x 2048
   //     9.1, 128 x 128 10.2, 4096 rows 21.1 / 18.1; 8192 x 8415 -> 256 26.4 / 29.6, 12288 rows 37.3 / 30.6;
-  //   128 x 128 then, and 128 x 256, where it fits the columns, for long K (262144 x 8415 -> 256 474, 128 x 128 523; 16384 rows
-  //     47.8 / 32.3) and for a bf16 C past the caches (235868 x 128 -> 1024 120 / 137; 235868 x 128 -> 256 27.2 / 23.6).
+  //   128 x 128 then, and 128 x 256, where it fits the columns, for long K in no whole steps of 256 (262144 x 8500 -> 256 541,
+  //     128 x 128 625; 8192 x 4200 -> 1024, 256 tiles, 31.1 / 32.5; 33000 x 8500 -> 256, 258 of them, 90.6 / 84.8; 16384 rows, 128 of
+  //     them, 50.5 / 35.9) and for a bf16 C past the caches (235868 x 128 -> 1024 120 / 137; 235868 x 128 -> 256 27.2 / 23.6).
   const bool near = W->ld_codes < (1 << 23) && (!A4 || A4->ld_codes < (1 << 23));
   auto tiles = [&](int64_t rows, int64_t cols) { return (M + rows - 1) / rows * ((n_out + cols - 1) / cols); };
   if (A4 && near && tiles(32, 32) > 512) {

@@ -15,6 +15,8 @@ head is one reduction kernel.  Chunks of ``chunk`` edges bound the scratch.
 dtype "mxfp4": the student answers in 4 bits (llp_mx).  Node features, pair products and hidden
 activations are quantised (a hidden layer hands MXFP4 rows to the next), weights too; embeddings are
 bf16 and the Linear(H, 1) head works on the last hidden layer in bf16.
+Every call quantises the weights anew, so MXFP4 pays for many edges or nodes: 262,144 edges of 1,024-wide embeddings through
+one hidden layer 0.90 ms (bf16 1.44), two 1.08 (1.87), two of 2,048 2.6 (5.9); one edge at width 256 53 us (bf16 43).
 """
 from __future__ import annotations
 

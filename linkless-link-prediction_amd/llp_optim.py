@@ -283,7 +283,13 @@ class AdamW(torch.optim.Optimizer):
     is; the update number is the group's, so params that step together must always have done so (refused
     else).  After a first eager step on the same gradients' storage ``step()`` can be captured into a
     graph (``zero_grad(set_to_none=False)``); a graph keeps the hyper-parameters and the state that were
-    there, so ``load_state_dict`` asks for a new capture."""
+    there, so ``load_state_dict`` asks for a new capture.
+
+    The kernel works from a table of addresses, which lasts while params, gradients and state stay where
+    they are.  Gradients elsewhere, as after ``zero_grad()``, take a new table and a device synchronisation, some
+    0.3 ms a step: in a loop of short steps keep them (``zero_grad(set_to_none=False)``).  A student of 0.4 M
+    params on 512 rows, forward, backward and step: 496 us with the gradients kept, 786 without
+    (torch.optim.AdamW 694 and 645, fused 523 and 556)."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
         if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and 0 <= betas[0] < 1 and 0 <= betas[1] < 1):
