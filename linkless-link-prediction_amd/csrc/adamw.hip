@@ -276,7 +276,12 @@ __global__ __launch_bounds__(256) void adamw_kernel(const llp_adamw_desc* __rest
       p[i] = p[i] * keep - size * (m[i] / (r[i] * inv_bc2 + eps));
     }
     store8<ONCE>((P*)d.param_out, e, n, p);
-    if (d.copy) store_copy<ONCE>(d, e, n, p);
+    if (d.copy) {
+      if constexpr (sizeof(P) == 2)   // an f32 copy of a bf16 param holds the param, as the transposed one does
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = bf2f(f2bf(p[i]));
+      store_copy<ONCE>(d, e, n, p);
+    }
     if constexpr (BITS == 32) {
       store8<false>((float*)d.exp_avg_out, e, n, m);
       store8<false>((float*)d.exp_avg_sq_out, e, n, v);
