@@ -420,3 +420,7 @@ class AdamW(torch.optim.Optimizer):
             if k in state_dict["state"]:
                 for name, v in state_dict["state"][k].items():
                     self.state[p][name] = v.detach().clone() if name == "step" else v.detach().clone().to(p.device)
+                if self.state_bits == 8 and "exp_avg" in self.state[p]:
+                    # a second moment of 0 beside a first one that is not, as a step does not leave them: its least code
+                    m, r = self.state[p]["exp_avg"], self.state[p]["exp_avg_sq"]
+                    r[(r == 0) & ((m & 127) != 0)] = 1

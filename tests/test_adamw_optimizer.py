@@ -136,3 +136,15 @@ def test_gradients_are_not_kept(monkeypatch):
     opt = llp_optim.AdamW([p])
     opt.step()
     assert len(made) == 1 and made[0]() is None
+
+
+def test_loaded_second_moments_are_not_0_beside_first_ones():
+    p = torch.nn.Parameter(torch.zeros(6))
+    opt = llp_optim.AdamW([p], state_bits=8)
+    opt.init_state(p)
+    sd = opt.state_dict()
+    sd["state"][0]["exp_avg"] = torch.tensor([0, 5, 128, 133, 7, 0], dtype=torch.uint8)       # (128: -0)
+    sd["state"][0]["exp_avg_sq"] = kept = torch.tensor([0, 0, 0, 0, 9, 4], dtype=torch.uint8)
+    opt.load_state_dict(sd)
+    assert opt.state[p]["exp_avg_sq"].tolist() == [0, 1, 0, 1, 9, 4] and kept.tolist() == [0, 0, 0, 0, 9, 4]
+    assert opt.state[p]["exp_avg"].tolist() == [0, 5, 128, 133, 7, 0]
