@@ -630,7 +630,8 @@ def main():
             res["fp32_step"] = fp32_step(data, a, t_h, init, dev)
         if not opt.no_sage:
             res["sage_aggregate"] = sage_aggregate(data, dev)
-            res["sage_teacher_step"] = sage_teacher_step(data, dev, opt.dtype)
+            if world == 1:      # (its engine's collectives need every rank, and this is rank 0 alone)
+                res["sage_teacher_step"] = sage_teacher_step(data, dev, opt.dtype)
         if world == 1 and not opt.no_physics:
             res["physics_production_step"] = physics_production_step(opt.dtype)
         if world == 1 and not opt.no_cpu_baseline:
