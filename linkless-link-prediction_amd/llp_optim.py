@@ -352,6 +352,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        moments = ("exp_avg", "exp_avg_sq") + (("exp_avg_scale", "exp_avg_sq_scale") if self.state_bits == 8 else ())
         for i, group in enumerate(self.param_groups):
             params = [p for p in group["params"] if p.grad is not None]
             if not params:
@@ -361,7 +362,7 @@ class AdamW(torch.optim.Optimizer):
                 raise RuntimeError("AdamW: dense gradients only")
             # all that the table took from these tensors: where they and the moments lie, types and layouts
             where = tuple((p.data_ptr(), g.data_ptr(), p.numel(), p.dtype, g.dtype, p.is_contiguous(), g.is_contiguous(),
-                           *(t.data_ptr() for k, t in self.init_state(p).items() if k != "step"))
+                           *(self.init_state(p)[k].data_ptr() for k in moments))
                           for p, g in zip(params, grads))
             at = self._tables.get(i)
             capturing = params[0].is_cuda and torch.cuda.is_current_stream_capturing()

@@ -55,7 +55,9 @@ def test_replaced_state_is_another_table(tables, bits):
     p = torch.nn.Parameter(torch.zeros(6, 6))
     opt = llp_optim.AdamW([p], state_bits=bits)
     p.grad = torch.randn(6, 6)
+    opt.init_state(p)["note"] = "a user's own entry"
     opt.step()
+    del opt.state[p]["note"]
     for n, name in enumerate(k for k in list(opt.state[p]) if k != "step"):
         opt.state[p][name] = opt.state[p][name].clone()
         opt.step()
